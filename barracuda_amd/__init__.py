@@ -8,12 +8,13 @@ from .error import (BarracudaError, CastOverflow, DeviceError, DeviceLost, Devic
                     ExecutionError, InvalidInput, InvalidOperation, InvalidShape, OutOfMemory,
                     ShapeMismatch, UnsupportedOperation)
 from . import ipc, linalg, nn
+from .kv_cache import KvCache, KvStep
 from .linalg import F64Buffer, GemmCachedF64, GemmF64
 from .nn import Activation, fused_mlp
 from .session import AttentionDims, SessionTensor, TensorSession
 from .tensor import (GELU, Attention, BatchMatMul, CausalAttention, FlashAttention, GroupedQueryAttention,
                      HipDevice, LayerNorm, LcgStream, MatMul, MatmulTiled, MultiHeadAttention, ReLU,
-                     ScaledDotProductAttention, Softmax, Tensor, get_device)
+                     ScaledDotProductAttention, SlidingWindowAttention, Softmax, Tensor, get_device)
 
 __all__ = [
     "BarracudaError", "CastOverflow", "DeviceError", "DeviceLost", "DeviceNotAvailable",
@@ -22,6 +23,6 @@ __all__ = [
     "Activation", "fused_mlp", "nn", "linalg", "ipc", "F64Buffer", "GemmCachedF64", "GemmF64",
     "Attention", "BatchMatMul", "CausalAttention", "FlashAttention", "GroupedQueryAttention", "HipDevice",
     "MatMul", "MultiHeadAttention",
-    "MatmulTiled", "ScaledDotProductAttention", "Softmax", "Tensor", "get_device", "LcgStream",
-    "ReLU", "GELU", "LayerNorm",
+    "MatmulTiled", "ScaledDotProductAttention", "SlidingWindowAttention", "Softmax", "Tensor", "get_device", "LcgStream",
+    "ReLU", "GELU", "LayerNorm", "KvCache", "KvStep",
 ]

@@ -41,6 +41,17 @@ class AttnLayout(C.Structure):
     _fields_ = [("batch_stride", C.c_longlong), ("head_stride", C.c_longlong), ("row_stride", C.c_longlong)]
 
 
+class KvPages(C.Structure):
+    """bch_kv_pages: one layer of a paged key/value cache."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_layout", AttnLayout), ("v_layout", AttnLayout), ("num_pages", _i),
+                ("page_size", _i), ("Hkv", _i), ("D", _i), ("table", _vp), ("table_width", _i)]
+
+
+class KvBatch(C.Structure):
+    """bch_kv_batch: the sequences of a call and their new tokens."""
+    _fields_ = [("B", _i), ("total", _i), ("max_new", _i), ("max_len", _i), ("start", _vp), ("len", _vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "bch_device_count": (_i, [C.POINTER(_i)]),
@@ -77,6 +88,13 @@ SIGNATURES = {
     "bch_sdpa_fwd": (_i, [_vp, _i, _i, _i, _i, _i, _f, _i, _vp, _vp, _vp, _vp]),
     "bch_sdpa_fwd_ex": (_i, [_vp, _i, _i, _i, _i, _i, _i, _f, _i, _vp, AttnLayout, _vp, AttnLayout, _vp,
                              AttnLayout, _vp, AttnLayout]),
+    "bch_sdpa_paged": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _i, _f, _i, _i, _vp, _vp, AttnLayout, _vp,
+                            AttnLayout]),
+    "bch_sdpa_window": (_i, [_vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, AttnLayout, _vp, AttnLayout, _vp,
+                             AttnLayout, _vp, AttnLayout]),
+    "bch_kv_append": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, AttnLayout, _vp, AttnLayout]),
+    "bch_kv_copy_pages": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, C.POINTER(_i), C.POINTER(_i)]),
+    "bch_kv_keep": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, _i, _vp, _vp, _vp]),
     "bch_launch_code_object": (_i, [_vp, _vp, _sz, C.c_char_p, C.POINTER(C.c_uint),
                                     C.POINTER(C.c_uint), C.POINTER(_vp), _sz, _sz]),
     "bch_event_create": (_i, [_vp, C.POINTER(_vp)]),

@@ -15,6 +15,7 @@
 #include <stdlib.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <map>
 #include <mutex>
@@ -26,6 +27,7 @@
 
 #include "../../include/barracuda_hip.h"
 #include "bch_internal.h"
+#include "paged.h"
 
 // Fixed scratch of bch_sgemm_noalloc (no hipMalloc on that path): the
 // skinny GEMM's split-k partials.  Each device that loads the library holds
@@ -868,6 +870,203 @@ bch_status bch_sdpa_fwd_ex(bch_ctx* ctx, int B, int H, int Hkv, int Sq, int Skv,
   s.v = {vl.batch_stride, vl.head_stride, vl.row_stride};
   s.o = {ol.batch_stride, ol.head_stride, ol.row_stride};
   return sdpa_run(ctx, B, H, Hkv, Sq, Skv, D, scale, causal, q, k, v, o, s);
+}
+
+namespace {
+
+constexpr int kPagedMaxD = 1024;
+
+bool bad_layout(const bch_attn_layout& l, int D) {
+  return l.batch_stride < 0 || l.head_stride < 0 || l.row_stride < D;
+}
+bch::SdpaLayout layout(const bch_attn_layout& l) { return {l.batch_stride, l.head_stride, l.row_stride}; }
+
+bch_status check_layout(bch_ctx* ctx, const char* op, const char* what, const bch_attn_layout& l, int D) {
+  if (!bad_layout(l, D)) return BCH_OK;
+  return fail(ctx, BCH_E_INVALID,
+              "%s: %s layout (batch %lld, head %lld, row %lld) needs non-negative strides and row stride >= D = %d", op,
+              what, l.batch_stride, l.head_stride, l.row_stride, D);
+}
+
+// What the cache's calls have in common; pointers are looked at after the shapes, and after ctx.
+bch_status check_pages(bch_ctx* ctx, const char* op, const bch_kv_pages* kv, bool table) {
+  if (!kv) return fail(ctx, BCH_E_INVALID, "%s: pages are NULL", op);
+  if (kv->num_pages < 1 || kv->page_size < 1 || kv->Hkv < 1 || kv->D < 1 || (table && kv->table_width < 1))
+    return fail(ctx, BCH_E_SHAPE, "%s: empty dimension (num_pages=%d, page_size=%d, Hkv=%d, D=%d, table_width=%d)", op,
+                kv->num_pages, kv->page_size, kv->Hkv, kv->D, kv->table_width);
+  bch_status st = check_layout(ctx, op, "k", kv->k_layout, kv->D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "v", kv->v_layout, kv->D);
+  return st;
+}
+bch_status check_batch(bch_ctx* ctx, const char* op, const bch_kv_batch* batch) {
+  if (!batch) return fail(ctx, BCH_E_INVALID, "%s: batch is NULL", op);
+  if (batch->B < 0 || batch->total < 0 || batch->max_new < 0 || batch->max_len < 0)
+    return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (B=%d, total=%d, max_new=%d, max_len=%d)", op, batch->B,
+                batch->total, batch->max_new, batch->max_len);
+  return BCH_OK;
+}
+bch_status check_layers(bch_ctx* ctx, const char* op, const bch_kv_pages* kv, int layers, long long k_stride,
+                        long long v_stride) {
+  if (layers < 0 || k_stride < 0 || v_stride < 0)
+    return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (layers=%d, strides %lld, %lld)", op, layers, k_stride,
+                v_stride);
+  return BCH_OK;
+}
+
+bch::KvPages pages_of(const bch_kv_pages& kv) {
+  bch::KvPages p;
+  p.k = kv.k;
+  p.v = kv.v;
+  p.kl = layout(kv.k_layout);
+  p.vl = layout(kv.v_layout);
+  p.num_pages = kv.num_pages;
+  p.table = kv.table;
+  p.width = kv.table_width;
+  bch::set_page_size(p, kv.page_size);
+  return p;
+}
+bch::KvSeqs seqs_of(const bch_kv_batch& b) { return {b.start, b.len, b.total, std::min(b.max_new, b.total), 0}; }
+
+bch_status paged_run(bch_ctx* ctx, const bch::PagedCall& c, int max_len) {
+  bch_status st = use(ctx);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx, bch::launch_sdpa_paged(ctx->stream, c), "attention launch");
+}
+
+}  // namespace
+
+bch_status bch_sdpa_paged(bch_ctx* ctx, const bch_kv_pages* kv, const bch_kv_batch* batch, int H, float scale,
+                          int window, int sinks, const int* parent, const float* q, bch_attn_layout ql, float* o,
+                          bch_attn_layout ol) {
+  const char* op = "paged attention";
+  bch_status st = check_pages(ctx, op, kv, true);
+  if (st == BCH_OK) st = check_batch(ctx, op, batch);
+  if (st != BCH_OK) return st;
+  if (H < 1) return fail(ctx, BCH_E_SHAPE, "%s: empty dimension (H=%d)", op, H);
+  if (H % kv->Hkv != 0)
+    return fail(ctx, BCH_E_INVALID, "num_q_heads (%d) must be divisible by num_kv_heads (%d)", H, kv->Hkv);
+  if (window < 0 || sinks < 0)
+    return fail(ctx, BCH_E_INVALID, "%s: window (%d) and sinks (%d) must not be negative", op, window, sinks);
+  st = check_layout(ctx, op, "q", ql, kv->D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "o", ol, kv->D);
+  if (st != BCH_OK) return st;
+  if (kv->D > kPagedMaxD) return fail(ctx, BCH_E_UNSUPPORTED, "%s: head dimension %d > %d", op, kv->D, kPagedMaxD);
+  const int max_new = std::min(batch->max_new, batch->total);
+  if (parent && max_new > bch::kMaxDrafts)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d drafts in one tree, at most %d", op, max_new, bch::kMaxDrafts);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (batch->B == 0 || max_new == 0) return BCH_OK;
+  if (!kv->k || !kv->v || !kv->table || !batch->start || !batch->len || !q || !o)
+    return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  bch::PagedCall c{batch->B, H, kv->Hkv, kv->D, scale * 1.44269504088896340736f, window, sinks, parent, pages_of(*kv),
+                   seqs_of(*batch), q, o, layout(ql), layout(ol)};
+  c.ql.batch = c.ol.batch = 0;
+  return paged_run(ctx, c, batch->max_len);
+}
+
+bch_status bch_sdpa_window(bch_ctx* ctx, int B, int H, int Hkv, int Sq, int Skv, int D, float scale, int window,
+                           int sinks, const float* q, bch_attn_layout ql, const float* k, bch_attn_layout kl,
+                           const float* v, bch_attn_layout vl, float* o, bch_attn_layout ol) {
+  const char* op = "window attention";
+  if (B < 1 || H < 1 || Hkv < 1 || Sq < 1 || Skv < 1 || D < 1)
+    return fail(ctx, BCH_E_SHAPE, "%s: empty dimension (B=%d, H=%d, Hkv=%d, Sq=%d, Skv=%d, D=%d)", op, B, H, Hkv, Sq,
+                Skv, D);
+  if (H % Hkv != 0)
+    return fail(ctx, BCH_E_INVALID, "num_q_heads (%d) must be divisible by num_kv_heads (%d)", H, Hkv);
+  if (window < 0 || sinks < 0)
+    return fail(ctx, BCH_E_INVALID, "%s: window (%d) and sinks (%d) must not be negative", op, window, sinks);
+  bch_status st = check_layout(ctx, op, "q", ql, D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "k", kl, D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "v", vl, D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "o", ol, D);
+  if (st != BCH_OK) return st;
+  if (D > kPagedMaxD) return fail(ctx, BCH_E_UNSUPPORTED, "%s: head dimension %d > %d", op, D, kPagedMaxD);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (!q || !k || !v || !o) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  bch::KvPages p{k, v, layout(kl), layout(vl), B, 0, 0, 0, nullptr, 1};
+  bch::set_page_size(p, Skv);
+  return paged_run(ctx,
+                   bch::PagedCall{B, H, Hkv, D, scale * 1.44269504088896340736f, window, sinks, nullptr, p,
+                                  bch::KvSeqs{nullptr, nullptr, 0, Sq, Skv}, q, o, layout(ql), layout(ol)},
+                   Skv);
+}
+
+bch_status bch_kv_append(bch_ctx* ctx, const bch_kv_pages* kv, const bch_kv_batch* batch, const float* k,
+                         bch_attn_layout kl, const float* v, bch_attn_layout vl) {
+  const char* op = "kv_append";
+  bch_status st = check_pages(ctx, op, kv, true);
+  if (st == BCH_OK) st = check_batch(ctx, op, batch);
+  if (st == BCH_OK) st = check_layout(ctx, op, "new k", kl, kv->D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "new v", vl, kv->D);
+  if (st != BCH_OK) return st;
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (batch->B == 0 || batch->total == 0 || batch->max_new == 0) return BCH_OK;
+  if (!kv->k || !kv->v || !kv->table || !batch->start || !batch->len || !k || !v)
+    return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx,
+                  bch::launch_kv_append(ctx->stream, pages_of(*kv), kv->k, kv->v, seqs_of(*batch), batch->B, kv->Hkv,
+                                        kv->D, k, layout(kl), v, layout(vl)),
+                  "kv_append launch");
+}
+
+bch_status bch_kv_copy_pages(bch_ctx* ctx, const bch_kv_pages* kv, int layers, long long k_layer_stride,
+                             long long v_layer_stride, int n, const int* src, const int* dst) {
+  const char* op = "kv_copy_pages";
+  bch_status st = check_pages(ctx, op, kv, false);
+  if (st == BCH_OK) st = check_layers(ctx, op, kv, layers, k_layer_stride, v_layer_stride);
+  if (st != BCH_OK) return st;
+  if (n < 0) return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (n=%d)", op, n);
+  if (n > 0 && (!src || !dst)) return fail(ctx, BCH_E_INVALID, "%s: NULL page list", op);
+  if (n > 0) {
+    // a bit for every page that is written
+    unsigned char* to = static_cast<unsigned char*>(calloc(((size_t)kv->num_pages + 7) / 8, 1));
+    if (!to) return fail(ctx, BCH_E_OOM, "%s: no host memory to check %d pages", op, kv->num_pages);
+    for (int x = 0; x < n && st == BCH_OK; ++x) {
+      if (src[x] < 0 || src[x] >= kv->num_pages || dst[x] < 0 || dst[x] >= kv->num_pages)
+        st = fail(ctx, BCH_E_INVALID, "%s: copy %d (page %d to %d) is outside the %d pages", op, x, src[x], dst[x],
+                  kv->num_pages);
+      else if (to[dst[x] >> 3] & (1 << (dst[x] & 7)))
+        st = fail(ctx, BCH_E_INVALID, "%s: two copies into page %d", op, dst[x]);
+      else
+        to[dst[x] >> 3] |= 1 << (dst[x] & 7);
+    }
+    for (int x = 0; x < n && st == BCH_OK; ++x)
+      if (to[src[x] >> 3] & (1 << (src[x] & 7)))
+        st = fail(ctx, BCH_E_INVALID, "%s: page %d is both read and written", op, src[x]);
+    free(to);
+    if (st != BCH_OK) return st;
+  }
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (n == 0 || layers == 0) return BCH_OK;
+  if (!kv->k || !kv->v) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx,
+                  bch::launch_kv_copy_pages(ctx->stream, pages_of(*kv), kv->k, kv->v, layers, k_layer_stride,
+                                            v_layer_stride, kv->Hkv, kv->D, n, src, dst),
+                  "kv_copy_pages launch");
+}
+
+bch_status bch_kv_keep(bch_ctx* ctx, const bch_kv_pages* kv, int layers, long long k_layer_stride,
+                       long long v_layer_stride, int B, int total, const int* start, const int* keep, const int* to) {
+  const char* op = "kv_keep";
+  bch_status st = check_pages(ctx, op, kv, true);
+  if (st == BCH_OK) st = check_layers(ctx, op, kv, layers, k_layer_stride, v_layer_stride);
+  if (st != BCH_OK) return st;
+  if (B < 0 || total < 0) return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (B=%d, total=%d)", op, B, total);
+  if (B > 65535 || layers > 32767)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d sequences (at most 65535) of %d layers (at most 32767)", op, B, layers);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (B == 0 || total == 0 || layers == 0) return BCH_OK;
+  if (!kv->k || !kv->v || !kv->table || !start || !keep || !to) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx,
+                  bch::launch_kv_keep(ctx->stream, pages_of(*kv), kv->k, kv->v, layers, k_layer_stride, v_layer_stride,
+                                      kv->Hkv, kv->D, B, total, start, keep, to),
+                  "kv_keep launch");
 }
 
 bch_status bch_fill_uniform(bch_ctx* ctx, float* dst, size_t n, unsigned long long* state, double lo,

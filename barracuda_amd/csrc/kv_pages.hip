@@ -1,0 +1,237 @@
+// kv_pages.hip -- what writes a paged key/value cache (paged.h): new tokens appended, whole pages
+// copied, keys moved down within their sequences.  The reference has no cache; these stand beside its
+// attention ops as bch_copy and the head permutations do.
+//
+// All three only move data: 16 bytes of K and V a column read and written, so HBM bounds the large
+// calls and the launch the small ones.  Rows go as 16-byte accesses where D, the strides and the
+// pointers allow (VEC 4), else as single floats.
+#include "paged.h"
+
+#include <algorithm>
+
+namespace {
+
+using bch::KvPages;
+using bch::KvSeqs;
+using bch::SdpaLayout;
+
+constexpr int kThreads = 256;
+
+template <int VEC>
+struct Elem;
+template <>
+struct Elem<1> {
+  typedef float type;
+};
+template <>
+struct Elem<4> {
+  typedef bch::f32x4 type;
+};
+
+// ---- append: row i of sequence b is key len[b] - n + i ----
+// A workgroup takes kAppend tokens of one sequence; a thread the same columns of each, K and V, with
+// all of its loads ahead of its stores.
+constexpr int kAppend = 4;
+
+template <int VEC>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* k, float* v, KvSeqs seqs, int tiles,
+                                                             int Hkv, int D, const float* __restrict__ nk,
+                                                             SdpaLayout nkl, const float* __restrict__ nv,
+                                                             SdpaLayout nvl) {
+  typedef typename Elem<VEC>::type T;
+  const int b = blockIdx.x / tiles, i0 = (blockIdx.x % tiles) * kAppend;
+  const bch::Seq s = bch::load_seq(kv, seqs, b);
+  if (i0 >= s.n) return;
+  bch::Slot slot[kAppend];
+#pragma unroll
+  for (int u = 0; u < kAppend; ++u) {
+    const int j = s.first + i0 + u;
+    slot[u] = i0 + u < s.n && j >= 0 ? bch::key_slot(kv, b, j) : bch::Slot{-1, 0};
+  }
+  const int dv = D / VEC;
+  for (int e = threadIdx.x; e < Hkv * dv; e += kThreads) {
+    const int h = e / dv, d = (e - h * dv) * VEC;
+    T x[kAppend], y[kAppend];
+#pragma unroll
+    for (int u = 0; u < kAppend; ++u) {
+      const long long row = s.row0 + min(i0 + u, s.n - 1);
+      x[u] = *reinterpret_cast<const T*>(nk + row * nkl.row + h * nkl.head + d);
+      y[u] = *reinterpret_cast<const T*>(nv + row * nvl.row + h * nvl.head + d);
+    }
+#pragma unroll
+    for (int u = 0; u < kAppend; ++u)
+      if (slot[u].page >= 0) {
+        *reinterpret_cast<T*>(k + bch::slot_offset(kv.kl, slot[u]) + h * kv.kl.head + d) = x[u];
+        *reinterpret_cast<T*>(v + bch::slot_offset(kv.vl, slot[u]) + h * kv.vl.head + d) = y[u];
+      }
+  }
+}
+
+// ---- copy of whole pages ----
+// The pairs travel as kernel arguments: a captured graph holds them, and no copy of them to the device
+// is waited for.  A page is [n1][n2][run] floats with strides s1, s2 (merged where they are dense).
+constexpr int kPairs = 480;
+struct Pairs {
+  int src[kPairs], dst[kPairs];
+};
+struct PageShape {
+  float* base;
+  long long page, layer, s1, s2;
+  int n2;
+  long long run, total;  // floats
+};
+
+template <int VEC>
+__global__ __launch_bounds__(kThreads) void kv_copy_kernel(PageShape ks, PageShape vs, Pairs pairs) {
+  typedef typename Elem<VEC>::type T;
+  constexpr int U = 4;
+  const PageShape& p = blockIdx.z & 1 ? vs : ks;
+  float* base = p.base + (blockIdx.z >> 1) * p.layer;
+  const float* src = base + pairs.src[blockIdx.y] * p.page;
+  float* dst = base + pairs.dst[blockIdx.y] * p.page;
+  T x[U];
+  long long off[U];
+  const long long e0 = ((long long)blockIdx.x * U * kThreads + threadIdx.x) * VEC;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const long long e = e0 + (long long)u * kThreads * VEC;
+    off[u] = -1;
+    if (e < p.total) {
+      const long long r = e / p.run;
+      off[u] = (r / p.n2) * p.s1 + (r % p.n2) * p.s2 + (e - r * p.run);
+      x[u] = *reinterpret_cast<const T*>(src + off[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+    if (off[u] >= 0) *reinterpret_cast<T*>(dst + off[u]) = x[u];
+}
+
+PageShape page_shape(float* base, const SdpaLayout& l, long long layer, int Hkv, int page_size, int D) {
+  PageShape p{base, l.batch, layer, l.head, l.row, page_size, D, (long long)Hkv * page_size * D};
+  int n1 = Hkv;
+  if (p.s1 < p.s2) {  // heads inside keys
+    std::swap(p.s1, p.s2);
+    std::swap(n1, p.n2);
+  }
+  if (p.s2 == p.run || p.n2 == 1) {
+    p.run *= p.n2;
+    p.n2 = n1;
+    p.s2 = p.s1;
+    p.s1 = 0;
+    if (p.s2 == p.run || p.n2 == 1) {
+      p.run *= p.n2;
+      p.n2 = 1;
+      p.s2 = 0;
+    }
+  }
+  return p;
+}
+
+// ---- keep: key to[b] + i = key keep[start[b] + i] ----
+// A thread owns its columns of a sequence's keys and moves them in ascending i, kKeep at a time, so
+// that a key is read before a later one of the same call takes its place (keep ascends and no key moves
+// up: to[b] + i <= keep[i] < keep[i + 1]).
+constexpr int kKeep = 8;
+
+template <int VEC>
+__global__ __launch_bounds__(kThreads) void kv_keep_kernel(KvPages kv, float* k, float* v, long long k_layer,
+                                                           long long v_layer, int Hkv, int D, int total,
+                                                           const int* start, const int* keep, const int* to) {
+  typedef typename Elem<VEC>::type T;
+  const int b = blockIdx.y;
+  const bool is_v = blockIdx.z & 1;
+  const SdpaLayout& l = is_v ? kv.vl : kv.kl;
+  float* base = (is_v ? v : k) + (blockIdx.z >> 1) * (is_v ? v_layer : k_layer);
+  const int a = min(max(start[b], 0), total), n = min(max(start[b + 1], a), total) - a;
+  const int t0 = to[b], dv = D / VEC;
+  const int e = blockIdx.x * kThreads + threadIdx.x;
+  if (e >= Hkv * dv) return;
+  float* col = base + (e / dv) * l.head + (e % dv) * VEC;
+  for (int i0 = 0; i0 < n; i0 += kKeep) {
+    T x[kKeep];
+    bch::Slot dst[kKeep];
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u) {
+      const int i = min(i0 + u, n - 1), j = keep[a + i];
+      const long long to_j = (long long)t0 + i;
+      const bool on = i0 + u < n && j > to_j && to_j >= 0;
+      const bch::Slot src = on ? bch::key_slot(kv, b, j) : bch::Slot{-1, 0};
+      dst[u] = src.page >= 0 ? bch::key_slot(kv, b, (int)to_j) : src;
+      if (dst[u].page >= 0) x[u] = *reinterpret_cast<const T*>(col + bch::slot_offset(l, src));
+    }
+#pragma unroll
+    for (int u = 0; u < kKeep; ++u)
+      if (dst[u].page >= 0) *reinterpret_cast<T*>(col + bch::slot_offset(l, dst[u])) = x[u];
+  }
+}
+
+bool mult4(const SdpaLayout& l) { return l.batch % 4 == 0 && l.head % 4 == 0 && l.row % 4 == 0; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool vec4(const KvPages& kv, const float* k, const float* v, int D) {
+  return D % 4 == 0 && aligned16(k) && aligned16(v) && mult4(kv.kl) && mult4(kv.vl);
+}
+
+}  // namespace
+
+namespace bch {
+
+hipError_t launch_kv_append(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B, int Hkv,
+                            int D, const float* nk, const SdpaLayout& nkl, const float* nv, const SdpaLayout& nvl) {
+  const int tiles = (seqs.max_new + kAppend - 1) / kAppend;
+  if ((long long)tiles * B > 0x7fffffffLL || (long long)Hkv * D > 0x7fffffffLL - kThreads)
+    return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)(tiles * B)), block(kThreads);
+  if (vec4(kv, k, v, D) && aligned16(nk) && aligned16(nv) && nkl.row % 4 == 0 && nkl.head % 4 == 0 &&
+      nvl.row % 4 == 0 && nvl.head % 4 == 0)
+    hipLaunchKernelGGL(kv_append_kernel<4>, grid, block, 0, s, kv, k, v, seqs, tiles, Hkv, D, nk, nkl, nv, nvl);
+  else
+    hipLaunchKernelGGL(kv_append_kernel<1>, grid, block, 0, s, kv, k, v, seqs, tiles, Hkv, D, nk, nkl, nv, nvl);
+  return hipGetLastError();
+}
+
+hipError_t launch_kv_copy_pages(hipStream_t s, const KvPages& kv, float* k, float* v, int layers, long long k_layer,
+                                long long v_layer, int Hkv, int D, int n, const int* src, const int* dst) {
+  const bool vec = vec4(kv, k, v, D) && k_layer % 4 == 0 && v_layer % 4 == 0;
+  const PageShape ks = page_shape(k, kv.kl, k_layer, Hkv, kv.page_size, D);
+  const PageShape vs = page_shape(v, kv.vl, v_layer, Hkv, kv.page_size, D);
+  const long long per = (long long)kThreads * 4 * (vec ? 4 : 1);
+  const long long chunks = (ks.total + per - 1) / per;
+  if (chunks > 0x7fffffffLL / kThreads) return hipErrorInvalidConfiguration;
+  for (int l0 = 0; l0 < layers; l0 += 16384) {
+    const int nl = std::min(layers - l0, 16384);
+    PageShape kl = ks, vl = vs;
+    kl.base += l0 * k_layer;
+    vl.base += l0 * v_layer;
+    for (int p0 = 0; p0 < n; p0 += kPairs) {
+      const int np = std::min(n - p0, kPairs);
+      Pairs pairs;
+      std::copy(src + p0, src + p0 + np, pairs.src);
+      std::copy(dst + p0, dst + p0 + np, pairs.dst);
+      const dim3 grid((unsigned)chunks, np, 2 * nl), block(kThreads);
+      if (vec)
+        hipLaunchKernelGGL(kv_copy_kernel<4>, grid, block, 0, s, kl, vl, pairs);
+      else
+        hipLaunchKernelGGL(kv_copy_kernel<1>, grid, block, 0, s, kl, vl, pairs);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
+  }
+  return hipSuccess;
+}
+
+hipError_t launch_kv_keep(hipStream_t s, const KvPages& kv, float* k, float* v, int layers, long long k_layer,
+                          long long v_layer, int Hkv, int D, int B, int total, const int* start, const int* keep,
+                          const int* to) {
+  const bool vec = vec4(kv, k, v, D) && k_layer % 4 == 0 && v_layer % 4 == 0;
+  const long long cols = (long long)Hkv * D / (vec ? 4 : 1);
+  if (cols > 0x7fffffffLL - kThreads || B > 65535 || layers > 32767) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)((cols + kThreads - 1) / kThreads), B, 2 * layers), block(kThreads);
+  if (vec)
+    hipLaunchKernelGGL(kv_keep_kernel<4>, grid, block, 0, s, kv, k, v, k_layer, v_layer, Hkv, D, total, start, keep, to);
+  else
+    hipLaunchKernelGGL(kv_keep_kernel<1>, grid, block, 0, s, kv, k, v, k_layer, v_layer, Hkv, D, total, start, keep, to);
+  return hipGetLastError();
+}
+
+}  // namespace bch

@@ -37,7 +37,7 @@ from .error import (BarracudaError, DeviceError, DeviceNotAvailable, InvalidInpu
 __all__ = [
     "HipDevice", "get_device", "Tensor", "MatMul", "MatmulTiled", "BatchMatMul",
     "Softmax", "Attention", "ScaledDotProductAttention", "CausalAttention",
-    "FlashAttention", "GroupedQueryAttention", "MultiHeadAttention", "LcgStream",
+    "FlashAttention", "GroupedQueryAttention", "SlidingWindowAttention", "MultiHeadAttention", "LcgStream",
     "ReLU", "GELU", "LayerNorm",
 ]
 
@@ -298,6 +298,9 @@ class Tensor:
 
     def grouped_query_attention(self, key: "Tensor", value: "Tensor") -> "Tensor":
         return GroupedQueryAttention(self, key, value).execute()
+
+    def sliding_window_attention(self, key: "Tensor", value: "Tensor", window: int, sinks: int = 0) -> "Tensor":
+        return SlidingWindowAttention(self, key, value, window, sinks).execute()
 
     def multi_head_attention(self, key: "Tensor", value: "Tensor", w_q: "Tensor", w_k: "Tensor",
                              w_v: "Tensor", w_o: "Tensor", num_heads: int) -> "Tensor":
@@ -646,6 +649,52 @@ class GroupedQueryAttention:
         _sdpa_ex(dev, "grouped_query_attention", b, hq, hkv, s, s, d, False,
                  self.q, _dense(hq, s, d), self.k, _dense(hkv, s, d), self.v, _dense(hkv, s, d),
                  out, _dense(hq, s, d))
+        return out
+
+
+class SlidingWindowAttention:
+    """Causal attention in which a query sees the last `window` keys up to its
+    own (0: all of them) and the first `sinks` keys: Q [B, Hq, Sq, D], K/V
+    [B, Hkv, Skv, D], query head h with key/value head h / (Hq / Hkv), the
+    queries the last Sq positions of the Skv.  A query with no key in sight
+    (Sq > Skv) gives zeros.  The reference has no windowed op; its causal one
+    (ops/causal_attn/mod.rs:64-158) is window 0 with Hq = Hkv and Sq = Skv."""
+
+    def __init__(self, query: Tensor, key: Tensor, value: Tensor, window: int, sinks: int = 0):
+        qs, ks, vs = query.shape(), key.shape(), value.shape()
+        if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
+            raise InvalidInput("All inputs must be 4D tensors [batch, heads, seq_len, head_dim]")
+        if ks[0] != qs[0] or ks[3] != qs[3]:
+            raise ShapeMismatch(qs, ks)
+        if vs != ks:
+            raise ShapeMismatch(ks, vs)
+        if ks[1] == 0 or qs[1] % ks[1] != 0:
+            raise InvalidInput(f"num_q_heads ({qs[1]}) must be divisible by num_kv_heads ({ks[1]})")
+        if window < 0 or sinks < 0:
+            raise InvalidInput(f"window ({window}) and sinks ({sinks}) must not be negative")
+        _same_device(query, key, value)
+        self.q, self.k, self.v = query, key, value
+        self.window, self.sinks = int(window), int(sinks)
+
+    def execute(self) -> Tensor:
+        op = "sliding_window_attention"
+        b, h, sq, d = self.q.shape()
+        hkv, skv = self.k.shape()[1:3]
+        dev = self.q.device()
+        _check_i32(op, dev, batch=b, heads=h, q_len=sq, kv_len=skv, head_dim=d)
+        out = Tensor.empty([b, h, sq, d], dev)
+        if b * h * sq * d == 0:
+            return out
+        if skv == 0:
+            raise InvalidOperation(op, "key sequence is empty (shape/dimension mismatch)")
+        scale = np.float32(1.0) / np.sqrt(np.float32(d))
+        # a window or sinks beyond any position are the same as the largest int
+        window, sinks = min(self.window, _I32_MAX), min(self.sinks, _I32_MAX)
+        with dev._lock:
+            dev.check(dev._lib.bch_sdpa_window(dev.ctx, b, h, hkv, sq, skv, d, float(scale), window, sinks,
+                                               C.c_void_p(self.q.ptr), _dense(h, sq, d), C.c_void_p(self.k.ptr),
+                                               _dense(hkv, skv, d), C.c_void_p(self.v.ptr), _dense(hkv, skv, d),
+                                               C.c_void_p(out.ptr), _dense(h, sq, d)), op)
         return out
 
 

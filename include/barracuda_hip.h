@@ -359,6 +359,110 @@ bch_status bch_sdpa_fwd_ex(bch_ctx *ctx, int B, int H, int Hkv, int Sq,
                            const float *v, bch_attn_layout v_layout,
                            float *o, bch_attn_layout o_layout);
 
+/* ---- attention with a sliding window, and over a paged key/value cache ----
+ * The reference has neither (its causal and grouped-query ops take dense
+ * [B,H,S,D] operands, ops/causal_attn/mod.rs:64-158,
+ * ops/grouped_query_attention/mod.rs:52-147); these stand beside them for
+ * programs that serve sequences token by token. */
+
+/* A paged cache of one layer.  Element (page p, head h, slot i, d) of k is at
+ * p*k_layout.batch_stride + h*k_layout.head_stride + i*k_layout.row_stride + d,
+ * of v alike; a page holds page_size keys (any number from 1 on) of Hkv heads
+ * of D floats.  Key j of sequence b is slot j % page_size of page
+ * table[b*table_width + j/page_size]; the table is device memory, [B]
+ * [table_width].  An entry outside 0 .. num_pages-1 is a page that is not
+ * held: its keys are not read, seen or written.  A sequence has at most
+ * table_width*page_size keys (and 2^31 - 1); a longer length counts as that. */
+typedef struct bch_kv_pages {
+  float *k;
+  float *v;
+  bch_attn_layout k_layout;
+  bch_attn_layout v_layout;
+  int num_pages;
+  int page_size;
+  int Hkv;
+  int D;
+  const int *table;
+  int table_width;
+} bch_kv_pages;
+
+/* The sequences of a call.  start [B+1] and len [B] are device memory, read
+ * when the kernels run (a captured graph reads them at each replay):
+ * sequence b's new tokens are rows start[b] .. start[b+1]-1 of q, o and of an
+ * append's inputs, and the last of its len[b] keys.  The host says how many
+ * rows there are in all (starts are clamped to 0 .. total), the most new
+ * tokens of one sequence (rows beyond max_new are left as they were), and the
+ * most keys of one sequence (max_len: for planning alone; a longer sequence is
+ * computed all the same). */
+typedef struct bch_kv_batch {
+  int B;
+  int total;
+  int max_new;
+  int max_len;
+  const int *start;
+  const int *len;
+} bch_kv_batch;
+
+/* o[row] = softmax(scale q[row] . k_j) v_j over the keys j that the row sees.
+ * Row i of sequence b's n new tokens stands at position p = len[b]-n+i and
+ * sees the keys up to its own.  With `parent` (device, [total]) the n tokens
+ * are a tree of drafts: parent[start[b]+i] is the draft (below i, counted from
+ * the sequence's first; anything else makes i a child of the last committed
+ * token) that i follows; i stands behind it, and sees the len[b]-n committed
+ * keys, its ancestors and itself.  Of those keys, with window > 0, a row sees
+ * the ones less than `window` positions back and the ones at positions below
+ * `sinks`.  A row that sees no key gets zeros; values a row does not see never
+ * reach it, infinite and NaN ones included.  A key whose score is -inf counts as
+ * not seen.  Row r, head h of q is at r*row_stride + h*head_stride (batch_stride
+ * is not used); query head h reads key/value head h / (H / Hkv).  o must not
+ * overlap q, k or v.  D <= 1024; a tree has at most 128 drafts a sequence
+ * (max_new; BCH_E_UNSUPPORTED beyond).  total, max_new or B of 0: nothing
+ * happens. */
+bch_status bch_sdpa_paged(bch_ctx *ctx, const bch_kv_pages *kv,
+                          const bch_kv_batch *batch, int H, float scale,
+                          int window, int sinks, const int *parent,
+                          const float *q, bch_attn_layout q_layout, float *o,
+                          bch_attn_layout o_layout);
+
+/* The same over dense operands (layouts as bch_sdpa_fwd_ex): row i of Sq stands
+ * at position Skv - Sq + i, so with Sq < Skv the queries are the last ones of
+ * their sequence, and with Sq > Skv the first Sq - Skv rows see nothing and get
+ * zeros.  window 0 is causal attention; no tree. */
+bch_status bch_sdpa_window(bch_ctx *ctx, int B, int H, int Hkv, int Sq, int Skv,
+                           int D, float scale, int window, int sinks,
+                           const float *q, bch_attn_layout q_layout,
+                           const float *k, bch_attn_layout k_layout,
+                           const float *v, bch_attn_layout v_layout, float *o,
+                           bch_attn_layout o_layout);
+
+/* The new tokens' keys and values into their pages: row start[b]+i, head h of k
+ * (at r*row_stride + h*head_stride) becomes key len[b]-n+i of sequence b.  A
+ * page that two sequences of the batch share must not get keys from both. */
+bch_status bch_kv_append(bch_ctx *ctx, const bch_kv_pages *kv,
+                         const bch_kv_batch *batch, const float *k,
+                         bch_attn_layout k_layout, const float *v,
+                         bch_attn_layout v_layout);
+
+/* Whole pages copied, K and V: page dst[x] = page src[x] for x < n, in each of
+ * `layers` layers whose pools lie k_layer_stride (v_layer_stride) floats apart
+ * from kv->k (kv->v) on.  src and dst are host memory, read before the call
+ * returns; the table is not used.  A page outside the pool, two copies into one
+ * page, or a page that is both read and written is BCH_E_INVALID. */
+bch_status bch_kv_copy_pages(bch_ctx *ctx, const bch_kv_pages *kv, int layers,
+                             long long k_layer_stride, long long v_layer_stride,
+                             int n, const int *src, const int *dst);
+
+/* Keys moved down in their sequences, K and V of each layer: key to[b]+i of
+ * sequence b = key keep[start[b]+i] for i < start[b+1]-start[b] (the accepted
+ * drafts of a verification step, or what an eviction leaves).  start [B+1],
+ * keep [total] and to [B] are device memory.  A sequence's keep must ascend,
+ * with keep[start[b]+i] >= to[b]+i; keys that would move up, and keys of pages
+ * that are not held, stay.  The pages written must not be shared. */
+bch_status bch_kv_keep(bch_ctx *ctx, const bch_kv_pages *kv, int layers,
+                       long long k_layer_stride, long long v_layer_stride,
+                       int B, int total, const int *start, const int *keep,
+                       const int *to);
+
 /* ---- seeded synthetic inputs, generated in HBM ---- */
 
 /* Fill dst[0..n) from the reference's seeded generators: uniform [lo, hi)
