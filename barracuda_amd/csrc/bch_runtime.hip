@@ -930,7 +930,10 @@ bch::KvSeqs seqs_of(const bch_kv_batch& b) { return {b.start, b.len, b.total, st
 bch_status paged_run(bch_ctx* ctx, const bch::PagedCall& c, int max_len) {
   bch_status st = use(ctx);
   if (st != BCH_OK) return st;
-  return from_hip(ctx, bch::launch_sdpa_paged(ctx->stream, c), "attention launch");
+  // as sdpa_run: the keys are split over workgroups where the workspace holds the partial results
+  st = size_ws(ctx, bch::sdpa_paged_workspace_bytes(c, max_len), 0);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx, bch::launch_sdpa_paged(ctx->stream, c, max_len, ctx->ws, ctx->ws_bytes), "attention launch");
 }
 
 }  // namespace
@@ -981,6 +984,8 @@ bch_status bch_sdpa_window(bch_ctx* ctx, int B, int H, int Hkv, int Sq, int Skv,
   if (st == BCH_OK) st = check_layout(ctx, op, "o", ol, D);
   if (st != BCH_OK) return st;
   if (D > kPagedMaxD) return fail(ctx, BCH_E_UNSUPPORTED, "%s: head dimension %d > %d", op, D, kPagedMaxD);
+  if (Skv > bch::kMaxKeys || Sq > bch::kMaxKeys)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d queries, %d keys, at most %lld", op, Sq, Skv, bch::kMaxKeys);
   if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
   if (!q || !k || !v || !o) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
   bch::KvPages p{k, v, layout(kl), layout(vl), B, 0, 0, 0, nullptr, 1};

@@ -19,6 +19,8 @@ namespace bch {
 
 constexpr int kMaxDrafts = 128;  // rows of one sequence's tree: its ancestor masks are four words
 
+constexpr long long kMaxKeys = 0x7fffff00;  // of a sequence: a block's last key still has a 32-bit number
+
 struct KvPages {
   const float *k, *v;
   SdpaLayout kl, vl;  // (page, head, row) strides
@@ -72,7 +74,7 @@ __device__ __forceinline__ Seq load_seq(const KvPages& kv, const KvSeqs& s, int 
   const int a = min(max(s.start[b], 0), s.total), e = min(max(s.start[b + 1], a), s.total);
   const long long most = (long long)kv.width * kv.page_size;
   r.row0 = a;
-  r.len = (int)min((long long)max(s.len[b], 0), min(most, 0x7fffffffLL));
+  r.len = (int)min((long long)max(s.len[b], 0), min(most, kMaxKeys));
   r.first = r.len - (e - a);
   r.n = min(e - a, s.max_new);
   return r;
@@ -156,7 +158,14 @@ __device__ __forceinline__ void tree_masks(TreeMasks& t, const int* parent, cons
   __syncthreads();
 }
 
-hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c);
+// ws: the results of split keys; with less than sdpa_paged_workspace_bytes it runs unsplit.  max_len:
+// the longest sequence, for the plan.
+hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
+size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
+// 4 <= D <= 256 (sdpa_paged_rows.hip).
+bool sdpa_paged_rows_applies(const PagedCall& c);
+hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
+size_t sdpa_paged_rows_workspace_bytes(const PagedCall& c, int max_len);
 
 // ---- the cache's own calls (kv_pages.hip) ----
 hipError_t launch_kv_append(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B, int Hkv,

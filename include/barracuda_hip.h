@@ -372,7 +372,7 @@ bch_status bch_sdpa_fwd_ex(bch_ctx *ctx, int B, int H, int Hkv, int Sq,
  * table[b*table_width + j/page_size]; the table is device memory, [B]
  * [table_width].  An entry outside 0 .. num_pages-1 is a page that is not
  * held: its keys are not read, seen or written.  A sequence has at most
- * table_width*page_size keys (and 2^31 - 1); a longer length counts as that. */
+ * table_width*page_size keys (and 2^31 - 256); a longer length counts as that. */
 typedef struct bch_kv_pages {
   float *k;
   float *v;
