@@ -15,6 +15,8 @@
 #pragma once
 #include "bch_internal.h"
 
+#include <algorithm>
+
 namespace bch {
 
 constexpr int kMaxDrafts = 128;  // rows of one sequence's tree: its ancestor masks are four words
@@ -158,10 +160,57 @@ __device__ __forceinline__ void tree_masks(TreeMasks& t, const int* parent, cons
   __syncthreads();
 }
 
+// ---- a block of rows and the keys that it reads ----
+// Rows of a sequence and key/value head: token t, query head hk * group + g is row t * group + g.  The keys
+// that any of the tokens t_lo .. t_hi sees, [0, s_hi) and [lo, hi), as a list of n blocks of BLK keys (each
+// starting at a multiple of BLK), the first ns of them the sinks'.
+struct KeyList {
+  int hi, lo, s_hi, ns, m0, n;
+  template <int BLK>
+  __device__ __forceinline__ int key0(int t) const {
+    return (t < ns ? t : t - ns + m0) * BLK;
+  }
+  __device__ __forceinline__ bool any(int j) const { return j < hi && (j >= lo || j < s_hi); }
+};
+template <int BLK>
+__device__ __forceinline__ KeyList key_list(const Seq& s, int t_lo, int t_hi, int window, int sinks, bool tree) {
+  KeyList k;
+  k.hi = s.first + t_hi + 1;
+  k.lo = window_begin(tree ? s.first : s.first + t_lo, window);
+  k.s_hi = min(min(sinks, k.lo), k.hi);
+  k.m0 = k.lo / BLK;
+  k.ns = k.s_hi > 0 ? min((k.s_hi - 1) / BLK + 1, k.m0) : 0;
+  k.n = k.hi > 0 ? k.ns + (k.hi - 1) / BLK + 1 - k.m0 : 0;
+  return k;
+}
+
+// How a call is cut: row blocks of block_rows (the most of any sequence: tiles), the list of each block's
+// keys over at most `splits` workgroups of at least min_blocks key blocks.
+struct PagedPlan {
+  int max_rows, block_rows, tiles, block_keys, min_blocks, splits;
+};
+__device__ __forceinline__ int split_count(int blocks, const PagedPlan& p) {
+  return min(p.splits, max(1, (blocks + p.min_blocks - 1) / p.min_blocks));
+}
+// The most keys that a row block of the call reads.
+inline long long most_keys(const PagedCall& c, int max_len) {
+  return c.window > 0 ? std::min<long long>(max_len, (long long)c.window + c.sinks + c.seqs.max_new) : max_len;
+}
+inline size_t paged_part_bytes(const PagedCall& c, const PagedPlan& p) {
+  return p.splits > 1 ? sizeof(float) * (size_t)c.B * c.Hkv * p.splits * sdpa_part_floats(p.max_rows, c.D) : 0;
+}
+// o = the splits' results joined, for the rows whose keys were split (sdpa_paged_rows.hip).
+hipError_t launch_paged_combine(hipStream_t s, const PagedCall& c, const PagedPlan& p, const float* part);
+
 // ws: the results of split keys; with less than sdpa_paged_workspace_bytes it runs unsplit.  max_len:
 // the longest sequence, for the plan.
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
+// More than kTileRows rows a key/value head, 8 <= D <= 128 (sdpa_paged_tile.hip).
+constexpr int kTileRows = 64;
+bool sdpa_paged_tile_applies(const PagedCall& c);
+hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
+size_t sdpa_paged_tile_workspace_bytes(const PagedCall& c, int max_len);
 // 4 <= D <= 256 (sdpa_paged_rows.hip).
 bool sdpa_paged_rows_applies(const PagedCall& c);
 hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);

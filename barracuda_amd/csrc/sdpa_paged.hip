@@ -91,10 +91,12 @@ __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCal
 namespace bch {
 
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len) {
+  if (sdpa_paged_tile_applies(c)) return sdpa_paged_tile_workspace_bytes(c, max_len);
   return sdpa_paged_rows_applies(c) ? sdpa_paged_rows_workspace_bytes(c, max_len) : 0;
 }
 
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes) {
+  if (sdpa_paged_tile_applies(c)) return launch_sdpa_paged_tile(s, c, max_len, ws, ws_bytes);
   if (sdpa_paged_rows_applies(c)) return launch_sdpa_paged_rows(s, c, max_len, ws, ws_bytes);
   const long long tiles = ((long long)c.seqs.max_new * c.H + kAnyWaves - 1) / kAnyWaves;
   if (tiles * c.B > 0x7fffffffLL) return hipErrorInvalidConfiguration;

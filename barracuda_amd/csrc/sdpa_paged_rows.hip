@@ -32,6 +32,7 @@ namespace {
 
 using bch::f32x4;
 using bch::PagedCall;
+using bch::PagedPlan;
 
 constexpr float kLazy = 8.0f;  // log2 headroom before the reference max moves
 constexpr int kRows = 16;      // rows per workgroup
@@ -70,12 +71,8 @@ __device__ __forceinline__ f32x4 once(f32x4 x, int d0, int D) {
   return x;
 }
 
-struct RowsPlan {
-  int rblocks, splits, max_rows;
-};
-
 template <int DP, bool FULL, bool TREE>
-__global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows_kernel(PagedCall c, RowsPlan plan,
+__global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows_kernel(PagedCall c, PagedPlan plan,
                                                                                       float* __restrict__ part) {
   constexpr int NC = DP / 16, NH = DP / 64;
   __shared__ float red_m[kWaves][kRows], red_l[kWaves][kRows];
@@ -87,13 +84,17 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
   const int nb = gridDim.x;
   int L = blockIdx.x;
   if ((nb & 7) == 0) L = (L & 7) * (nb >> 3) + (L >> 3);
-  const int rb = L % plan.rblocks;
-  const int sp = L / plan.rblocks % plan.splits;
-  const int bk = L / plan.rblocks / plan.splits;
+  const int rb = L % plan.tiles;
+  const int sp = L / plan.tiles % plan.splits;
+  const int bk = L / plan.tiles / plan.splits;
   const int b = bk / c.Hkv, hk = bk - b * c.Hkv;
   const bch::Seq s = bch::load_seq(c.kv, c.seqs, b);
   const int group = c.H / c.Hkv, rows = s.n * group;
   if (rb * kRows >= rows) return;
+  const int t_lo = rb * kRows / group, t_hi = (min(rb * kRows + kRows, rows) - 1) / group;
+  const bch::KeyList keys = bch::key_list<kBlk>(s, t_lo, t_hi, c.window, c.sinks, TREE);
+  const int splits = bch::split_count(keys.n, plan);
+  if (sp >= splits) return;
   if constexpr (TREE) {
     static_assert(64 * kWaves >= bch::kMaxDrafts, "tree_masks");
     bch::tree_masks(tree, c.parent, s, c.window, c.sinks);
@@ -120,14 +121,9 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
     qf[n] = once<FULL>(load4(qr + four<FULL>(d0, D)), d0, D) * c.qscale;
   }
 
-  // ---- the keys that any of these rows sees: [0, s_hi) and [lo, hi), as a list of blocks ----
-  const int t_lo = rb * kRows / group, t_hi = min(rb * kRows + kRows - 1, rows - 1) / group;
   const int p_lo = TREE ? s.first : s.first + t_lo, p_hi = s.first + t_hi;
-  const int hi = p_hi + 1, lo = bch::window_begin(p_lo, c.window), s_hi = min(min(c.sinks, lo), hi);
-  const int m0 = lo / kBlk, ns = s_hi > 0 ? min((s_hi - 1) / kBlk + 1, m0) : 0;
-  const int nall = hi > 0 ? ns + (hi - 1) / kBlk + 1 - m0 : 0;
-  const int t0 = (int)((long long)nall * sp / plan.splits), t1 = (int)((long long)nall * (sp + 1) / plan.splits);
-  auto key0 = [&](int t) { return (t < ns ? t : t - ns + m0) * kBlk; };
+  const int t0 = (int)((long long)keys.n * sp / splits), t1 = (int)((long long)keys.n * (sp + 1) / splits);
+  auto key0 = [&](int t) { return keys.key0<kBlk>(t); };
 
   f32x4 acc[4 * NH];
   float m_ref, l_run;
@@ -151,7 +147,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
     const int j = key0(t) + i, n = (int)(((unsigned long long)(unsigned)j * c.kv.mul) >> c.kv.shift);
     bch::Slot slot{b, j};
     if (c.kv.table) slot = {entry, j - n * c.kv.page_size};
-    const bool on = j < hi && (j >= lo || j < s_hi) && (unsigned)slot.page < (unsigned)c.kv.num_pages;
+    const bool on = keys.any(j) && (unsigned)slot.page < (unsigned)c.kv.num_pages;
     if (!on) slot = {0, 0};
     there[u] = (unsigned)__ballot(on) & 0xffffu;
     const float* kr = kh + bch::slot_offset(c.kv.kl, slot);
@@ -332,7 +328,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
   if (my >= rows) return;
   float* dst;
   float inv = 1.0f;
-  if (plan.splits > 1) {
+  if (splits > 1) {
     float* p = part + ((long long)bk * plan.splits + sp) * bch::sdpa_part_floats(plan.max_rows, D);
     dst = p + (long long)my * D;
     if (g == 0) {
@@ -358,18 +354,23 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
 
 // o[row] = sum over splits of 2^(m_s - m) O_s / sum of 2^(m_s - m) l_s, in split order: a wavefront per
 // row, lane s the maximum and sum of split s.  A split without a key that the row sees has l = 0 and
-// counts nothing; a row without any gives zeros.
-__global__ __launch_bounds__(64) void paged_combine(PagedCall c, RowsPlan plan, const float* __restrict__ part) {
+// counts nothing; a row without any gives zeros.  Rows whose keys were not split are there already.
+template <int BLK, bool TREE>
+__global__ __launch_bounds__(64) void paged_combine(PagedCall c, PagedPlan plan, const float* __restrict__ part) {
   const int bk = blockIdx.x / plan.max_rows, row = blockIdx.x % plan.max_rows;
   const int b = bk / c.Hkv, hk = bk - b * c.Hkv;
   const bch::Seq s = bch::load_seq(c.kv, c.seqs, b);
-  const int group = c.H / c.Hkv;
-  if (row >= s.n * group) return;
+  const int group = c.H / c.Hkv, rows = s.n * group;
+  if (row >= rows) return;
+  const int r0 = row / plan.block_rows * plan.block_rows;
+  const int splits = bch::split_count(
+      bch::key_list<BLK>(s, r0 / group, (min(r0 + plan.block_rows, rows) - 1) / group, c.window, c.sinks, TREE).n, plan);
+  if (splits == 1) return;
   const long long per = bch::sdpa_part_floats(plan.max_rows, c.D);
   const float* p = part + (long long)bk * plan.splits * per;
   const float* ml = p + (long long)plan.max_rows * c.D + 2 * row;
   const int lane = threadIdx.x;
-  const bool on = lane < plan.splits;
+  const bool on = lane < splits;
   const float ms = on ? ml[lane * per] : -INFINITY, ls = on ? ml[lane * per + 1] : 0.0f;
   const float m = bch::wave_allreduce(ms, bch::OpMax());
   const float as = __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.0f : m));
@@ -383,35 +384,37 @@ __global__ __launch_bounds__(64) void paged_combine(PagedCall c, RowsPlan plan, 
     const float* po = p + (long long)row * c.D + min(d, c.D - 1);
     float x = 0.0f;
     int u = 0;
-    for (; u + 8 <= plan.splits; u += 8) {
+    for (; u + 8 <= splits; u += 8) {
       float v[8];
 #pragma unroll
       for (int w = 0; w < 8; ++w) v[w] = po[(u + w) * per];
 #pragma unroll
       for (int w = 0; w < 8; ++w) x = fmaf(bch::readlane(as, u + w), v[w], x);
     }
-    for (; u < plan.splits; ++u) x = fmaf(bch::readlane(as, u), po[u * per], x);
+    for (; u < splits; ++u) x = fmaf(bch::readlane(as, u), po[u * per], x);
     if (d < c.D) dst[d] = x * inv;
   }
 }
 
-// Two workgroups per CU fill the chip's loads; a split keeps at least 128 keys (two blocks a wavefront)
-// and there are at most 64, whose results one wavefront still adds quickly.
-RowsPlan rows_plan(const PagedCall& c, int max_len, bool may_split) {
-  RowsPlan p;
+// Four workgroups per CU where the sequences may differ in length (the plan knows the longest alone), two
+// where there is one; a split keeps at least 128 keys (two blocks a wavefront) and there are at most 64,
+// whose results one wavefront still adds quickly.
+PagedPlan rows_plan(const PagedCall& c, int max_len, bool may_split) {
+  PagedPlan p;
   p.max_rows = c.seqs.max_new * (c.H / c.Hkv);
-  p.rblocks = (p.max_rows + kRows - 1) / kRows;
-  const long long units = (long long)c.B * c.Hkv * p.rblocks;
-  long long keys = max_len;
-  if (c.window > 0) keys = std::min(keys, (long long)c.window + c.sinks + c.seqs.max_new);
-  long long want = may_split ? (2LL * bch::device_cu_count() + units - 1) / units : 1;
-  p.splits = (int)std::max(1LL, std::min({want, keys / 128, 64LL}));
+  p.block_rows = kRows;
+  p.tiles = (p.max_rows + kRows - 1) / kRows;
+  p.block_keys = kBlk;
+  p.min_blocks = 8;
+  const long long units = (long long)c.B * c.Hkv * p.tiles;
+  const long long want = may_split ? ((c.B > 1 ? 4LL : 2LL) * bch::device_cu_count() + units - 1) / units : 1;
+  p.splits = (int)std::max(1LL, std::min({want, bch::most_keys(c, max_len) / (kBlk * p.min_blocks), 64LL}));
   return p;
 }
 
 template <int DP>
-void launch_dp(hipStream_t s, const PagedCall& c, const RowsPlan& p, float* part) {
-  const dim3 grid((unsigned)((long long)c.B * c.Hkv * p.rblocks * p.splits)), block(64 * kWaves);
+void launch_dp(hipStream_t s, const PagedCall& c, const PagedPlan& p, float* part) {
+  const dim3 grid((unsigned)((long long)c.B * c.Hkv * p.tiles * p.splits)), block(64 * kWaves);
   const bool full = c.D == DP, tree = c.parent != nullptr;
   auto kern = full ? (tree ? sdpa_paged_rows_kernel<DP, true, true> : sdpa_paged_rows_kernel<DP, true, false>)
                    : (tree ? sdpa_paged_rows_kernel<DP, false, true> : sdpa_paged_rows_kernel<DP, false, false>);
@@ -430,19 +433,25 @@ bool sdpa_paged_rows_applies(const PagedCall& c) {
 }
 
 size_t sdpa_paged_rows_workspace_bytes(const PagedCall& c, int max_len) {
-  const RowsPlan p = rows_plan(c, max_len, true);
-  return p.splits > 1 ? sizeof(float) * (size_t)c.B * c.Hkv * p.splits * sdpa_part_floats(p.max_rows, c.D) : 0;
+  return paged_part_bytes(c, rows_plan(c, max_len, true));
 }
 
 hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes) {
-  const RowsPlan p = rows_plan(c, max_len, ws_bytes >= sdpa_paged_rows_workspace_bytes(c, max_len));
+  const PagedPlan p = rows_plan(c, max_len, ws_bytes >= sdpa_paged_rows_workspace_bytes(c, max_len));
   float* part = static_cast<float*>(ws);
   if (c.D <= 64) launch_dp<64>(s, c, p, part);
   else if (c.D <= 128) launch_dp<128>(s, c, p, part);
   else launch_dp<256>(s, c, p, part);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.splits == 1) return e;
-  hipLaunchKernelGGL(paged_combine, dim3((unsigned)((long long)c.B * c.Hkv * p.max_rows)), dim3(64), 0, s, c, p, part);
+  return launch_paged_combine(s, c, p, part);
+}
+
+hipError_t launch_paged_combine(hipStream_t s, const PagedCall& c, const PagedPlan& p, const float* part) {
+  const bool tree = c.parent != nullptr;
+  auto kern = p.block_keys == 16 ? (tree ? paged_combine<16, true> : paged_combine<16, false>)
+                                 : (tree ? paged_combine<32, true> : paged_combine<32, false>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)((long long)c.B * c.Hkv * p.max_rows)), dim3(64), 0, s, c, p, part);
   return hipGetLastError();
 }
 
