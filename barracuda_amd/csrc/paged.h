@@ -184,37 +184,177 @@ __device__ __forceinline__ KeyList key_list(const Seq& s, int t_lo, int t_hi, in
   return k;
 }
 
-// How a call is cut: row blocks of block_rows (the most of any sequence: tiles), the list of each block's
-// keys over at most `splits` workgroups of at least min_blocks key blocks.
-struct PagedPlan {
-  int max_rows, block_rows, tiles, block_keys, min_blocks, splits;
+// ---- equal shares ----
+// The lists of all row blocks, key/value heads and sequences stand in one line, a list as long as its key
+// blocks and `over` more (what a workgroup spends on beginning and ending one, in blocks); the line is cut
+// into equal shares, a workgroup each, whatever the lengths of the sequences.  A share may hold the end of
+// one list, whole ones and the beginning of another; the parts of a list that was cut meet in
+// paged_combine.
+struct SharePlan {
+  int row_min, row_max;  // rows a key/value head of the sequences served
+  int tiles;             // row blocks of the longest of them
+  int part_rows;         // rows of a part: a row block's, if any sequence has as many
+  int slots;             // parts a list may be cut into; 1 (no workspace): a workgroup a list
+  int min_share;
 };
-__device__ __forceinline__ int split_count(int blocks, const PagedPlan& p) {
-  return min(p.splits, max(1, (blocks + p.min_blocks - 1) / p.min_blocks));
+// Workspace: the number of parts of every list, then the parts: rows of O, then (reference max, sum) pairs.
+__host__ __device__ inline long long part_floats(const SharePlan& p, int D) { return (long long)p.part_rows * (D + 2); }
+__host__ __device__ inline long long counts_floats(long long lists) { return (lists + 63) / 64 * 64; }
+inline long long lists_of(const PagedCall& c, const SharePlan& p) { return (long long)c.B * c.Hkv * p.tiles; }
+inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
+  if (p.slots <= 1) return 0;
+  const long long lists = lists_of(c, p);
+  return sizeof(float) * (size_t)(counts_floats(lists) + lists * p.slots * part_floats(p, c.D));
 }
+
+// The lists of 64 sequences from b0 on, one sequence a lane.
+struct Lane64 {
+  int tiles, length;  // a list's place in the line
+  long long sum;      // of all lists up to and with this sequence's
+};
+// Where a workgroup is in its share [.., end): the next place x, the sequences around it (b0 on, `before` the
+// line before them), and what it is to do: p0 .. p1 of a list, part number slot of count (0: done).
+struct Share {
+  Lane64 seqs[64];
+  long long share, x, end, before;
+  int b0, b, hk, rb, p0, p1, slot, count;
+};
+__device__ __forceinline__ long long uniform(long long v) {
+  return (long long)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+                     (unsigned)__builtin_amdgcn_readfirstlane((int)v));
+}
+
+// BLK keys a block, ROWS rows a block, OVER blocks for a list's beginning and end.
+template <int BLK, int ROWS, int OVER, bool TREE>
+struct Shares {
+  static __device__ __forceinline__ Lane64 line(const PagedCall& c, const SharePlan& plan, int b0, int lane) {
+    Lane64 r{0, 1, 0};
+    if (b0 + lane < c.B) {
+      const Seq s = load_seq(c.kv, c.seqs, b0 + lane);
+      const long long rows = (long long)s.n * (c.H / c.Hkv);
+      if (rows > 0 && rows >= plan.row_min && rows <= plan.row_max) {
+        r.tiles = ((int)rows - 1) / ROWS + 1;
+        // (that of all rows of the sequence; a row block's own list may be shorter, never longer)
+        r.length = key_list<BLK>(s, 0, s.n - 1, c.window, c.sinks, TREE).n + OVER;
+        r.sum = (long long)c.Hkv * r.tiles * r.length;
+      }
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const long long up = __shfl_up(r.sum, d);
+      if (lane >= d) r.sum += up;
+    }
+    return r;
+  }
+
+  // By the first wavefront.  The state is kept in LDS: held in registers, it would cost the loops over the
+  // keys some.
+  static __device__ __forceinline__ void begin(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
+    Lane64 seqs;
+    long long total = 0;
+    int longest = 1;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+      seqs = line(c, plan, b0, lane);
+      total += uniform(__shfl(seqs.sum, 63));
+      int w = seqs.tiles > 0 ? seqs.length : 1;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) w = max(w, __shfl_xor(w, d));
+      longest = max(longest, __builtin_amdgcn_readfirstlane(w));
+    }
+    if (c.B > 64) seqs = line(c, plan, 0, lane);
+    f.seqs[lane] = seqs;
+    // a list of length w is cut into at most ceil((w - 1) / share) + 1 parts
+    const long long share = max(max((long long)plan.min_share, (total + gridDim.x - 1) / gridDim.x),
+                                ((long long)longest + plan.slots - 2) / (plan.slots - 1));
+    if (lane == 0) {
+      f.share = share;
+      f.x = blockIdx.x * share;
+      f.end = min(total, f.x + share);
+      f.before = 0;
+      f.b0 = 0;
+    }
+  }
+
+  // The next list of the share, or the part of one; by the first wavefront, a barrier behind it.
+  static __device__ __forceinline__ void next(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
+    asm volatile("" ::: "memory");
+    const long long x = uniform(f.x), x1 = uniform(f.end), share = uniform(f.share);
+    int count = 0;
+    if (x < x1) {
+      const long long x0 = blockIdx.x * share;
+      long long before = uniform(f.before);
+      int b0 = __builtin_amdgcn_readfirstlane(f.b0);
+      Lane64 seqs = f.seqs[lane];
+      for (long long sum; before + (sum = uniform(__shfl(seqs.sum, 63))) <= x;) {
+        before += sum;
+        b0 += 64;
+        seqs = line(c, plan, b0, lane);
+        f.seqs[lane] = seqs;
+      }
+      const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + seqs.sum <= x)));
+      const int tiles = __builtin_amdgcn_readlane(seqs.tiles, at), length = __builtin_amdgcn_readlane(seqs.length, at);
+      const long long off = x - before - (at > 0 ? uniform(__shfl(seqs.sum, at - 1)) : 0);
+      const int list = (int)(off / length), p0 = (int)(off - (long long)list * length);
+      const int p1 = (int)min((long long)length, p0 + x1 - x);
+      // parts: the list begins at x - p0 and is cut at multiples of the share
+      const long long begin = x - p0;
+      const int slot = begin >= x0 ? 0 : (int)((x0 - begin + share - 1) / share);
+      count = begin + length <= x0 + share ? slot + 1 : slot + 1 + (int)((begin + length - x0 - 1) / share);
+      if (lane == 0) {
+        f.x = x + p1 - p0;
+        f.before = before;
+        f.b0 = b0;
+        f.b = b0 + at;
+        f.hk = list / tiles;
+        f.rb = list % tiles;
+        f.p0 = p0;
+        f.p1 = p1;
+        f.slot = slot;
+      }
+    }
+    if (lane == 0) f.count = count;
+  }
+};
+
+// A workgroup's piece of work: blocks t0 .. t1 of a list, part `slot` of `count` (0: none left).
+struct Piece {
+  int b, hk, rb, p0, p1, slot, count;
+};
+__device__ __forceinline__ Piece read_piece(const Share& f) {
+  auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+  return {u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1), u(f.slot), u(f.count)};
+}
+// Part `slot` of a list in the workspace; the list's number of parts is noted by its first.
+__device__ __forceinline__ float* part_of(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
+  const long long list = ((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb;
+  return ws + counts_floats((long long)c.B * c.Hkv * plan.tiles) + (list * plan.slots + p.slot) * part_floats(plan, c.D);
+}
+__device__ __forceinline__ void note_count(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
+  if (plan.slots > 1 && p.slot == 0)
+    reinterpret_cast<int*>(ws)[((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb] = p.count;
+}
+// o of the lists that were cut; rows: of a row block (16 or 256) (sdpa_paged.hip).
+hipError_t launch_paged_combine(hipStream_t s, const PagedCall& c, const SharePlan& p, int rows, const float* ws);
+
 // The most keys that a row block of the call reads.
 inline long long most_keys(const PagedCall& c, int max_len) {
   return c.window > 0 ? std::min<long long>(max_len, (long long)c.window + c.sinks + c.seqs.max_new) : max_len;
 }
-inline size_t paged_part_bytes(const PagedCall& c, const PagedPlan& p) {
-  return p.splits > 1 ? sizeof(float) * (size_t)c.B * c.Hkv * p.splits * sdpa_part_floats(p.max_rows, c.D) : 0;
-}
-// o = the splits' results joined, for the rows whose keys were split (sdpa_paged_rows.hip).
-hipError_t launch_paged_combine(hipStream_t s, const PagedCall& c, const PagedPlan& p, const float* part);
 
 // ws: the results of split keys; with less than sdpa_paged_workspace_bytes it runs unsplit.  max_len:
 // the longest sequence, for the plan.
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
-// More than kTileRows rows a key/value head, 8 <= D <= 128 (sdpa_paged_tile.hip).
+// The sequences with more than kTileRows rows a key/value head, 8 <= D <= 128 (sdpa_paged_tile.hip).
 constexpr int kTileRows = 64;
 bool sdpa_paged_tile_applies(const PagedCall& c);
 hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
 size_t sdpa_paged_tile_workspace_bytes(const PagedCall& c, int max_len);
-// 4 <= D <= 256 (sdpa_paged_rows.hip).
-bool sdpa_paged_rows_applies(const PagedCall& c);
-hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
-size_t sdpa_paged_rows_workspace_bytes(const PagedCall& c, int max_len);
+// The sequences with up to row_limit rows a key/value head, 4 <= D <= 256 (sdpa_paged_rows.hip).
+bool sdpa_paged_rows_applies(const PagedCall& c, int row_limit);
+hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, int row_limit, void* ws,
+                                  size_t ws_bytes);
+size_t sdpa_paged_rows_workspace_bytes(const PagedCall& c, int max_len, int row_limit);
 
 // ---- the cache's own calls (kv_pages.hip) ----
 hipError_t launch_kv_append(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B, int Hkv,
