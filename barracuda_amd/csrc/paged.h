@@ -189,7 +189,8 @@ __device__ __forceinline__ KeyList key_list(const Seq& s, int t_lo, int t_hi, in
 // blocks and `over` more (what a workgroup spends on beginning and ending one, in blocks); the line is cut
 // into equal shares, a workgroup each, whatever the lengths of the sequences.  A share may hold the end of
 // one list, whole ones and the beginning of another; the parts of a list that was cut meet in
-// paged_combine.
+// paged_combine.  Where there are few lists or little to do, each list is cut into equal parts by itself
+// instead and a workgroup has one of them: no workgroup then begins two.
 struct SharePlan {
   int row_min, row_max;  // rows a key/value head of the sequences served
   int tiles;             // row blocks of the longest of them
@@ -201,6 +202,8 @@ struct SharePlan {
 __host__ __device__ inline long long part_floats(const SharePlan& p, int D) { return (long long)p.part_rows * (D + 2); }
 __host__ __device__ inline long long counts_floats(long long lists) { return (lists + 63) / 64 * 64; }
 inline long long lists_of(const PagedCall& c, const SharePlan& p) { return (long long)c.B * c.Hkv * p.tiles; }
+// A grid has fewer than 2^32 threads.
+inline bool fits_grid(long long workgroups, int threads) { return workgroups < (1LL << 32) / threads; }
 inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
   if (p.slots <= 1) return 0;
   const long long lists = lists_of(c, p);
@@ -218,6 +221,7 @@ struct Share {
   Lane64 seqs[64];
   long long share, x, end, before;
   int b0, b, hk, rb, p0, p1, slot, count;
+  int part;  // blocks a part, where each list is cut by itself (the line is then one of parts); else 0
 };
 __device__ __forceinline__ long long uniform(long long v) {
   return (long long)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
@@ -227,7 +231,7 @@ __device__ __forceinline__ long long uniform(long long v) {
 // BLK keys a block, ROWS rows a block, OVER blocks for a list's beginning and end.
 template <int BLK, int ROWS, int OVER, bool TREE>
 struct Shares {
-  static __device__ __forceinline__ Lane64 line(const PagedCall& c, const SharePlan& plan, int b0, int lane) {
+  static __device__ __forceinline__ Lane64 line(const PagedCall& c, const SharePlan& plan, int b0, int lane, int part) {
     Lane64 r{0, 1, 0};
     if (b0 + lane < c.B) {
       const Seq s = load_seq(c.kv, c.seqs, b0 + lane);
@@ -236,42 +240,64 @@ struct Shares {
         r.tiles = ((int)rows - 1) / ROWS + 1;
         // (that of all rows of the sequence; a row block's own list may be shorter, never longer)
         r.length = key_list<BLK>(s, 0, s.n - 1, c.window, c.sinks, TREE).n + OVER;
+        if (part) r.length = (r.length - 1) / part + 1;
         r.sum = (long long)c.Hkv * r.tiles * r.length;
       }
     }
+    add_up(r, lane);
+    return r;
+  }
+  static __device__ __forceinline__ void add_up(Lane64& r, int lane) {
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const long long up = __shfl_up(r.sum, d);
       if (lane >= d) r.sum += up;
     }
-    return r;
   }
 
   // By the first wavefront.  The state is kept in LDS: held in registers, it would cost the loops over the
   // keys some.
   static __device__ __forceinline__ void begin(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
     Lane64 seqs;
-    long long total = 0;
+    long long total = 0, lists = 0;
     int longest = 1;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-      seqs = line(c, plan, b0, lane);
+      seqs = line(c, plan, b0, lane, 0);
       total += uniform(__shfl(seqs.sum, 63));
-      int w = seqs.tiles > 0 ? seqs.length : 1;
+      int w = seqs.tiles > 0 ? seqs.length : 1, n = seqs.tiles;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) w = max(w, __shfl_xor(w, d));
+      for (int d = 1; d < 64; d *= 2) {
+        w = max(w, __shfl_xor(w, d));
+        n += __shfl_xor(n, d);
+      }
       longest = max(longest, __builtin_amdgcn_readfirstlane(w));
+      lists += (long long)c.Hkv * __builtin_amdgcn_readfirstlane(n);
     }
-    if (c.B > 64) seqs = line(c, plan, 0, lane);
-    f.seqs[lane] = seqs;
     // a list of length w is cut into at most ceil((w - 1) / share) + 1 parts
-    const long long share = max(max((long long)plan.min_share, (total + gridDim.x - 1) / gridDim.x),
-                                ((long long)longest + plan.slots - 2) / (plan.slots - 1));
+    const long long grid = gridDim.x, slots = plan.slots - 1;
+    long long share = max(max((long long)plan.min_share, (total + grid - 1) / grid), (longest + slots - 1) / slots);
+    // parts of one list each: ceil(w / part) <= w / part + 1 of them, in all no more than workgroups; up to a
+    // twentieth longer than the shares
+    int part = 0;
+    if (lists < grid) {
+      const long long p = max((long long)plan.min_share, (total + grid - lists - 1) / (grid - lists));
+      if (20 * p <= 21 * share && (longest - 1) / p < plan.slots) part = (int)p;
+    }
+    if (part || c.B > 64) seqs = line(c, plan, 0, lane, part);
+    f.seqs[lane] = seqs;
+    if (part) {
+      share = 1;
+      total = 0;
+      for (int b0 = 0; b0 < c.B; b0 += 64)
+        total += uniform(__shfl(b0 == 0 ? seqs.sum : line(c, plan, b0, lane, part).sum, 63));
+    }
     if (lane == 0) {
       f.share = share;
       f.x = blockIdx.x * share;
       f.end = min(total, f.x + share);
       f.before = 0;
       f.b0 = 0;
+      f.part = part;
     }
   }
 
@@ -288,7 +314,7 @@ struct Shares {
       for (long long sum; before + (sum = uniform(__shfl(seqs.sum, 63))) <= x;) {
         before += sum;
         b0 += 64;
-        seqs = line(c, plan, b0, lane);
+        seqs = line(c, plan, b0, lane, __builtin_amdgcn_readfirstlane(f.part));
         f.seqs[lane] = seqs;
       }
       const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + seqs.sum <= x)));
@@ -316,13 +342,19 @@ struct Shares {
   }
 };
 
-// A workgroup's piece of work: blocks t0 .. t1 of a list, part `slot` of `count` (0: none left).
+// A workgroup's piece of work: part `slot` of `count` (0: none left) of a list.
 struct Piece {
   int b, hk, rb, p0, p1, slot, count;
+  bool parts;  // p0 is the part's number; else p0 .. p1 of the list's length
+  // its blocks, of the n that the row block's list has
+  __device__ __forceinline__ void blocks(int n, int over, int& t0, int& t1) const {
+    t0 = parts ? (int)((long long)n * p0 / count) : min(max(p0 - over, 0), n);
+    t1 = parts ? (int)((long long)n * (p0 + 1) / count) : min(max(p1 - over, 0), n);
+  }
 };
 __device__ __forceinline__ Piece read_piece(const Share& f) {
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  return {u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1), u(f.slot), u(f.count)};
+  return {u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1), u(f.slot), u(f.count), u(f.part) != 0};
 }
 // Part `slot` of a list in the workspace; the list's number of parts is noted by its first.
 __device__ __forceinline__ float* part_of(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
@@ -333,8 +365,7 @@ __device__ __forceinline__ void note_count(float* ws, const PagedCall& c, const 
   if (plan.slots > 1 && p.slot == 0)
     reinterpret_cast<int*>(ws)[((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb] = p.count;
 }
-// o of the lists that were cut; rows: of a row block (16 or 256) (sdpa_paged.hip).
-hipError_t launch_paged_combine(hipStream_t s, const PagedCall& c, const SharePlan& p, int rows, const float* ws);
+constexpr int kShortRows = 16, kTileRows = 256;  // rows of a row block of the two kernels
 
 // The most keys that a row block of the call reads.
 inline long long most_keys(const PagedCall& c, int max_len) {
@@ -345,16 +376,15 @@ inline long long most_keys(const PagedCall& c, int max_len) {
 // the longest sequence, for the plan.
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
-// The sequences with more than kTileRows rows a key/value head, 8 <= D <= 128 (sdpa_paged_tile.hip).
-constexpr int kTileRows = 64;
+// The sequences with more than kFewRows rows a key/value head, 8 <= D <= 128 (sdpa_paged_tile.hip), and the
+// ones with up to row_limit, 4 <= D <= 256 (sdpa_paged_rows.hip).  A plan's workspace: share_bytes.
+constexpr int kFewRows = 64;
 bool sdpa_paged_tile_applies(const PagedCall& c);
-hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
-size_t sdpa_paged_tile_workspace_bytes(const PagedCall& c, int max_len);
-// The sequences with up to row_limit rows a key/value head, 4 <= D <= 256 (sdpa_paged_rows.hip).
+SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split);
+hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws);
 bool sdpa_paged_rows_applies(const PagedCall& c, int row_limit);
-hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, int row_limit, void* ws,
-                                  size_t ws_bytes);
-size_t sdpa_paged_rows_workspace_bytes(const PagedCall& c, int max_len, int row_limit);
+SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, bool may_split);
+hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws);
 
 // ---- the cache's own calls (kv_pages.hip) ----
 hipError_t launch_kv_append(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B, int Hkv,

@@ -88,143 +88,117 @@ __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCal
 }
 
 // o[row] = sum over a list's parts of 2^(m_s - m) O_s / sum of 2^(m_s - m) l_s, in their order: a
-// wavefront four rows, lane s the maximum and sum of part s, lane d (and on by 64) the columns.  A part
+// wavefront per row, lane s the maximum and sum of part s, lane d (and on by 64) the columns.  A part
 // without a key that the row sees has l = 0 and counts nothing; a row without any gives zeros.  Rows of a
-// list that was not cut are there already.  Trips to memory bound it, so a wavefront's four rows make
-// them together.
-template <int ROWS>
-__global__ __launch_bounds__(256) void paged_combine(PagedCall c, bch::SharePlan plan, const float* __restrict__ ws) {
-  constexpr int R = 4, Q = ROWS / 16;
-  const int list = blockIdx.x / Q;
+// list that was not cut are there already.  Trips to memory bound it: the rows of eight parts are loaded
+// before they are added.  The lists of both kernels in one launch: the first workgroups (four
+// rows each) have those of the tiles.
+struct Combined {
+  bch::SharePlan plan;
+  int block_rows, groups;
+  const float* ws;
+};
+__global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile, Combined rows16) {
+  const bool is_tile = (int)blockIdx.x < tile.groups;
+  const Combined& k = is_tile ? tile : rows16;
+  const bch::SharePlan& plan = k.plan;
+  const int per_list = k.block_rows / 4, at = is_tile ? blockIdx.x : blockIdx.x - tile.groups, list = at / per_list;
   const int rb = list % plan.tiles, bk = list / plan.tiles, b = bk / c.Hkv, hk = bk - b * c.Hkv;
   const Seq s = bch::load_seq(c.kv, c.seqs, b);
   const int group = c.H / c.Hkv;
   const long long rows = (long long)s.n * group;
-  const int lane = threadIdx.x & 63, r0 = (blockIdx.x % Q) * 16 + (threadIdx.x >> 6) * R;  // within the row block
-  if ((long long)rb * ROWS + r0 >= rows || rows < plan.row_min || rows > plan.row_max) return;
-  const int count = reinterpret_cast<const int*>(ws)[list];
+  const int lane = threadIdx.x & 63, r = (at % per_list) * 4 + (threadIdx.x >> 6);  // within the row block
+  const long long row = (long long)rb * k.block_rows + r;
+  if (row >= rows || rows < plan.row_min || rows > plan.row_max) return;
+  const int count = reinterpret_cast<const int*>(k.ws)[list];
   if (count <= 1) return;
   const long long per = bch::part_floats(plan, c.D);
-  const float* p = ws + bch::counts_floats((long long)c.B * c.Hkv * plan.tiles) + (long long)list * plan.slots * per;
-  const int last = (int)min(rows - (long long)rb * ROWS, (long long)plan.part_rows) - 1;
-  const float *ml[R], *po[R];
-  float m[R];
-#pragma unroll
-  for (int j = 0; j < R; ++j) {
-    const int r = min(r0 + j, last);
-    ml[j] = p + (long long)plan.part_rows * c.D + 2 * r;
-    po[j] = p + (long long)r * c.D;
-    m[j] = -INFINITY;
-  }
-  for (int u0 = 0; u0 < count; u0 += 64) {
-    float v[R];
-#pragma unroll
-    for (int j = 0; j < R; ++j) v[j] = u0 + lane < count ? ml[j][(u0 + lane) * per] : -INFINITY;
-#pragma unroll
-    for (int j = 0; j < R; ++j) m[j] = fmaxf(m[j], bch::wave_allreduce(v[j], bch::OpMax()));
-  }
+  const float* p = k.ws + bch::counts_floats((long long)c.B * c.Hkv * plan.tiles) + (long long)list * plan.slots * per;
+  const float* ml = p + (long long)plan.part_rows * c.D + 2 * r;
+  const float* po = p + (long long)r * c.D;
+  float m = -INFINITY;
+  for (int u0 = 0; u0 < count; u0 += 64)
+    m = fmaxf(m, bch::wave_allreduce(u0 + lane < count ? ml[(u0 + lane) * per] : -INFINITY, bch::OpMax()));
+  const int tok = (int)(row / group);
+  float* dst = c.o + b * c.ol.batch + (long long)(s.row0 + tok) * c.ol.row +
+               (hk * group + row - (long long)tok * group) * c.ol.head;
   for (int d0 = 0; d0 < c.D; d0 += 128) {
     const int da = min(d0 + lane, c.D - 1), db = min(d0 + lane + 64, c.D - 1);
-    float x[R], y[R], l[R];
-#pragma unroll
-    for (int j = 0; j < R; ++j) x[j] = y[j] = l[j] = 0.0f;
+    float x = 0.0f, y = 0.0f, l = 0.0f;
     for (int u0 = 0; u0 < count; u0 += 64) {
       const bool on = u0 + lane < count;
       const int n = min(64, count - u0);
-      float a[R];
+      const float ms = on ? ml[(u0 + lane) * per] : -INFINITY, ls = on ? ml[(u0 + lane) * per + 1] : 0.0f;
+      const float a = __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.0f : m));
+      l += bch::wave_allreduce(a * ls, bch::OpSum());
+      for (int u = 0; u < n; u += 8) {
+        float vx[8], vy[8];
 #pragma unroll
-      for (int j = 0; j < R; ++j) {
-        const float ms = on ? ml[j][(u0 + lane) * per] : -INFINITY, ls = on ? ml[j][(u0 + lane) * per + 1] : 0.0f;
-        a[j] = __builtin_amdgcn_exp2f(ms - (m[j] == -INFINITY ? 0.0f : m[j]));
-        l[j] += bch::wave_allreduce(a[j] * ls, bch::OpSum());
+        for (int w = 0; w < 8; ++w) {  // past the last part: it again, not added
+          const long long off = (u0 + min(u + w, n - 1)) * per;
+          vx[w] = po[off + da];
+          vy[w] = po[off + db];
+        }
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+          if (u + w < n) {
+            const float f = bch::readlane(a, u + w);
+            x = fmaf(f, vx[w], x);
+            y = fmaf(f, vy[w], y);
+          }
       }
-      auto add = [&](auto width, int u) {  // the next U parts, their rows loaded before they are added
-        constexpr int U = decltype(width)::value;
-        float vx[U][R], vy[U][R];
-#pragma unroll
-        for (int w = 0; w < U; ++w)
-#pragma unroll
-          for (int j = 0; j < R; ++j) {
-            vx[w][j] = po[j][(u0 + u + w) * per + da];
-            vy[w][j] = po[j][(u0 + u + w) * per + db];
-          }
-#pragma unroll
-        for (int w = 0; w < U; ++w)
-#pragma unroll
-          for (int j = 0; j < R; ++j) {
-            const float f = bch::readlane(a[j], u + w);
-            x[j] = fmaf(f, vx[w][j], x[j]);
-            y[j] = fmaf(f, vy[w][j], y[j]);
-          }
-      };
-      int u = 0;
-      for (; u + 4 <= n; u += 4) add(std::integral_constant<int, 4>{}, u);
-      for (; u < n; ++u) add(std::integral_constant<int, 1>{}, u);
     }
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const int row = rb * ROWS + r0 + j, tok = row / group;
-      if (r0 + j > last) break;
-      float* dst = c.o + b * c.ol.batch + (long long)(s.row0 + tok) * c.ol.row +
-                   (long long)(hk * group + row - tok * group) * c.ol.head;
-      if (d0 + lane < c.D) dst[d0 + lane] = l[j] == 0.0f ? 0.0f : x[j] / l[j];
-      if (d0 + lane + 64 < c.D) dst[d0 + lane + 64] = l[j] == 0.0f ? 0.0f : y[j] / l[j];
-    }
+    if (d0 + lane < c.D) dst[d0 + lane] = l == 0.0f ? 0.0f : x / l;
+    if (d0 + lane + 64 < c.D) dst[d0 + lane + 64] = l == 0.0f ? 0.0f : y / l;
   }
+}
+
+// Which kernels a call takes.  The tile kernel does 64 rows or fewer of a sequence as slowly as 256; a batch
+// may mix prompts and single tokens, so each kernel serves its own sequences.
+struct Route {
+  bool tile, rows;
+  bch::SharePlan tile_plan, rows_plan;
+  size_t tile_bytes, bytes;
+};
+Route route(const PagedCall& c, int max_len, bool may_split) {
+  Route r{};
+  r.tile = bch::sdpa_paged_tile_applies(c);
+  const int row_limit = r.tile ? bch::kFewRows : 0x7fffffff;
+  // dense operands: every sequence has max_new rows
+  r.rows = bch::sdpa_paged_rows_applies(c, row_limit) && !(r.tile && !c.seqs.start);
+  if (r.tile) {
+    r.tile_plan = bch::sdpa_paged_tile_plan(c, max_len, may_split);
+    r.tile_bytes = (bch::share_bytes(c, r.tile_plan) + 255) / 256 * 256;
+  }
+  if (r.rows) r.rows_plan = bch::sdpa_paged_rows_plan(c, max_len, row_limit, may_split);
+  r.bytes = r.tile_bytes + (r.rows ? bch::share_bytes(c, r.rows_plan) : 0);
+  return r;
 }
 
 }  // namespace
 
 namespace bch {
 
-hipError_t launch_paged_combine(hipStream_t s, const PagedCall& c, const SharePlan& p, int rows, const float* ws) {
-  // row blocks with rows in them: a part's rows are all that there are if they are fewer
-  const long long groups = lists_of(c, p) * (rows / 16);
-  if (groups > 0x7fffffffLL) return hipErrorInvalidConfiguration;
-  if (rows == 16)
-    hipLaunchKernelGGL(paged_combine<16>, dim3((unsigned)groups), dim3(256), 0, s, c, p, ws);
-  else
-    hipLaunchKernelGGL(paged_combine<256>, dim3((unsigned)groups), dim3(256), 0, s, c, p, ws);
-  return hipGetLastError();
-}
-
-namespace {
-
-// Which kernels a call takes.  The tile kernel does 64 rows or fewer of a sequence as slowly as 256; a batch
-// may mix prompts and single tokens, so each kernel serves its own sequences.
-struct Route {
-  bool tile, rows;
-  int row_limit;
-};
-Route route(const PagedCall& c) {
-  Route r;
-  r.tile = sdpa_paged_tile_applies(c);
-  r.row_limit = r.tile ? kTileRows : 0x7fffffff;
-  // dense operands: every sequence has max_new rows
-  r.rows = r.tile ? c.seqs.start != nullptr : sdpa_paged_rows_applies(c, r.row_limit);
-  return r;
-}
-size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-
-}  // namespace
-
-size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len) {
-  const Route r = route(c);
-  return (r.tile ? up256(sdpa_paged_tile_workspace_bytes(c, max_len)) : 0) +
-         (r.rows ? sdpa_paged_rows_workspace_bytes(c, max_len, r.row_limit) : 0);
-}
+size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len) { return route(c, max_len, true).bytes; }
 
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes) {
-  const Route r = route(c);
+  Route r = route(c, max_len, true);
+  if (ws_bytes < r.bytes) r = route(c, max_len, false);
   if (r.tile || r.rows) {
-    if (ws_bytes < sdpa_paged_workspace_bytes(c, max_len)) ws_bytes = 0;
-    const size_t at = r.tile ? std::min(ws_bytes, up256(sdpa_paged_tile_workspace_bytes(c, max_len))) : 0;
-    hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, max_len, ws, at) : hipSuccess;
-    if (e != hipSuccess || !r.rows) return e;
-    return launch_sdpa_paged_rows(s, c, max_len, r.row_limit, static_cast<char*>(ws) + at, ws_bytes - at);
+    float* tile_ws = static_cast<float*>(ws);
+    float* rows_ws = tile_ws + r.tile_bytes / sizeof(float);
+    hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, r.tile_plan, tile_ws) : hipSuccess;
+    if (e == hipSuccess && r.rows) e = launch_sdpa_paged_rows(s, c, r.rows_plan, rows_ws);
+    if (e != hipSuccess || r.bytes == 0) return e;
+    auto part = [&](const SharePlan& p, int block_rows, const float* w) {
+      return Combined{p, block_rows, p.slots > 1 ? (int)(lists_of(c, p) * (block_rows / 4)) : 0, w};
+    };
+    const Combined a = part(r.tile_plan, kTileRows, tile_ws), b = part(r.rows_plan, kShortRows, rows_ws);
+    hipLaunchKernelGGL(paged_combine, dim3((unsigned)a.groups + (unsigned)b.groups), dim3(256), 0, s, c, a, b);
+    return hipGetLastError();
   }
   const long long tiles = ((long long)c.seqs.max_new * c.H + kAnyWaves - 1) / kAnyWaves;
-  if (tiles * c.B > 0x7fffffffLL) return hipErrorInvalidConfiguration;
+  if (!fits_grid(tiles * c.B, 64 * kAnyWaves)) return hipErrorInvalidConfiguration;
   const dim3 grid((unsigned)(tiles * c.B)), block(64 * kAnyWaves);
 #define BCH_ANY(T_) hipLaunchKernelGGL(sdpa_paged_any_kernel<T_>, grid, block, 0, s, c, (int)tiles)
   if (c.D <= 64) BCH_ANY(1);

@@ -37,7 +37,7 @@ using bch::PagedCall;
 using bch::SharePlan;
 
 constexpr float kLazy = 8.0f;  // log2 headroom before the reference max moves
-constexpr int kRows = 16;      // rows per workgroup
+constexpr int kRows = bch::kShortRows;  // rows per workgroup
 constexpr int kBlk = 16;       // keys per block
 constexpr int kWaves = 4;
 
@@ -104,7 +104,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
       if (piece.count == 0) break;
     } else {
       const int bk = blockIdx.x / plan.tiles;
-      piece = {bk / c.Hkv, bk % c.Hkv, (int)(blockIdx.x % plan.tiles), 0, 0, 0, 1};
+      piece = {bk / c.Hkv, bk % c.Hkv, (int)(blockIdx.x % plan.tiles), 0, 0, 0, 1, true};
       more = false;
     }
     const int b = piece.b, hk = piece.hk, rb = piece.rb, count = piece.count;
@@ -118,8 +118,8 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
     }
     const int t_lo = rb * kRows / group, t_hi = (min(rb * kRows + kRows, rows) - 1) / group;
     const bch::KeyList keys = bch::key_list<kBlk>(s, t_lo, t_hi, c.window, c.sinks, TREE);
-    const int t0 = plan.slots > 1 ? min(max(piece.p0 - kOver, 0), keys.n) : 0;
-    const int t1 = plan.slots > 1 ? min(max(piece.p1 - kOver, 0), keys.n) : keys.n;
+    int t0, t1;
+    piece.blocks(keys.n, kOver, t0, t1);
     const float* kh = c.kv.k + hk * c.kv.kl.head;
     const float* vh = c.kv.v + hk * c.kv.vl.head;
 
@@ -375,29 +375,8 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
   }
 }
 
-// Workgroups: as many as are resident at once, so that equal shares end together; a share is at least 128
-// keys.  Up to 512 keys a list, a workgroup takes it whole, which saves the second launch.
+// Workgroups that are resident at once, so that equal shares end together.
 int resident(int D) { return (D <= 64 ? 3 : D <= 128 ? 2 : 1) * bch::device_cu_count(); }
-
-SharePlan rows_plan(const PagedCall& c, int max_len, int row_limit, bool may_split) {
-  SharePlan p;
-  const int group = c.H / c.Hkv;
-  p.row_min = 1;
-  p.row_max = row_limit;
-  const int most = (int)std::min((long long)c.seqs.max_new * group, (long long)row_limit / group * group);
-  p.tiles = (most + kRows - 1) / kRows;
-  p.part_rows = std::min(most, kRows);
-  p.min_share = 8 + kOver;
-  p.slots = 1;
-  if (p.tiles == 0) return p;
-  const long long blocks = bch::most_keys(c, max_len) / kBlk + 3;
-  if (may_split && blocks > 512 / kBlk + 3) {
-    const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p), most_bytes = 512LL << 20;
-    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, (long long)resident(c.D) + 1, most_bytes / part});
-    if (p.slots < 2) p.slots = 1;
-  }
-  return p;
-}
 
 template <int DP>
 void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
@@ -413,28 +392,40 @@ void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws)
 
 namespace bch {
 
+// A share is at least 128 keys.  Up to 512 keys a list, a workgroup takes it whole, which saves the second
+// launch.
+SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, bool may_split) {
+  SharePlan p;
+  const int group = c.H / c.Hkv;
+  p.row_min = 1;
+  p.row_max = row_limit;
+  const int most = (int)std::min((long long)c.seqs.max_new * group, (long long)row_limit / group * group);
+  p.tiles = (most + kRows - 1) / kRows;
+  p.part_rows = std::min(most, kRows);
+  p.min_share = 8 + kOver;
+  p.slots = 1;
+  if (p.tiles == 0) return p;
+  const long long blocks = bch::most_keys(c, max_len) / kBlk + 3;
+  if (may_split && blocks > 512 / kBlk + 3 && fits_grid(lists_of(c, p) * (kRows / 4), 512)) {
+    const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p), most_bytes = 512LL << 20;
+    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, (long long)resident(c.D) + 1, most_bytes / part});
+    if (p.slots < 2) p.slots = 1;
+  }
+  return p;
+}
+
 bool sdpa_paged_rows_applies(const PagedCall& c, int row_limit) {
   const long long rows = std::min((long long)c.seqs.max_new * (c.H / c.Hkv), (long long)row_limit);
   return c.D >= 4 && c.D <= 256 && rows <= 0x7fffffff - kRows &&
-         (long long)c.B * c.Hkv * ((rows + kRows - 1) / kRows) * kRows <= 0x7fffffffLL;
+         fits_grid((long long)c.B * c.Hkv * ((rows + kRows - 1) / kRows), 64 * kWaves);
 }
 
-size_t sdpa_paged_rows_workspace_bytes(const PagedCall& c, int max_len, int row_limit) {
-  return share_bytes(c, rows_plan(c, max_len, row_limit, true));
-}
-
-hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, int max_len, int row_limit, void* ws,
-                                  size_t ws_bytes) {
-  const SharePlan p = rows_plan(c, max_len, row_limit,
-                               ws_bytes >= sdpa_paged_rows_workspace_bytes(c, max_len, row_limit));
-  float* w = static_cast<float*>(ws);
+hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
   if (p.tiles == 0) return hipSuccess;  // a token alone has more rows than the limit
-  if (c.D <= 64) launch_dp<64>(s, c, p, w);
-  else if (c.D <= 128) launch_dp<128>(s, c, p, w);
-  else launch_dp<256>(s, c, p, w);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.slots == 1) return e;
-  return launch_paged_combine(s, c, p, kRows, w);
+  if (c.D <= 64) launch_dp<64>(s, c, p, ws);
+  else if (c.D <= 128) launch_dp<128>(s, c, p, ws);
+  else launch_dp<256>(s, c, p, ws);
+  return hipGetLastError();
 }
 
 }  // namespace bch

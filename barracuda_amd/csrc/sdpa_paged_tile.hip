@@ -54,7 +54,8 @@ __device__ __forceinline__ float half_swap_sum(float x) {
 // QL of the eight 16-d steps is kept in LDS too, which leaves two wavefronts per SIMD their registers.
 template <int DP>
 struct TileCfg {
-  static constexpr int NW = 8, NT = 64 * NW, BQ = 32 * NW;
+  static constexpr int NW = 8, NT = 64 * NW, BQ = bch::kTileRows;
+  static_assert(BQ == 32 * NW, "32 rows a wavefront");
   static constexpr int NO = DP / 8;
   static constexpr int KSTR = kBKV * 16, VSTR = DP * 16;
   static constexpr int KBYTES = 3 * NO * KSTR, VBYTES = 3 * 4 * VSTR;
@@ -107,7 +108,7 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
       // a workgroup a tile, last ones first (without a window the longest), all heads of a tile together: with
       // B * Hkv a multiple of 8 the tiles of a head share an XCD's L2
       const int nbk = c.B * c.Hkv, bk = blockIdx.x % nbk;
-      mine = {bk / c.Hkv, bk % c.Hkv, (int)(plan.tiles - 1 - blockIdx.x / nbk), 0, 0, 0, 1};
+      mine = {bk / c.Hkv, bk % c.Hkv, (int)(plan.tiles - 1 - blockIdx.x / nbk), 0, 0, 0, 1, true};
       more = false;
     }
     const int b = mine.b, hk = mine.hk, tile = mine.rb;
@@ -174,8 +175,8 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     };
     reset();
 
-    const int t0 = plan.slots > 1 ? min(max(mine.p0 - kOver, 0), keys.n) : 0;
-    const int t1 = plan.slots > 1 ? min(max(mine.p1 - kOver, 0), keys.n) : keys.n;
+    int t0, t1;
+    mine.blocks(keys.n, kOver, t0, t1);
 
     // ---- where block t's keys stand: lanes 0 .. 31 of the calling wavefront ----
     struct Found {
@@ -604,31 +605,6 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
   }
 }
 
-// Fewer tiles than two a CU: equal shares of their key blocks, a workgroup each, a share eight blocks at
-// least.  More: a workgroup a tile.
-SharePlan tile_plan(const PagedCall& c, int max_len, bool may_split) {
-  constexpr int kRows = TileCfg<32>::BQ;
-  SharePlan p;
-  const int group = c.H / c.Hkv;
-  const long long cu = bch::device_cu_count();
-  p.row_min = bch::kTileRows + 1;
-  p.row_max = 0x7fffffff;
-  const int most = c.seqs.max_new * group;
-  p.tiles = (most - 1) / kRows + 1;
-  p.part_rows = std::min(most, kRows);
-  p.min_share = 8 + kOver;
-  p.slots = 1;
-  // full tiles that there are: a batch's rows, or every sequence's
-  const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
-  const long long blocks = bch::most_keys(c, max_len) / kBKV + 3;
-  if (may_split && rows / kRows < 2 * cu) {
-    const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p);
-    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, cu + 1, (512LL << 20) / part});
-    if (p.slots < 2) p.slots = 1;
-  }
-  return p;
-}
-
 template <int DP>
 void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
   const long long lists = bch::lists_of(c, p);
@@ -643,26 +619,42 @@ void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws)
 
 namespace bch {
 
+// Fewer tiles than two a CU: equal shares of their key blocks, a workgroup each, a share eight blocks at
+// least.  More: a workgroup a tile.
+SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) {
+  SharePlan p;
+  const int group = c.H / c.Hkv;
+  const long long cu = device_cu_count();
+  p.row_min = kFewRows + 1;
+  p.row_max = 0x7fffffff;
+  const int most = c.seqs.max_new * group;
+  p.tiles = (most - 1) / kTileRows + 1;
+  p.part_rows = std::min(most, kTileRows);
+  p.min_share = 8 + kOver;
+  p.slots = 1;
+  // full tiles that there are: a batch's rows, or every sequence's
+  const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
+  const long long blocks = most_keys(c, max_len) / kBKV + 3;
+  if (may_split && rows / kTileRows < 2 * cu && fits_grid(lists_of(c, p) * (kTileRows / 4), 512)) {
+    const long long part = sizeof(float) * part_floats(p, c.D) * lists_of(c, p);
+    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, cu + 1, (512LL << 20) / part});
+    if (p.slots < 2) p.slots = 1;
+  }
+  return p;
+}
+
 bool sdpa_paged_tile_applies(const PagedCall& c) {
   const long long rows = (long long)c.seqs.max_new * (c.H / c.Hkv);
-  return c.D >= 8 && c.D <= 128 && rows > kTileRows && rows <= 0x7fffffff - 256 &&
-         (long long)c.B * c.Hkv * ((rows + 255) / 256) * 16 <= 0x7fffffffLL;
+  return c.D >= 8 && c.D <= 128 && rows > kFewRows && rows <= 0x7fffffff - 256 &&
+         fits_grid((long long)c.B * c.Hkv * ((rows + 255) / 256), TileCfg<32>::NT);
 }
 
-size_t sdpa_paged_tile_workspace_bytes(const PagedCall& c, int max_len) {
-  return share_bytes(c, tile_plan(c, max_len, true));
-}
-
-hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes) {
-  const SharePlan p = tile_plan(c, max_len, ws_bytes >= sdpa_paged_tile_workspace_bytes(c, max_len));
-  float* w = static_cast<float*>(ws);
-  if (c.D <= 32) launch_dp<32>(s, c, p, w);
-  else if (c.D <= 64) launch_dp<64>(s, c, p, w);
-  else if (c.D <= 96) launch_dp<96>(s, c, p, w);
-  else launch_dp<128>(s, c, p, w);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.slots == 1) return e;
-  return launch_paged_combine(s, c, p, TileCfg<32>::BQ, w);
+hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
+  if (c.D <= 32) launch_dp<32>(s, c, p, ws);
+  else if (c.D <= 64) launch_dp<64>(s, c, p, ws);
+  else if (c.D <= 96) launch_dp<96>(s, c, p, ws);
+  else launch_dp<128>(s, c, p, ws);
+  return hipGetLastError();
 }
 
 }  // namespace bch
