@@ -103,7 +103,7 @@ __device__ __forceinline__ long long slot_offset(const SdpaLayout& l, Slot s) {
 }
 
 // Ancestor masks of a tree's n <= kMaxDrafts drafts, by pointer jumping: every step joins a draft's
-// ancestors with those of its furthest one so far, so seven steps reach the root.  A parent that is not
+// ancestors with those of its furthest one so far, so log2(n) steps reach the root.  A parent that is not
 // below its draft (or is negative) makes it a root.  All threads of the workgroup (kMaxDrafts at
 // least) call; mask[i] then holds i and the ancestors that the window leaves, depth[i] their number.
 struct TreeMasks {
@@ -120,7 +120,7 @@ __device__ __forceinline__ void tree_masks(TreeMasks& t, const int* parent, cons
     for (int w = 0; w < 4; ++w) t.mask[i][w] = (i >> 5) == w ? 1u << (i & 31) : 0u;
   }
   __syncthreads();
-  for (int step = 1; step < kMaxDrafts; step *= 2) {
+  for (int step = 1; step < s.n; step *= 2) {
     const int p = on ? t.next[i] : -1;
     unsigned m[4] = {0, 0, 0, 0};
     int np = -1;
@@ -228,6 +228,11 @@ __device__ __forceinline__ long long uniform(long long v) {
                      (unsigned)__builtin_amdgcn_readfirstlane((int)v));
 }
 
+// a / b of a >= 0, b > 0; the 64-bit division takes a microsecond.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
 // BLK keys a block, ROWS rows a block, OVER blocks for a list's beginning and end.
 template <int BLK, int ROWS, int OVER, bool TREE>
 struct Shares {
@@ -275,13 +280,14 @@ struct Shares {
     }
     // a list of length w is cut into at most ceil((w - 1) / share) + 1 parts
     const long long grid = gridDim.x, slots = plan.slots - 1;
-    long long share = max(max((long long)plan.min_share, (total + grid - 1) / grid), (longest + slots - 1) / slots);
+    long long share = max(max((long long)plan.min_share, quotient(total + grid - 1, grid)),
+                          quotient(longest + slots - 1, slots));
     // parts of one list each: ceil(w / part) <= w / part + 1 of them, in all no more than workgroups; up to a
     // twentieth longer than the shares
     int part = 0;
     if (lists < grid) {
-      const long long p = max((long long)plan.min_share, (total + grid - lists - 1) / (grid - lists));
-      if (20 * p <= 21 * share && (longest - 1) / p < plan.slots) part = (int)p;
+      const long long p = max((long long)plan.min_share, quotient(total + grid - lists - 1, grid - lists));
+      if (20 * p <= 21 * share && quotient(longest - 1, p) < plan.slots) part = (int)p;
     }
     if (part || c.B > 64) seqs = line(c, plan, 0, lane, part);
     f.seqs[lane] = seqs;
@@ -320,12 +326,12 @@ struct Shares {
       const int at = __builtin_amdgcn_readfirstlane(__popcll(__ballot(before + seqs.sum <= x)));
       const int tiles = __builtin_amdgcn_readlane(seqs.tiles, at), length = __builtin_amdgcn_readlane(seqs.length, at);
       const long long off = x - before - (at > 0 ? uniform(__shfl(seqs.sum, at - 1)) : 0);
-      const int list = (int)(off / length), p0 = (int)(off - (long long)list * length);
+      const int list = (int)quotient(off, length), p0 = (int)(off - (long long)list * length);
       const int p1 = (int)min((long long)length, p0 + x1 - x);
       // parts: the list begins at x - p0 and is cut at multiples of the share
       const long long begin = x - p0;
-      const int slot = begin >= x0 ? 0 : (int)((x0 - begin + share - 1) / share);
-      count = begin + length <= x0 + share ? slot + 1 : slot + 1 + (int)((begin + length - x0 - 1) / share);
+      const int slot = begin >= x0 ? 0 : (int)quotient(x0 - begin + share - 1, share);
+      count = begin + length <= x0 + share ? slot + 1 : slot + 1 + (int)quotient(begin + length - x0 - 1, share);
       if (lane == 0) {
         f.x = x + p1 - p0;
         f.before = before;

@@ -91,46 +91,80 @@ __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCal
 // wavefront per row, lane s the maximum and sum of part s, lane d (and on by 64) the columns.  A part
 // without a key that the row sees has l = 0 and counts nothing; a row without any gives zeros.  Rows of a
 // list that was not cut are there already.  Trips to memory bound it: the rows of eight parts are loaded
-// before they are added.  The lists of both kernels in one launch: the first workgroups (four
-// rows each) have those of the tiles.
+// before they are added.  Both kernels' rows in one launch, a wavefront per row of q that there is (with one
+// per row that a sequence might have, those with nothing to do took 12 of 20 us for seven ragged chunks).
 struct Combined {
   bch::SharePlan plan;
-  int block_rows, groups;
+  int block_rows;
   const float* ws;
 };
-__global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile, Combined rows16) {
-  const bool is_tile = (int)blockIdx.x < tile.groups;
-  const Combined& k = is_tile ? tile : rows16;
-  const bch::SharePlan& plan = k.plan;
-  const int per_list = k.block_rows / 4, at = is_tile ? blockIdx.x : blockIdx.x - tile.groups, list = at / per_list;
-  const int rb = list % plan.tiles, bk = list / plan.tiles, b = bk / c.Hkv, hk = bk - b * c.Hkv;
-  const Seq s = bch::load_seq(c.kv, c.seqs, b);
-  const int group = c.H / c.Hkv;
-  const long long rows = (long long)s.n * group;
-  const int lane = threadIdx.x & 63, r = (at % per_list) * 4 + (threadIdx.x >> 6);  // within the row block
-  const long long row = (long long)rb * k.block_rows + r;
-  if (row >= rows || rows < plan.row_min || rows > plan.row_max) return;
-  const int count = reinterpret_cast<const int*>(k.ws)[list];
-  if (count <= 1) return;
-  const long long per = bch::part_floats(plan, c.D);
-  const float* p = k.ws + bch::counts_floats((long long)c.B * c.Hkv * plan.tiles) + (long long)list * plan.slots * per;
-  const float* ml = p + (long long)plan.part_rows * c.D + 2 * r;
+// most > 0: the tokens of a sequence that are looked at; else all rows of q.
+__global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile, Combined rows16, int most) {
+  const int lane = threadIdx.x & 63;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  int tok0 = (int)(at / c.H);
+  const int h = (int)(at - (long long)tok0 * c.H);
+  // the token's sequence b, with rows row0 .. end - 1 (as load_seq)
+  int b = 0, row0 = 0, end = 0;
+  if (most > 0) {
+    b = tok0 / most;
+    if (b >= c.B) return;
+    row0 = c.seqs.start[b];
+    end = c.seqs.start[b + 1];
+    tok0 = max(row0, 0) + tok0 % most;
+  } else if (c.seqs.start) {
+    if (tok0 >= c.seqs.total) return;
+    for (int b0 = 0; b0 < c.B; b0 += 64) {
+      const int e = c.seqs.start[min(b0 + lane, c.B - 1) + 1], first = b0 == 0 ? c.seqs.start[0] : end;
+      const int n = __popcll(__ballot(b0 + lane < c.B && e <= tok0));
+      b += n;
+      row0 = n > 0 ? __shfl(e, n - 1) : first;
+      end = __shfl(e, min(n, 63));
+      if (n < 64) break;
+    }
+  } else {
+    b = tok0 / c.seqs.max_new;
+    row0 = b * c.seqs.max_new;
+    end = row0 + c.seqs.max_new;
+  }
+  row0 = max(row0, 0);
+  const int n = min(min(end, c.seqs.start ? c.seqs.total : end) - row0, c.seqs.max_new), tok = tok0 - row0;
+  if (b >= c.B || tok < 0 || tok >= n) return;
+  const int group = c.H / c.Hkv, hk = h / group;
+  const long long rows = (long long)n * group, row = (long long)tok * group + h - hk * group;
+  const bool is_tile = tile.plan.slots > 1 && rows >= tile.plan.row_min;
+  if (!is_tile && (rows16.plan.slots <= 1 || rows > rows16.plan.row_max)) return;
+  const int block_rows = is_tile ? tile.block_rows : rows16.block_rows, slots = is_tile ? tile.plan.slots : rows16.plan.slots;
+  const int tiles = is_tile ? tile.plan.tiles : rows16.plan.tiles;
+  const int part_rows = is_tile ? tile.plan.part_rows : rows16.plan.part_rows;
+  const float* const ws = is_tile ? tile.ws : rows16.ws;
+  const long long list = ((long long)b * c.Hkv + hk) * tiles + row / block_rows;
+  const int r = (int)(row % block_rows);
+  const long long per = (long long)part_rows * (c.D + 2);
+  const float* p = ws + bch::counts_floats((long long)c.B * c.Hkv * tiles) + list * slots * per;
+  const float* ml = p + (long long)part_rows * c.D + 2 * r;
   const float* po = p + (long long)r * c.D;
-  float m = -INFINITY;
-  for (int u0 = 0; u0 < count; u0 += 64)
+  // the first 64 parts' maxima and sums come with the number of parts
+  float ms = ml[min(lane, slots - 1) * per], ls = ml[min(lane, slots - 1) * per + 1];
+  const int count = reinterpret_cast<const int*>(ws)[list];
+  if (count <= 1) return;
+  float m = bch::wave_allreduce(lane < count ? ms : -INFINITY, bch::OpMax());
+  for (int u0 = 64; u0 < count; u0 += 64)
     m = fmaxf(m, bch::wave_allreduce(u0 + lane < count ? ml[(u0 + lane) * per] : -INFINITY, bch::OpMax()));
-  const int tok = (int)(row / group);
-  float* dst = c.o + b * c.ol.batch + (long long)(s.row0 + tok) * c.ol.row +
-               (hk * group + row - (long long)tok * group) * c.ol.head;
+  float* dst = c.o + (c.seqs.start ? (long long)tok0 * c.ol.row : b * c.ol.batch + (long long)tok * c.ol.row) +
+               h * c.ol.head;
   for (int d0 = 0; d0 < c.D; d0 += 128) {
     const int da = min(d0 + lane, c.D - 1), db = min(d0 + lane + 64, c.D - 1);
     float x = 0.0f, y = 0.0f, l = 0.0f;
     for (int u0 = 0; u0 < count; u0 += 64) {
       const bool on = u0 + lane < count;
       const int n = min(64, count - u0);
-      const float ms = on ? ml[(u0 + lane) * per] : -INFINITY, ls = on ? ml[(u0 + lane) * per + 1] : 0.0f;
-      const float a = __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.0f : m));
-      l += bch::wave_allreduce(a * ls, bch::OpSum());
+      if (count > 64) {
+        ms = ml[min(u0 + lane, count - 1) * per];
+        ls = ml[min(u0 + lane, count - 1) * per + 1];
+      }
+      const float a = on ? __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.0f : m)) : 0.0f;
+      l += bch::wave_allreduce(on ? a * ls : 0.0f, bch::OpSum());
       for (int u = 0; u < n; u += 8) {
         float vx[8], vy[8];
 #pragma unroll
@@ -161,6 +195,8 @@ struct Route {
   size_t tile_bytes, bytes;
 };
 Route route(const PagedCall& c, int max_len, bool may_split) {
+  const long long all = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
+  if (!bch::fits_grid(all / 4 + 1, 256)) may_split = false;  // paged_combine's
   Route r{};
   r.tile = bch::sdpa_paged_tile_applies(c);
   const int row_limit = r.tile ? bch::kFewRows : 0x7fffffff;
@@ -190,11 +226,14 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, r.tile_plan, tile_ws) : hipSuccess;
     if (e == hipSuccess && r.rows) e = launch_sdpa_paged_rows(s, c, r.rows_plan, rows_ws);
     if (e != hipSuccess || r.bytes == 0) return e;
-    auto part = [&](const SharePlan& p, int block_rows, const float* w) {
-      return Combined{p, block_rows, p.slots > 1 ? (int)(lists_of(c, p) * (block_rows / 4)) : 0, w};
-    };
-    const Combined a = part(r.tile_plan, kTileRows, tile_ws), b = part(r.rows_plan, kShortRows, rows_ws);
-    hipLaunchKernelGGL(paged_combine, dim3((unsigned)a.groups + (unsigned)b.groups), dim3(256), 0, s, c, a, b);
+    const Combined a{r.tile_plan, kTileRows, tile_ws}, b{r.rows_plan, kShortRows, rows_ws};
+    const long long rows = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
+    // where only short sequences can have been cut, their first tokens, if those are fewer
+    const int group = c.H / c.Hkv, few = std::min(kFewRows / group, c.seqs.max_new);
+    const bool only_few = r.tile && r.tile_plan.slots == 1 && (long long)c.B * few * c.H < rows;
+    const long long waves = only_few ? (long long)c.B * few * c.H : rows;
+    if (waves == 0) return hipSuccess;
+    hipLaunchKernelGGL(paged_combine, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, c, a, b, only_few ? few : 0);
     return hipGetLastError();
   }
   const long long tiles = ((long long)c.seqs.max_new * c.H + kAnyWaves - 1) / kAnyWaves;

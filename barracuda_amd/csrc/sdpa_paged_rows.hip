@@ -8,7 +8,8 @@
 //   * Keys: the sink blocks and the window's blocks of 16 keys of a row block are one list, and the lists of
 //     all row blocks, key/value heads and sequences one line that is cut into equal shares, a workgroup
 //     each, whatever the lengths of the sequences: a share may hold the end of one list, whole ones and the
-//     beginning of another.  The four wavefronts of a workgroup take a list's blocks in turn.  K and V go from global memory
+//     beginning of another.  The four wavefronts of a workgroup (eight, where it takes one list whole) take a
+//     list's blocks in turn.  K and V go from global memory
 //     straight into the operand registers of v_mfma_f32_16x16x4_f32, the next block's loads in flight and
 //     the page numbers of the one after that.  No barrier until the end.
 //   * S^T = K Q^T: lane (g = l / 16, i = l % 16) holds K[key i][16 c + 4 g .. + 3] and q[row i] alike; value r
@@ -21,7 +22,7 @@
 //     not held) have their V rows zeroed, whatever stands there; masked scores are -inf.  A weight of 0
 //     still turns an infinite V that only some rows see into NaN, so a wavefront whose result is not
 //     finite does its blocks again with those values added by the vector unit, to the rows that see them.
-//   * Each wavefront keeps its own lazily moved reference maximum, sum and O; the four meet in LDS, and the
+//   * Each wavefront keeps its own lazily moved reference maximum, sum and O; they meet in LDS, and the
 //     results of a list that was cut in paged_combine.  Fixed cuts and order: deterministic.
 #include "paged.h"
 
@@ -39,7 +40,6 @@ using bch::SharePlan;
 constexpr float kLazy = 8.0f;  // log2 headroom before the reference max moves
 constexpr int kRows = bch::kShortRows;  // rows per workgroup
 constexpr int kBlk = 16;       // keys per block
-constexpr int kWaves = 4;
 
 __device__ __forceinline__ float quad_max(float x) {
   auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -76,7 +76,7 @@ __device__ __forceinline__ f32x4 once(f32x4 x, int d0, int D) {
 // A list's beginning and end take about 3 us, in which a workgroup reads three blocks when the chip is full.
 constexpr int kOver = 3;
 
-template <int DP, bool FULL, bool TREE>
+template <int DP, int kWaves, bool FULL, bool TREE>
 __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows_kernel(PagedCall c, SharePlan plan,
                                                                                       float* __restrict__ ws) {
   constexpr int NC = DP / 16, NH = DP / 64;
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
       }
     }
 
-    // ---- the four wavefronts' results, in wavefront order ----
+    // ---- the wavefronts' results, in wavefront order ----
     if (g == 0) {
       red_m[wave][i] = m_ref;
       red_l[wave][i] = l_run;
@@ -378,14 +378,19 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
 // Workgroups that are resident at once, so that equal shares end together.
 int resident(int D) { return (D <= 64 ? 3 : D <= 128 ? 2 : 1) * bch::device_cu_count(); }
 
-template <int DP>
+template <int DP, int WAVES>
 void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
-  const long long lists = bch::lists_of(c, p);
-  const dim3 grid((unsigned)(p.slots > 1 ? (long long)resident(c.D) : lists)), block(64 * kWaves);
+  const dim3 grid((unsigned)(p.slots > 1 ? (long long)resident(c.D) : bch::lists_of(c, p))), block(64 * WAVES);
   const bool full = c.D == DP, tree = c.parent != nullptr;
-  auto kern = full ? (tree ? sdpa_paged_rows_kernel<DP, true, true> : sdpa_paged_rows_kernel<DP, true, false>)
-                   : (tree ? sdpa_paged_rows_kernel<DP, false, true> : sdpa_paged_rows_kernel<DP, false, false>);
+  auto kern = full ? (tree ? sdpa_paged_rows_kernel<DP, WAVES, true, true> : sdpa_paged_rows_kernel<DP, WAVES, true, false>)
+                   : (tree ? sdpa_paged_rows_kernel<DP, WAVES, false, true> : sdpa_paged_rows_kernel<DP, WAVES, false, false>);
   hipLaunchKernelGGL(kern, grid, block, 0, s, c, p, ws);
+}
+// A list that one workgroup takes whole: eight wavefronts, where the registers leave that many room.
+template <int DP>
+void launch_waves(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
+  if (p.slots == 1 && DP <= 128) launch_dp<DP, DP <= 128 ? 8 : 4>(s, c, p, ws);
+  else launch_dp<DP, 4>(s, c, p, ws);
 }
 
 }  // namespace
@@ -406,7 +411,7 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
   p.slots = 1;
   if (p.tiles == 0) return p;
   const long long blocks = bch::most_keys(c, max_len) / kBlk + 3;
-  if (may_split && blocks > 512 / kBlk + 3 && fits_grid(lists_of(c, p) * (kRows / 4), 512)) {
+  if (may_split && blocks > 512 / kBlk + 3) {
     const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p), most_bytes = 512LL << 20;
     p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, (long long)resident(c.D) + 1, most_bytes / part});
     if (p.slots < 2) p.slots = 1;
@@ -417,14 +422,14 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
 bool sdpa_paged_rows_applies(const PagedCall& c, int row_limit) {
   const long long rows = std::min((long long)c.seqs.max_new * (c.H / c.Hkv), (long long)row_limit);
   return c.D >= 4 && c.D <= 256 && rows <= 0x7fffffff - kRows &&
-         fits_grid((long long)c.B * c.Hkv * ((rows + kRows - 1) / kRows), 64 * kWaves);
+         fits_grid((long long)c.B * c.Hkv * ((rows + kRows - 1) / kRows), 512);
 }
 
 hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
   if (p.tiles == 0) return hipSuccess;  // a token alone has more rows than the limit
-  if (c.D <= 64) launch_dp<64>(s, c, p, ws);
-  else if (c.D <= 128) launch_dp<128>(s, c, p, ws);
-  else launch_dp<256>(s, c, p, ws);
+  if (c.D <= 64) launch_waves<64>(s, c, p, ws);
+  else if (c.D <= 128) launch_waves<128>(s, c, p, ws);
+  else launch_waves<256>(s, c, p, ws);
   return hipGetLastError();
 }
 

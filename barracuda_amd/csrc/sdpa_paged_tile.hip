@@ -635,7 +635,7 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
   const long long blocks = most_keys(c, max_len) / kBKV + 3;
-  if (may_split && rows / kTileRows < 2 * cu && fits_grid(lists_of(c, p) * (kTileRows / 4), 512)) {
+  if (may_split && rows / kTileRows < 2 * cu) {
     const long long part = sizeof(float) * part_floats(p, c.D) * lists_of(c, p);
     p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, cu + 1, (512LL << 20) / part});
     if (p.slots < 2) p.slots = 1;
