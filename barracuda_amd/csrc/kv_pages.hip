@@ -30,8 +30,9 @@ struct Elem<4> {
 
 // ---- append: row i of sequence b is key len[b] - n + i ----
 // A workgroup takes kAppend tokens of one sequence; a thread the same columns of each, K and V, with
-// all of its loads ahead of its stores.
-constexpr int kAppend = 4;
+// all of its loads ahead of its stores, past the caches (8 ragged prompts, 8391 tokens of 8 KB, 133 MB: 23.8 us,
+// 5.6 TB/s; through them, four tokens 29; past them, one token 28.8, four 24.9).
+constexpr int kAppend = 2;
 
 template <int VEC>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* k, float* v, KvSeqs seqs, int tiles,
@@ -55,14 +56,14 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* 
 #pragma unroll
     for (int u = 0; u < kAppend; ++u) {
       const long long row = s.row0 + min(i0 + u, s.n - 1);
-      x[u] = *reinterpret_cast<const T*>(nk + row * nkl.row + h * nkl.head + d);
-      y[u] = *reinterpret_cast<const T*>(nv + row * nvl.row + h * nvl.head + d);
+      x[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(nk + row * nkl.row + h * nkl.head + d));
+      y[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(nv + row * nvl.row + h * nvl.head + d));
     }
 #pragma unroll
     for (int u = 0; u < kAppend; ++u)
       if (slot[u].page >= 0) {
-        *reinterpret_cast<T*>(k + bch::slot_offset(kv.kl, slot[u]) + h * kv.kl.head + d) = x[u];
-        *reinterpret_cast<T*>(v + bch::slot_offset(kv.vl, slot[u]) + h * kv.vl.head + d) = y[u];
+        __builtin_nontemporal_store(x[u], reinterpret_cast<T*>(k + bch::slot_offset(kv.kl, slot[u]) + h * kv.kl.head + d));
+        __builtin_nontemporal_store(y[u], reinterpret_cast<T*>(v + bch::slot_offset(kv.vl, slot[u]) + h * kv.vl.head + d));
       }
   }
 }
@@ -81,30 +82,22 @@ struct PageShape {
   long long run, total;  // floats
 };
 
+// One access a thread, past the caches (1500 pages of 64 KB, K and V, 393 MB: 75 us, 5.2 TB/s; through them
+// 95; two or four accesses a thread past them 83, eight 131).
 template <int VEC>
 __global__ __launch_bounds__(kThreads) void kv_copy_kernel(PageShape ks, PageShape vs, Pairs pairs) {
   typedef typename Elem<VEC>::type T;
-  constexpr int U = 4;
   const PageShape& p = blockIdx.z & 1 ? vs : ks;
-  float* base = p.base + (blockIdx.z >> 1) * p.layer;
-  const float* src = base + pairs.src[blockIdx.y] * p.page;
-  float* dst = base + pairs.dst[blockIdx.y] * p.page;
-  T x[U];
-  long long off[U];
-  const long long e0 = ((long long)blockIdx.x * U * kThreads + threadIdx.x) * VEC;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const long long e = e0 + (long long)u * kThreads * VEC;
-    off[u] = -1;
-    if (e < p.total) {
-      const long long r = e / p.run;
-      off[u] = (r / p.n2) * p.s1 + (r % p.n2) * p.s2 + (e - r * p.run);
-      x[u] = *reinterpret_cast<const T*>(src + off[u]);
-    }
+  const long long e = ((long long)blockIdx.x * kThreads + threadIdx.x) * VEC;
+  if (e >= p.total) return;
+  long long off = e;
+  if (p.run != p.total) {
+    const long long r = e / p.run;
+    off = (r / p.n2) * p.s1 + (r % p.n2) * p.s2 + (e - r * p.run);
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u)
-    if (off[u] >= 0) *reinterpret_cast<T*>(dst + off[u]) = x[u];
+  float* base = p.base + (blockIdx.z >> 1) * p.layer + off;
+  const T x = __builtin_nontemporal_load(reinterpret_cast<const T*>(base + pairs.src[blockIdx.y] * p.page));
+  __builtin_nontemporal_store(x, reinterpret_cast<T*>(base + pairs.dst[blockIdx.y] * p.page));
 }
 
 PageShape page_shape(float* base, const SdpaLayout& l, long long layer, int Hkv, int page_size, int D) {
@@ -131,31 +124,36 @@ PageShape page_shape(float* base, const SdpaLayout& l, long long layer, int Hkv,
 // ---- keep: key to[b] + i = key keep[start[b] + i] ----
 // A thread owns its columns of a sequence's keys and moves them in ascending i, kKeep at a time, so
 // that a key is read before a later one of the same call takes its place (keep ascends and no key moves
-// up: to[b] + i <= keep[i] < keep[i + 1]).
+// up: to[b] + i <= keep[i] < keep[i + 1]).  Where the keys read lie behind all that are written, their order
+// does not matter, and `chunks` workgroups share them.
 constexpr int kKeep = 8;
 
 template <int VEC>
 __global__ __launch_bounds__(kThreads) void kv_keep_kernel(KvPages kv, float* k, float* v, long long k_layer,
-                                                           long long v_layer, int Hkv, int D, int total,
+                                                           long long v_layer, int Hkv, int D, int chunks, int total,
                                                            const int* start, const int* keep, const int* to) {
   typedef typename Elem<VEC>::type T;
-  const int b = blockIdx.y;
+  const int b = blockIdx.y, chunk = blockIdx.x % chunks;
   const bool is_v = blockIdx.z & 1;
   const SdpaLayout& l = is_v ? kv.vl : kv.kl;
   float* base = (is_v ? v : k) + (blockIdx.z >> 1) * (is_v ? v_layer : k_layer);
   const int a = min(max(start[b], 0), total), n = min(max(start[b + 1], a), total) - a;
   const int t0 = to[b], dv = D / VEC;
-  const int e = blockIdx.x * kThreads + threadIdx.x;
-  if (e >= Hkv * dv) return;
+  const int e = blockIdx.x / chunks * kThreads + threadIdx.x;
+  if (n == 0 || e >= Hkv * dv) return;
+  const bool apart = keep[a] >= (long long)t0 + n;
+  if (!apart && chunk > 0) return;
+  const int per = apart ? ((n - 1) / chunks / kKeep + 1) * kKeep : n;
+  const int i1 = (int)min((long long)n, ((long long)chunk + 1) * per);
   float* col = base + (e / dv) * l.head + (e % dv) * VEC;
-  for (int i0 = 0; i0 < n; i0 += kKeep) {
+  for (int i0 = chunk * per; i0 < i1; i0 += kKeep) {
     T x[kKeep];
     bch::Slot dst[kKeep];
 #pragma unroll
     for (int u = 0; u < kKeep; ++u) {
-      const int i = min(i0 + u, n - 1), j = keep[a + i];
+      const int i = min(i0 + u, i1 - 1), j = keep[a + i];
       const long long to_j = (long long)t0 + i;
-      const bool on = i0 + u < n && j > to_j && to_j >= 0;
+      const bool on = i0 + u < i1 && j > to_j && to_j >= 0;
       const bch::Slot src = on ? bch::key_slot(kv, b, j) : bch::Slot{-1, 0};
       dst[u] = src.page >= 0 ? bch::key_slot(kv, b, (int)to_j) : src;
       if (dst[u].page >= 0) x[u] = *reinterpret_cast<const T*>(col + bch::slot_offset(l, src));
@@ -195,7 +193,7 @@ hipError_t launch_kv_copy_pages(hipStream_t s, const KvPages& kv, float* k, floa
   const bool vec = vec4(kv, k, v, D) && k_layer % 4 == 0 && v_layer % 4 == 0;
   const PageShape ks = page_shape(k, kv.kl, k_layer, Hkv, kv.page_size, D);
   const PageShape vs = page_shape(v, kv.vl, v_layer, Hkv, kv.page_size, D);
-  const long long per = (long long)kThreads * 4 * (vec ? 4 : 1);
+  const long long per = (long long)kThreads * (vec ? 4 : 1);
   const long long chunks = (ks.total + per - 1) / per;
   if (chunks > 0x7fffffffLL / kThreads) return hipErrorInvalidConfiguration;
   for (int l0 = 0; l0 < layers; l0 += 16384) {
@@ -226,11 +224,15 @@ hipError_t launch_kv_keep(hipStream_t s, const KvPages& kv, float* k, float* v, 
   const bool vec = vec4(kv, k, v, D) && k_layer % 4 == 0 && v_layer % 4 == 0;
   const long long cols = (long long)Hkv * D / (vec ? 4 : 1);
   if (cols > 0x7fffffffLL - kThreads || B > 65535 || layers > 32767) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)((cols + kThreads - 1) / kThreads), B, 2 * layers), block(kThreads);
+  // 32 keys or more a workgroup on the average
+  const int chunks = (int)std::max(1LL, std::min(64LL, (long long)total / B / 32));
+  const long long blocks = (cols + kThreads - 1) / kThreads * chunks;
+  if (!fits_grid(blocks * B, kThreads) || !fits_grid(blocks * B * 2 * layers, 1)) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)blocks, B, 2 * layers), block(kThreads);
   if (vec)
-    hipLaunchKernelGGL(kv_keep_kernel<4>, grid, block, 0, s, kv, k, v, k_layer, v_layer, Hkv, D, total, start, keep, to);
+    hipLaunchKernelGGL(kv_keep_kernel<4>, grid, block, 0, s, kv, k, v, k_layer, v_layer, Hkv, D, chunks, total, start, keep, to);
   else
-    hipLaunchKernelGGL(kv_keep_kernel<1>, grid, block, 0, s, kv, k, v, k_layer, v_layer, Hkv, D, total, start, keep, to);
+    hipLaunchKernelGGL(kv_keep_kernel<1>, grid, block, 0, s, kv, k, v, k_layer, v_layer, Hkv, D, chunks, total, start, keep, to);
   return hipGetLastError();
 }
 
