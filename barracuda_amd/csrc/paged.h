@@ -212,16 +212,29 @@ inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
 
 // The lists of 64 sequences from b0 on, one sequence a lane.
 struct Lane64 {
+  Seq seq;
   int tiles, length;  // a list's place in the line
   long long sum;      // of all lists up to and with this sequence's
 };
+// A workgroup's piece of work: part `slot` of `count` (0: none left) of a list.
+struct Piece {
+  Seq seq;
+  int b, hk, rb, p0, p1, slot, count;
+  int parts;  // not 0: p0 is the part's number; else p0 .. p1 of the list's length
+  // its blocks, of the n that the row block's list has
+  __device__ __forceinline__ void blocks(int n, int over, int& t0, int& t1) const {
+    t0 = parts ? (int)((long long)n * p0 / count) : min(max(p0 - over, 0), n);
+    t1 = parts ? (int)((long long)n * (p0 + 1) / count) : min(max(p1 - over, 0), n);
+  }
+};
 // Where a workgroup is in its share [.., end): the next place x, the sequences around it (b0 on, `before` the
-// line before them), and what it is to do: p0 .. p1 of a list, part number slot of count (0: done).
+// line before them), and the piece it has and the next one, in turn.
 struct Share {
   Lane64 seqs[64];
   long long share, x, end, before;
-  int b0, b, hk, rb, p0, p1, slot, count;
+  int b0;
   int part;  // blocks a part, where each list is cut by itself (the line is then one of parts); else 0
+  Piece piece[2];
 };
 __device__ __forceinline__ long long uniform(long long v) {
   return (long long)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
@@ -237,9 +250,9 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 template <int BLK, int ROWS, int OVER, bool TREE>
 struct Shares {
   static __device__ __forceinline__ Lane64 line(const PagedCall& c, const SharePlan& plan, int b0, int lane, int part) {
-    Lane64 r{0, 1, 0};
+    Lane64 r{{0, 0, 0, 0}, 0, 1, 0};
     if (b0 + lane < c.B) {
-      const Seq s = load_seq(c.kv, c.seqs, b0 + lane);
+      const Seq s = r.seq = load_seq(c.kv, c.seqs, b0 + lane);
       const long long rows = (long long)s.n * (c.H / c.Hkv);
       if (rows > 0 && rows >= plan.row_min && rows <= plan.row_max) {
         r.tiles = ((int)rows - 1) / ROWS + 1;
@@ -307,8 +320,9 @@ struct Shares {
     }
   }
 
-  // The next list of the share, or the part of one; by the first wavefront, a barrier behind it.
-  static __device__ __forceinline__ void next(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
+  // The next list of the share, or the part of one, into piece[turn]; by the first wavefront, a barrier behind
+  // it.  It is called one piece ahead, so that its time does not stand between two pieces.
+  static __device__ __forceinline__ void next(Share& f, const PagedCall& c, const SharePlan& plan, int lane, int turn) {
     asm volatile("" ::: "memory");
     const long long x = uniform(f.x), x1 = uniform(f.end), share = uniform(f.share);
     int count = 0;
@@ -332,35 +346,21 @@ struct Shares {
       const long long begin = x - p0;
       const int slot = begin >= x0 ? 0 : (int)quotient(x0 - begin + share - 1, share);
       count = begin + length <= x0 + share ? slot + 1 : slot + 1 + (int)quotient(begin + length - x0 - 1, share);
+      if (lane == at) f.piece[turn] = {seqs.seq, b0 + at, list / tiles, list % tiles, p0, p1, slot, count, f.part};
       if (lane == 0) {
         f.x = x + p1 - p0;
         f.before = before;
         f.b0 = b0;
-        f.b = b0 + at;
-        f.hk = list / tiles;
-        f.rb = list % tiles;
-        f.p0 = p0;
-        f.p1 = p1;
-        f.slot = slot;
       }
     }
-    if (lane == 0) f.count = count;
+    if (lane == 0 && count == 0) f.piece[turn].count = 0;
   }
 };
 
-// A workgroup's piece of work: part `slot` of `count` (0: none left) of a list.
-struct Piece {
-  int b, hk, rb, p0, p1, slot, count;
-  bool parts;  // p0 is the part's number; else p0 .. p1 of the list's length
-  // its blocks, of the n that the row block's list has
-  __device__ __forceinline__ void blocks(int n, int over, int& t0, int& t1) const {
-    t0 = parts ? (int)((long long)n * p0 / count) : min(max(p0 - over, 0), n);
-    t1 = parts ? (int)((long long)n * (p0 + 1) / count) : min(max(p1 - over, 0), n);
-  }
-};
-__device__ __forceinline__ Piece read_piece(const Share& f) {
+__device__ __forceinline__ Piece read_piece(const Piece& f) {
   auto u = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-  return {u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1), u(f.slot), u(f.count), u(f.part) != 0};
+  return {{u(f.seq.row0), u(f.seq.n), u(f.seq.len), u(f.seq.first)}, u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1),
+          u(f.slot), u(f.count), u(f.parts)};
 }
 // Part `slot` of a list in the workspace; the list's number of parts is noted by its first.
 __device__ __forceinline__ float* part_of(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {

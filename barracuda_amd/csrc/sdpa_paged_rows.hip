@@ -73,8 +73,10 @@ __device__ __forceinline__ f32x4 once(f32x4 x, int d0, int D) {
   return x;
 }
 
-// A list's beginning and end take about 3 us, in which a workgroup reads three blocks when the chip is full.
-constexpr int kOver = 3;
+// What a list's beginning and end (the trips to memory for its pages and its first keys, the wavefronts'
+// results) cost in blocks when the chip is full: 32 ragged sequences (389 MB) took 110 us with 3, 84 with 8 to
+// 12, 85 with 16.
+constexpr int kOver = 8;
 
 template <int DP, int kWaves, bool FULL, bool TREE>
 __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows_kernel(PagedCall c, SharePlan plan,
@@ -88,27 +90,31 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
   const int D = c.D, group = c.H / c.Hkv;
 
   using Line = bch::Shares<kBlk, kRows, kOver, TREE>;
-  if (plan.slots > 1 && threadIdx.x < 64) Line::begin(find, c, plan, threadIdx.x);
+  if (plan.slots > 1 && threadIdx.x < 64) {
+    Line::begin(find, c, plan, threadIdx.x);
+    Line::next(find, c, plan, threadIdx.x, 0);
+  }
 
   int tree_of = -1;
-  for (bool more = true; more;) {
+  bool more = true;
+  for (int turn = 0; more; turn ^= 1) {
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // what follows from it is not held in registers from one piece to the next
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
     bch::Piece piece;
     if (plan.slots > 1) {
-      if (wave == 0) Line::next(find, c, plan, lane);
       __syncthreads();
-      piece = bch::read_piece(find);
+      piece = bch::read_piece(find.piece[turn]);
       if (piece.count == 0) break;
+      if (wave == 0) Line::next(find, c, plan, lane, turn ^ 1);
     } else {
       const int bk = blockIdx.x / plan.tiles;
-      piece = {bk / c.Hkv, bk % c.Hkv, (int)(blockIdx.x % plan.tiles), 0, 0, 0, 1, true};
+      piece = {bch::load_seq(c.kv, c.seqs, bk / c.Hkv), bk / c.Hkv, bk % c.Hkv, (int)(blockIdx.x % plan.tiles), 0, 0, 0, 1, 1};
       more = false;
     }
     const int b = piece.b, hk = piece.hk, rb = piece.rb, count = piece.count;
-    const bch::Seq s = bch::load_seq(c.kv, c.seqs, b);
+    const bch::Seq s = piece.seq;
     const int rows = s.n * group;
     if (plan.slots == 1 && (rb * kRows >= rows || rows > plan.row_max)) break;
     if constexpr (TREE) {
@@ -324,24 +330,21 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) m = fmaxf(m, red_m[w][i]);
       const float m_use = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f;
-      float a[kWaves];
+      // a wavefront without a key has m = -inf: its factor is 0 and so is its O
+      float f = __builtin_amdgcn_exp2f(m_ref - m_use), l = f * l_run;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        // a wavefront without a key has m = -inf: its factor is 0 and so is its O
-        a[w] = __builtin_amdgcn_exp2f(red_m[w][i] - m_use);
-        l += a[w] * red_l[w][i];
-      }
-#pragma unroll
-      for (int n = 0; n < 4 * NH; ++n) acc[n] *= a[0];
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w)
+      for (int n = 0; n < 4 * NH; ++n) acc[n] *= f;
+#pragma unroll 1
+      for (int w = 1; w < kWaves; ++w) {
+        f = __builtin_amdgcn_exp2f(red_m[w][i] - m_use);
+        l += f * red_l[w][i];
 #pragma unroll
         for (int h = 0; h < NH; ++h)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) acc[4 * h + e][r] += a[w] * red_o[w - 1][i][4 * (4 * g + r + 16 * h) + e];
+            for (int r = 0; r < 4; ++r) acc[4 * h + e][r] += f * red_o[w - 1][i][4 * (4 * g + r + 16 * h) + e];
+      }
 
       if (lane == 0) bch::note_count(ws, c, plan, piece);
       if (rb * kRows + i < rows) {

@@ -91,28 +91,33 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     return l;
   };
   using Line = bch::Shares<kBKV, G::BQ, kOver, TREE>;
-  if (plan.slots > 1 && threadIdx.x < 64) Line::begin(share, c, plan, threadIdx.x);
+  if (plan.slots > 1 && threadIdx.x < 64) {
+    Line::begin(share, c, plan, threadIdx.x);
+    Line::next(share, c, plan, threadIdx.x, 0);
+  }
 
   int tree_of = -1;
-  for (bool more = true; more;) {
+  bool more = true;
+  for (int turn = 0; more; turn ^= 1) {
     const int tid = anew(threadIdx.x);
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
     bch::Piece mine;
     if (plan.slots > 1) {
-      if (wave == 0) Line::next(share, c, plan, lane);
       __syncthreads();
-      mine = bch::read_piece(share);
+      mine = bch::read_piece(share.piece[turn]);
       if (mine.count == 0) break;
+      if (wave == 0) Line::next(share, c, plan, lane, turn ^ 1);
     } else {
       // a workgroup a tile, last ones first (without a window the longest), all heads of a tile together: with
       // B * Hkv a multiple of 8 the tiles of a head share an XCD's L2
       const int nbk = c.B * c.Hkv, bk = blockIdx.x % nbk;
-      mine = {bk / c.Hkv, bk % c.Hkv, (int)(plan.tiles - 1 - blockIdx.x / nbk), 0, 0, 0, 1, true};
+      mine = {bch::load_seq(c.kv, c.seqs, bk / c.Hkv), bk / c.Hkv, bk % c.Hkv, (int)(plan.tiles - 1 - blockIdx.x / nbk),
+              0, 0, 0, 1, 1};
       more = false;
     }
     const int b = mine.b, hk = mine.hk, tile = mine.rb;
-    const bch::Seq s = bch::load_seq(c.kv, c.seqs, b);
+    const bch::Seq s = mine.seq;
     const int group = c.H / c.Hkv, rows = s.n * group;
     if (plan.slots == 1 && (rows < plan.row_min || tile * G::BQ >= rows)) break;
     const bch::KeyList keys = bch::key_list<kBKV>(s, tile * G::BQ / group, (min(tile * G::BQ + G::BQ, rows) - 1) / group,
@@ -630,7 +635,7 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   const int most = c.seqs.max_new * group;
   p.tiles = (most - 1) / kTileRows + 1;
   p.part_rows = std::min(most, kTileRows);
-  p.min_share = 8 + kOver;
+  p.min_share = 4 + kOver;
   p.slots = 1;
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
