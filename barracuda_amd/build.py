@@ -7,7 +7,7 @@ Outputs (git-ignored, shipped with the tree):
     barracuda_amd/lib/libbarracuda_hip.so
     barracuda_amd/lib/bch_softmax_rows.hsaco
     oracle/libbc_oracle.so                  (test infrastructure only)
-    tests/cpp/bch_host_tests                (C++ host-API tests)
+    tests/cpp/bch_host_tests, bch_window_tests   (C++ host-API tests)
 """
 from __future__ import annotations
 
@@ -89,13 +89,13 @@ def build_hip(verbose: bool = True) -> Path:
 
 
 def build_host_tests(verbose: bool = True) -> Path:
-    """The C++ host-API tests (tests/cpp/test_ops.cpp) against include/barracuda_hip_ops.hpp."""
-    exe = ROOT / "tests" / "cpp" / "bch_host_tests"
-    _run(["g++", "-std=c++17", "-O2", "-Wall", "-Wextra", f"-I{ROOT / 'include'}",
-          str(ROOT / "tests" / "cpp" / "test_ops.cpp"), f"-L{LIB}", "-lbarracuda_hip",
-          "-Wl,-rpath,$ORIGIN/../../barracuda_amd/lib", "-o", str(exe)])
-    if verbose:
-        print(f"built {exe.relative_to(ROOT)}")
+    """The C++ host-API tests (tests/cpp/test_ops.cpp, test_window.cpp) against include/barracuda_hip_ops.hpp."""
+    cpp = ROOT / "tests" / "cpp"
+    for src, exe in (("test_window.cpp", cpp / "bch_window_tests"), ("test_ops.cpp", cpp / "bch_host_tests")):
+        _run(["g++", "-std=c++17", "-O2", "-Wall", "-Wextra", f"-I{ROOT / 'include'}", str(cpp / src), f"-L{LIB}",
+              "-lbarracuda_hip", "-Wl,-rpath,$ORIGIN/../../barracuda_amd/lib", "-o", str(exe)])
+        if verbose:
+            print(f"built {exe.relative_to(ROOT)}")
     return exe
 
 

@@ -146,7 +146,8 @@ __global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile,
   const float* po = p + (long long)r * c.D;
   // the first 64 parts' maxima and sums come with the number of parts
   float ms = ml[min(lane, slots - 1) * per], ls = ml[min(lane, slots - 1) * per + 1];
-  const int count = reinterpret_cast<const int*>(ws)[list];
+  // (starts that do not ascend name lists that nobody wrote: still no more than there is room for)
+  const int count = min(reinterpret_cast<const int*>(ws)[list], slots);
   if (count <= 1) return;
   float m = bch::wave_allreduce(lane < count ? ms : -INFINITY, bch::OpMax());
   for (int u0 = 64; u0 < count; u0 += 64)

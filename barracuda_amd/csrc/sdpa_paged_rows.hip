@@ -415,7 +415,7 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
   if (p.tiles == 0) return p;
   const long long blocks = bch::most_keys(c, max_len) / kBlk + 3;
   if (may_split && blocks > 512 / kBlk + 3) {
-    const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p), most_bytes = 512LL << 20;
+    const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p), most_bytes = 256LL << 20;
     p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, (long long)resident(c.D) + 1, most_bytes / part});
     if (p.slots < 2) p.slots = 1;
   }

@@ -323,10 +323,10 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     };
     auto cut = [&](int kb) {  // some row of the wavefront does not see some key of the block
       return kb + kBKV - 1 > pw_lo - (TREE ? 1 : 0) ||
-             (c.window > 0 && kb <= pw_hi - c.window && kb + kBKV > c.sinks);
+             (c.window > 0 && kb <= max(pw_hi, 0) - c.window && kb + kBKV > c.sinks);
     };
     auto unseen = [&](int kb) {  // none sees any
-      return r0w >= rows || kb > pw_hi || (c.window > 0 && kb + kBKV - 1 <= pw_lo - c.window && kb >= c.sinks);
+      return r0w >= rows || kb > pw_hi || (c.window > 0 && kb + kBKV - 1 <= max(pw_lo, 0) - c.window && kb >= c.sinks);
     };
 
     // Scores -> probabilities against the reference max, which moves when a block exceeds it by more than
@@ -642,7 +642,7 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   const long long blocks = most_keys(c, max_len) / kBKV + 3;
   if (may_split && rows / kTileRows < 2 * cu) {
     const long long part = sizeof(float) * part_floats(p, c.D) * lists_of(c, p);
-    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, cu + 1, (512LL << 20) / part});
+    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, cu + 1, (256LL << 20) / part});
     if (p.slots < 2) p.slots = 1;
   }
   return p;

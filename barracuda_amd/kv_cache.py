@@ -68,7 +68,7 @@ class KvStep:
     def __init__(self, cache: "KvCache", sequences: Sequence[int], counts: Sequence[int], parents):
         self._cache = cache
         self.sequences, self.counts = list(sequences), list(counts)
-        lens = [cache._seqs[s].length for s in sequences]
+        lens = self._lens = [cache._seqs[s].length for s in sequences]
         self.start = np.concatenate([[0], np.cumsum(counts, dtype=np.int64)]).astype(np.int64)
         self.total = int(self.start[-1])
         width = max([1] + [len(cache._seqs[s].pages) for s in sequences])
@@ -243,6 +243,8 @@ class KvCache:
         self._check_step("KvCache.keep", step, 0)
         if len(kept) != len(step.sequences):
             raise InvalidInput(f"KvCache.keep: {len(kept)} lists for {len(step.sequences)} sequences")
+        if any(self._seqs[s].length != length for s, length in zip(step.sequences, step._lens)):
+            raise InvalidOperation("KvCache.keep", "a later step has added tokens behind this one's")
         moves = []
         for s, n, ids in zip(step.sequences, step.counts, kept):
             ids = [int(x) for x in ids]

@@ -415,7 +415,9 @@ typedef struct bch_kv_batch {
  * reach it, infinite and NaN ones included.  A key whose score is -inf counts as
  * not seen.  Row r, head h of q is at r*row_stride + h*head_stride (batch_stride
  * is not used); query head h reads key/value head h / (H / Hkv).  o must not
- * overlap q, k or v.  D <= 1024; a tree has at most 128 drafts a sequence
+ * overlap q, k or v.  Keys are split over workgroups where that fills the chip,
+ * with the partial results in the context's workspace (512 MiB at most), or not
+ * where that may not grow (under capture, or out of memory).  D <= 1024; a tree has at most 128 drafts a sequence
  * (max_new; BCH_E_UNSUPPORTED beyond).  total, max_new or B of 0: nothing
  * happens. */
 bch_status bch_sdpa_paged(bch_ctx *ctx, const bch_kv_pages *kv,
@@ -427,7 +429,7 @@ bch_status bch_sdpa_paged(bch_ctx *ctx, const bch_kv_pages *kv,
 /* The same over dense operands (layouts as bch_sdpa_fwd_ex): row i of Sq stands
  * at position Skv - Sq + i, so with Sq < Skv the queries are the last ones of
  * their sequence, and with Sq > Skv the first Sq - Skv rows see nothing and get
- * zeros.  window 0 is causal attention; no tree. */
+ * zeros.  window 0 is causal attention; no tree.  D <= 1024. */
 bch_status bch_sdpa_window(bch_ctx *ctx, int B, int H, int Hkv, int Sq, int Skv,
                            int D, float scale, int window, int sinks,
                            const float *q, bch_attn_layout q_layout,

@@ -268,6 +268,9 @@ class Tensor {
   inline Result<Tensor> scaled_dot_product_attention(const Tensor& key, const Tensor& value) const;
   inline Result<Tensor> causal_attention(const Tensor& key, const Tensor& value) const;
   inline Result<Tensor> grouped_query_attention(const Tensor& key, const Tensor& value) const;
+  // window 0: every key up to the query's own; the first `sinks` keys stay visible
+  inline Result<Tensor> sliding_window_attention(const Tensor& key, const Tensor& value, size_t window,
+                                                 size_t sinks = 0) const;
   inline Result<Tensor> multi_head_attention(const Tensor& key, const Tensor& value, const Tensor& w_q,
                                              const Tensor& w_k, const Tensor& w_v, const Tensor& w_o,
                                              size_t num_heads) const;
@@ -605,6 +608,53 @@ struct GroupedQueryAttention {
   }
 };
 
+// Causal attention in which a query sees the last `window` keys up to its own (0: all of them) and the
+// first `sinks` keys: Q [B, Hq, Sq, D], K = V [B, Hkv, Skv, D], the queries the last Sq positions of the
+// Skv.  A query with no key in sight (Sq > Skv) gives zeros.  The reference has no windowed op; its causal
+// one (ops/causal_attn/mod.rs:64-158) is window 0 with Hq = Hkv and Sq = Skv.
+struct SlidingWindowAttention {
+  const Tensor& q;
+  const Tensor& k;
+  const Tensor& v;
+  size_t window;
+  size_t sinks = 0;
+  static std::optional<BarracudaError> validate(const std::vector<size_t>& qs, const std::vector<size_t>& ks,
+                                                const std::vector<size_t>& vs) {
+    if (qs.size() != 4 || ks.size() != 4 || vs.size() != 4)
+      return BarracudaError::invalid_input("All inputs must be 4D tensors [batch, heads, seq_len, head_dim]");
+    if (ks[0] != qs[0] || ks[3] != qs[3]) return BarracudaError::shape_mismatch(qs, ks);
+    if (vs != ks) return BarracudaError::shape_mismatch(ks, vs);
+    if (ks[1] == 0 || qs[1] % ks[1] != 0)
+      return BarracudaError::invalid_input("num_q_heads (" + std::to_string(qs[1]) +
+                                           ") must be divisible by num_kv_heads (" + std::to_string(ks[1]) + ")");
+    return std::nullopt;
+  }
+  Result<Tensor> execute() const {
+    const char* op = "sliding_window_attention";
+    if (auto e = validate(q.shape(), k.shape(), v.shape())) return *e;
+    if (q.device() != k.device() || q.device() != v.device())
+      return BarracudaError::device("All tensors must be on the same device");
+    const auto& s = q.shape();
+    const size_t B = s[0], Hq = s[1], Sq = s[2], D = s[3], Hkv = k.shape()[1], Skv = k.shape()[2];
+    if (auto e = detail::check_i32(op, {B, Hq, Sq, Skv, D})) return *e;
+    auto dev = q.device();
+    auto r = Tensor::empty(s, dev);
+    if (r.is_err() || B * Hq * Sq * D == 0) return r;
+    if (Skv == 0) return BarracudaError::invalid_op(op, "key sequence is empty (shape/dimension mismatch)");
+    Tensor out = std::move(r).unwrap();
+    const auto ql = detail::dense_layout(Hq, Sq, D), kl = detail::dense_layout(Hkv, Skv, D);
+    // a window or sinks beyond any position are the same as the largest int
+    const int w = (int)std::min(window, (size_t)INT_MAX), n = (int)std::min(sinks, (size_t)INT_MAX);
+    std::lock_guard<std::mutex> g(dev->mutex());
+    if (auto e = dev->check(bch_sdpa_window(dev->ctx(), (int)B, (int)Hq, (int)Hkv, (int)Sq, (int)Skv, (int)D,
+                                            1.0f / std::sqrt((float)D), w, n, q.data_ptr(), ql, k.data_ptr(), kl,
+                                            v.data_ptr(), kl, out.data_ptr(), ql),
+                            op))
+      return *e;
+    return out;
+  }
+};
+
 // ops/mha/mod.rs:48-187: query [B, Sq, D], key = value [B, Skv, D], four
 // [D, D] weights, num_heads dividing D.  Q' = query W_q etc. (three GEMMs),
 // attention per head over the [B, S, H, D/H] views of the projections (the
@@ -704,6 +754,10 @@ inline Result<Tensor> Tensor::causal_attention(const Tensor& key, const Tensor& 
 }
 inline Result<Tensor> Tensor::grouped_query_attention(const Tensor& key, const Tensor& value) const {
   return GroupedQueryAttention{*this, key, value}.execute();
+}
+inline Result<Tensor> Tensor::sliding_window_attention(const Tensor& key, const Tensor& value, size_t window,
+                                                       size_t sinks) const {
+  return SlidingWindowAttention{*this, key, value, window, sinks}.execute();
 }
 inline Result<Tensor> Tensor::multi_head_attention(const Tensor& key, const Tensor& value, const Tensor& w_q,
                                                    const Tensor& w_k, const Tensor& w_v, const Tensor& w_o,

@@ -235,6 +235,19 @@ def test_starts_are_clamped_to_the_rows(dev):
         c.output()  # padding and the rows behind stay
 
 
+def test_starts_that_do_not_ascend_stay_in_bounds(dev):
+    """Keys split over workgroups and starts that name no sequence's rows: nothing outside the rows is written."""
+    for news, starts in (([3, 2, 4], ([0, 7, 3, 9], [9, 0, 0, 5], [5, 2, 2**31 - 1, 1])),
+                         ([40, 100, 70], ([100, 0, 150, 30], [210, 1, 0, 90], [-8, 150, 10, 2**31 - 1]))):
+        c = Case(dev, [3000, 2500, 1800], news, 8, 2, 128, 16)
+        c.check()
+        for start in starts:
+            c.i32 = _I32(dev, start, c.lens, c.pool.table)
+            c.kv.table, c.batch.start, c.batch.len = c.i32.ptrs[2], c.i32.ptrs[0], c.i32.ptrs[1]
+            dev.check(c.call(dev._lib, dev.ctx), "attention")
+            c.output()
+
+
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf, np.finfo(np.float32).max])
 @pytest.mark.parametrize("lens,news,h,hkv,d,page", [
     ([170, 45], [1, 1], 4, 2, 64, 16), ([170, 45, 300], [50, 45, 130], 4, 2, 128, 16), ([200], [200], 3, 3, 80, 24)])
@@ -368,6 +381,17 @@ def test_dense_windows_beyond_any_position(dev):
     want = t[0].sliding_window_attention(t[1], t[2], 0).to_numpy()
     for window, sinks in ((50, 0), (2**31 - 1, 2**31 - 1), (2**40, 0), (1, 50), (3, 2**40)):
         assert np.array_equal(t[0].sliding_window_attention(t[1], t[2], window, sinks).to_numpy(), want), (window, sinks)
+
+
+@pytest.mark.parametrize("sq,skv", [(300, 100), (20, 7), (129, 128)])
+def test_dense_windows_beyond_any_position_with_more_rows_than_keys(dev, sq, skv):
+    rng = np.random.default_rng(sq)
+    q = rng.standard_normal((1, 2, sq, 64), dtype=np.float32)
+    k, v = (rng.standard_normal((1, 2, skv, 64), dtype=np.float32) for _ in range(2))
+    t = [Tensor.from_data(x, list(x.shape), dev) for x in (q, k, v)]
+    want = t[0].sliding_window_attention(t[1], t[2], 0).to_numpy()
+    for window in (skv, 2**31 - 1, 2**31 - 200):
+        assert np.array_equal(t[0].sliding_window_attention(t[1], t[2], window).to_numpy(), want), window
 
 
 def test_dense_strides_and_empty_batches(dev):

@@ -302,6 +302,17 @@ def test_stale_steps_and_bad_arguments_are_refused():
         KvCache(1, 0, 4, 2, 3, cache.device)
 
 
+def test_keep_of_a_step_with_a_later_one_behind_is_refused():
+    cache = _cache()
+    a = cache.new_sequence()
+    first = cache.batch([(a, 3)])
+    _append(cache, first, 0)
+    _append(cache, cache.batch([(a, 1)]), 3)
+    with pytest.raises(InvalidOperation):
+        cache.keep(first, [[0]])
+    assert _read(cache, a) == [0, 1, 2, 3]
+
+
 def test_sliding_window_attention_checks_shapes():
     def t(*s):
         x = Tensor.__new__(Tensor)
