@@ -195,19 +195,24 @@ struct SharePlan {
   int row_min, row_max;  // rows a key/value head of the sequences served
   int tiles;             // row blocks of the longest of them
   int part_rows;         // rows of a part: a row block's, if any sequence has as many
-  int slots;             // parts a list may be cut into; 1 (no workspace): a workgroup a list
+  int shares;            // workgroups of the line; 0 (no workspace): a workgroup a list
   int min_share;
 };
-// Workspace: the number of parts of every list, then the parts: rows of O, then (reference max, sum) pairs.
+// Workspace: for every list the workgroup of its first part and the number of its parts (in that workgroup and
+// the ones behind it), then two parts a workgroup, the one that ends a list begun before its share and the one
+// that its share leaves unended: rows of O, then (reference max, sum) pairs.
 __host__ __device__ inline long long part_floats(const SharePlan& p, int D) { return (long long)p.part_rows * (D + 2); }
-__host__ __device__ inline long long counts_floats(long long lists) { return (lists + 63) / 64 * 64; }
+__host__ __device__ inline long long notes_floats(long long lists) { return (2 * lists + 63) / 64 * 64; }
+__host__ __device__ inline long long part_at(const SharePlan& p, int first, int u, int D) {
+  return (2LL * (first + u) + (u == 0)) * part_floats(p, D);
+}
 inline long long lists_of(const PagedCall& c, const SharePlan& p) { return (long long)c.B * c.Hkv * p.tiles; }
 // A grid has fewer than 2^32 threads.
 inline bool fits_grid(long long workgroups, int threads) { return workgroups < (1LL << 32) / threads; }
 inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
-  if (p.slots <= 1) return 0;
+  if (p.shares == 0) return 0;
   const long long lists = lists_of(c, p);
-  return sizeof(float) * (size_t)(counts_floats(lists) + lists * p.slots * part_floats(p, c.D));
+  return sizeof(float) * (size_t)(notes_floats(lists) + 2LL * p.shares * part_floats(p, c.D));
 }
 
 // The lists of 64 sequences from b0 on, one sequence a lane.
@@ -278,29 +283,22 @@ struct Shares {
   static __device__ __forceinline__ void begin(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
     Lane64 seqs;
     long long total = 0, lists = 0;
-    int longest = 1;
     for (int b0 = 0; b0 < c.B; b0 += 64) {
       seqs = line(c, plan, b0, lane, 0);
       total += uniform(__shfl(seqs.sum, 63));
-      int w = seqs.tiles > 0 ? seqs.length : 1, n = seqs.tiles;
+      int n = seqs.tiles;
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        w = max(w, __shfl_xor(w, d));
-        n += __shfl_xor(n, d);
-      }
-      longest = max(longest, __builtin_amdgcn_readfirstlane(w));
+      for (int d = 1; d < 64; d *= 2) n += __shfl_xor(n, d);
       lists += (long long)c.Hkv * __builtin_amdgcn_readfirstlane(n);
     }
-    // a list of length w is cut into at most ceil((w - 1) / share) + 1 parts
-    const long long grid = gridDim.x, slots = plan.slots - 1;
-    long long share = max(max((long long)plan.min_share, quotient(total + grid - 1, grid)),
-                          quotient(longest + slots - 1, slots));
+    const long long grid = gridDim.x;
+    long long share = max((long long)plan.min_share, quotient(total + grid - 1, grid));
     // parts of one list each: ceil(w / part) <= w / part + 1 of them, in all no more than workgroups; up to a
     // twentieth longer than the shares
     int part = 0;
     if (lists < grid) {
       const long long p = max((long long)plan.min_share, quotient(total + grid - lists - 1, grid - lists));
-      if (20 * p <= 21 * share && quotient(longest - 1, p) < plan.slots) part = (int)p;
+      if (20 * p <= 21 * share && p <= 0x7fffffff) part = (int)p;
     }
     if (part || c.B > 64) seqs = line(c, plan, 0, lane, part);
     f.seqs[lane] = seqs;
@@ -362,14 +360,17 @@ __device__ __forceinline__ Piece read_piece(const Piece& f) {
   return {{u(f.seq.row0), u(f.seq.n), u(f.seq.len), u(f.seq.first)}, u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1),
           u(f.slot), u(f.count), u(f.parts)};
 }
-// Part `slot` of a list in the workspace; the list's number of parts is noted by its first.
+// Where a workgroup leaves its part of a list that was cut, and (the first part's) the list's note.
 __device__ __forceinline__ float* part_of(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
-  const long long list = ((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb;
-  return ws + counts_floats((long long)c.B * c.Hkv * plan.tiles) + (list * plan.slots + p.slot) * part_floats(plan, c.D);
+  return ws + notes_floats((long long)c.B * c.Hkv * plan.tiles) +
+         part_at(plan, (int)blockIdx.x - p.slot, p.slot, c.D);
 }
-__device__ __forceinline__ void note_count(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
-  if (plan.slots > 1 && p.slot == 0)
-    reinterpret_cast<int*>(ws)[((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb] = p.count;
+__device__ __forceinline__ void note_list(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
+  if (plan.shares > 0 && p.slot == 0) {
+    int* note = reinterpret_cast<int*>(ws) + 2 * (((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb);
+    note[0] = blockIdx.x;
+    note[1] = p.count;
+  }
 }
 constexpr int kShortRows = 16, kTileRows = 256;  // rows of a row block of the two kernels
 

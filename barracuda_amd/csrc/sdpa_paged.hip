@@ -132,26 +132,24 @@ __global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile,
   if (b >= c.B || tok < 0 || tok >= n) return;
   const int group = c.H / c.Hkv, hk = h / group;
   const long long rows = (long long)n * group, row = (long long)tok * group + h - hk * group;
-  const bool is_tile = tile.plan.slots > 1 && rows >= tile.plan.row_min;
-  if (!is_tile && (rows16.plan.slots <= 1 || rows > rows16.plan.row_max)) return;
-  const int block_rows = is_tile ? tile.block_rows : rows16.block_rows, slots = is_tile ? tile.plan.slots : rows16.plan.slots;
-  const int tiles = is_tile ? tile.plan.tiles : rows16.plan.tiles;
-  const int part_rows = is_tile ? tile.plan.part_rows : rows16.plan.part_rows;
+  const bool is_tile = tile.plan.shares > 0 && rows >= tile.plan.row_min;
+  if (!is_tile && (rows16.plan.shares == 0 || rows > rows16.plan.row_max)) return;
+  const int block_rows = is_tile ? tile.block_rows : rows16.block_rows;
+  bch::SharePlan plan = rows16.plan;
+  if (is_tile) plan = tile.plan;
   const float* const ws = is_tile ? tile.ws : rows16.ws;
-  const long long list = ((long long)b * c.Hkv + hk) * tiles + row / block_rows;
+  const long long list = ((long long)b * c.Hkv + hk) * plan.tiles + row / block_rows;
   const int r = (int)(row % block_rows);
-  const long long per = (long long)part_rows * (c.D + 2);
-  const float* p = ws + bch::counts_floats((long long)c.B * c.Hkv * tiles) + list * slots * per;
-  const float* ml = p + (long long)part_rows * c.D + 2 * r;
-  const float* po = p + (long long)r * c.D;
-  // the first 64 parts' maxima and sums come with the number of parts
-  float ms = ml[min(lane, slots - 1) * per], ls = ml[min(lane, slots - 1) * per + 1];
-  // (starts that do not ascend name lists that nobody wrote: still no more than there is room for)
-  const int count = min(reinterpret_cast<const int*>(ws)[list], slots);
+  // (starts that do not ascend name lists that nobody noted: still no more than there is room for)
+  const int2 note = reinterpret_cast<const int2*>(ws)[list];
+  const int first = min(max(note.x, 0), plan.shares - 1), count = min(note.y, plan.shares - first);
   if (count <= 1) return;
+  const float* const parts = ws + bch::notes_floats((long long)c.B * c.Hkv * plan.tiles);
+  auto ml = [&](int u) { return parts + bch::part_at(plan, first, u, c.D) + (long long)plan.part_rows * c.D + 2 * r; };
+  float ms = ml(min(lane, count - 1))[0], ls = ml(min(lane, count - 1))[1];
   float m = bch::wave_allreduce(lane < count ? ms : -INFINITY, bch::OpMax());
   for (int u0 = 64; u0 < count; u0 += 64)
-    m = fmaxf(m, bch::wave_allreduce(u0 + lane < count ? ml[(u0 + lane) * per] : -INFINITY, bch::OpMax()));
+    m = fmaxf(m, bch::wave_allreduce(u0 + lane < count ? ml(u0 + lane)[0] : -INFINITY, bch::OpMax()));
   float* dst = c.o + (c.seqs.start ? (long long)tok0 * c.ol.row : b * c.ol.batch + (long long)tok * c.ol.row) +
                h * c.ol.head;
   for (int d0 = 0; d0 < c.D; d0 += 128) {
@@ -161,8 +159,8 @@ __global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile,
       const bool on = u0 + lane < count;
       const int n = min(64, count - u0);
       if (count > 64) {
-        ms = ml[min(u0 + lane, count - 1) * per];
-        ls = ml[min(u0 + lane, count - 1) * per + 1];
+        ms = ml(min(u0 + lane, count - 1))[0];
+        ls = ml(min(u0 + lane, count - 1))[1];
       }
       const float a = on ? __builtin_amdgcn_exp2f(ms - (m == -INFINITY ? 0.0f : m)) : 0.0f;
       l += bch::wave_allreduce(on ? a * ls : 0.0f, bch::OpSum());
@@ -170,9 +168,9 @@ __global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile,
         float vx[8], vy[8];
 #pragma unroll
         for (int w = 0; w < 8; ++w) {  // past the last part: it again, not added
-          const long long off = (u0 + min(u + w, n - 1)) * per;
-          vx[w] = po[off + da];
-          vy[w] = po[off + db];
+          const float* po = parts + bch::part_at(plan, first, u0 + min(u + w, n - 1), c.D) + (long long)r * c.D;
+          vx[w] = po[da];
+          vy[w] = po[db];
         }
 #pragma unroll
         for (int w = 0; w < 8; ++w)
@@ -231,7 +229,7 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     const long long rows = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
     // where only short sequences can have been cut, their first tokens, if those are fewer
     const int group = c.H / c.Hkv, few = std::min(kFewRows / group, c.seqs.max_new);
-    const bool only_few = r.tile && r.tile_plan.slots == 1 && (long long)c.B * few * c.H < rows;
+    const bool only_few = r.tile && r.tile_plan.shares == 0 && (long long)c.B * few * c.H < rows;
     const long long waves = only_few ? (long long)c.B * few * c.H : rows;
     if (waves == 0) return hipSuccess;
     hipLaunchKernelGGL(paged_combine, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, c, a, b, only_few ? few : 0);

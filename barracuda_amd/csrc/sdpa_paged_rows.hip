@@ -90,7 +90,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
   const int D = c.D, group = c.H / c.Hkv;
 
   using Line = bch::Shares<kBlk, kRows, kOver, TREE>;
-  if (plan.slots > 1 && threadIdx.x < 64) {
+  if (plan.shares > 0 && threadIdx.x < 64) {
     Line::begin(find, c, plan, threadIdx.x);
     Line::next(find, c, plan, threadIdx.x, 0);
   }
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
     bch::Piece piece;
-    if (plan.slots > 1) {
+    if (plan.shares > 0) {
       __syncthreads();
       piece = bch::read_piece(find.piece[turn]);
       if (piece.count == 0) break;
@@ -116,7 +116,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
     const int b = piece.b, hk = piece.hk, rb = piece.rb, count = piece.count;
     const bch::Seq s = piece.seq;
     const int rows = s.n * group;
-    if (plan.slots == 1 && (rb * kRows >= rows || rows > plan.row_max)) break;
+    if (plan.shares == 0 && (rb * kRows >= rows || rows > plan.row_max)) break;
     if constexpr (TREE) {
       static_assert(64 * kWaves >= bch::kMaxDrafts, "tree_masks");
       if (b != tree_of) bch::tree_masks(tree, c.parent, s, c.window, c.sinks);
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
             for (int r = 0; r < 4; ++r) acc[4 * h + e][r] += f * red_o[w - 1][i][4 * (4 * g + r + 16 * h) + e];
       }
 
-      if (lane == 0) bch::note_count(ws, c, plan, piece);
+      if (lane == 0) bch::note_list(ws, c, plan, piece);
       if (rb * kRows + i < rows) {
         float* dst;
         float inv = 1.0f;
@@ -383,7 +383,7 @@ int resident(int D) { return (D <= 64 ? 3 : D <= 128 ? 2 : 1) * bch::device_cu_c
 
 template <int DP, int WAVES>
 void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
-  const dim3 grid((unsigned)(p.slots > 1 ? (long long)resident(c.D) : bch::lists_of(c, p))), block(64 * WAVES);
+  const dim3 grid((unsigned)(p.shares > 0 ? (long long)p.shares : bch::lists_of(c, p))), block(64 * WAVES);
   const bool full = c.D == DP, tree = c.parent != nullptr;
   auto kern = full ? (tree ? sdpa_paged_rows_kernel<DP, WAVES, true, true> : sdpa_paged_rows_kernel<DP, WAVES, true, false>)
                    : (tree ? sdpa_paged_rows_kernel<DP, WAVES, false, true> : sdpa_paged_rows_kernel<DP, WAVES, false, false>);
@@ -392,7 +392,7 @@ void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws)
 // A list that one workgroup takes whole: eight wavefronts, where the registers leave that many room.
 template <int DP>
 void launch_waves(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
-  if (p.slots == 1 && DP <= 128) launch_dp<DP, DP <= 128 ? 8 : 4>(s, c, p, ws);
+  if (p.shares == 0 && DP <= 128) launch_dp<DP, DP <= 128 ? 8 : 4>(s, c, p, ws);
   else launch_dp<DP, 4>(s, c, p, ws);
 }
 
@@ -411,14 +411,8 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
   p.tiles = (most + kRows - 1) / kRows;
   p.part_rows = std::min(most, kRows);
   p.min_share = 8 + kOver;
-  p.slots = 1;
-  if (p.tiles == 0) return p;
-  const long long blocks = bch::most_keys(c, max_len) / kBlk + 3;
-  if (may_split && blocks > 512 / kBlk + 3) {
-    const long long part = sizeof(float) * bch::part_floats(p, c.D) * bch::lists_of(c, p), most_bytes = 256LL << 20;
-    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, (long long)resident(c.D) + 1, most_bytes / part});
-    if (p.slots < 2) p.slots = 1;
-  }
+  p.shares = 0;
+  if (may_split && p.tiles > 0 && most_keys(c, max_len) > 512) p.shares = resident(c.D);
   return p;
 }
 

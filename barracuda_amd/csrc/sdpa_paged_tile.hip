@@ -91,7 +91,7 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     return l;
   };
   using Line = bch::Shares<kBKV, G::BQ, kOver, TREE>;
-  if (plan.slots > 1 && threadIdx.x < 64) {
+  if (plan.shares > 0 && threadIdx.x < 64) {
     Line::begin(share, c, plan, threadIdx.x);
     Line::next(share, c, plan, threadIdx.x, 0);
   }
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int li = lane & 31, lh = lane >> 5;
     bch::Piece mine;
-    if (plan.slots > 1) {
+    if (plan.shares > 0) {
       __syncthreads();
       mine = bch::read_piece(share.piece[turn]);
       if (mine.count == 0) break;
@@ -119,7 +119,7 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     const int b = mine.b, hk = mine.hk, tile = mine.rb;
     const bch::Seq s = mine.seq;
     const int group = c.H / c.Hkv, rows = s.n * group;
-    if (plan.slots == 1 && (rows < plan.row_min || tile * G::BQ >= rows)) break;
+    if (plan.shares == 0 && (rows < plan.row_min || tile * G::BQ >= rows)) break;
     const bch::KeyList keys = bch::key_list<kBKV>(s, tile * G::BQ / group, (min(tile * G::BQ + G::BQ, rows) - 1) / group,
                                                   c.window, c.sinks, TREE);
     if constexpr (TREE) {
@@ -575,7 +575,7 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
     }
 
     // ---- epilogue: value r of block n is d = 32 n + 8 (r / 4) + 4 lh + r % 4 ----
-    if (tid == 0) bch::note_count(ws, c, plan, mine);
+    if (tid == 0) bch::note_list(ws, c, plan, mine);
     const Row me = lane_row(anew(lane));
     if (r0w + li < rows) {
       float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
@@ -613,7 +613,7 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
 template <int DP>
 void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
   const long long lists = bch::lists_of(c, p);
-  const dim3 grid((unsigned)(p.slots > 1 ? (long long)bch::device_cu_count() : lists)), block(TileCfg<DP>::NT);
+  const dim3 grid((unsigned)(p.shares > 0 ? (long long)p.shares : lists)), block(TileCfg<DP>::NT);
   const bool full = c.D == DP, tree = c.parent != nullptr;
   auto kern = full ? (tree ? sdpa_paged_tile_kernel<DP, true, true> : sdpa_paged_tile_kernel<DP, true, false>)
                    : (tree ? sdpa_paged_tile_kernel<DP, false, true> : sdpa_paged_tile_kernel<DP, false, false>);
@@ -636,15 +636,9 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   p.tiles = (most - 1) / kTileRows + 1;
   p.part_rows = std::min(most, kTileRows);
   p.min_share = 4 + kOver;
-  p.slots = 1;
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
-  const long long blocks = most_keys(c, max_len) / kBKV + 3;
-  if (may_split && rows / kTileRows < 2 * cu) {
-    const long long part = sizeof(float) * part_floats(p, c.D) * lists_of(c, p);
-    p.slots = (int)std::min({(blocks + kOver) / p.min_share + 2, cu + 1, (256LL << 20) / part});
-    if (p.slots < 2) p.slots = 1;
-  }
+  p.shares = may_split && rows / kTileRows < 2 * cu ? (int)cu : 0;
   return p;
 }
 

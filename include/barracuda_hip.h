@@ -416,7 +416,7 @@ typedef struct bch_kv_batch {
  * not seen.  Row r, head h of q is at r*row_stride + h*head_stride (batch_stride
  * is not used); query head h reads key/value head h / (H / Hkv).  o must not
  * overlap q, k or v.  Keys are split over workgroups where that fills the chip,
- * with the partial results in the context's workspace (512 MiB at most), or not
+ * with the partial results in the context's workspace, or not
  * where that may not grow (under capture, or out of memory).  D <= 1024; a tree has at most 128 drafts a sequence
  * (max_new; BCH_E_UNSUPPORTED beyond).  total, max_new or B of 0: nothing
  * happens. */
