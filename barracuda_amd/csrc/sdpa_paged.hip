@@ -18,19 +18,23 @@ using bch::Seq;
 
 constexpr int kAnyWaves = 4;
 
-// A wavefront per row and query head, lane l the columns l + 64 t: one key after the other, its score
-// by a reduction over the wavefront.  Reads nothing that the row does not see.
+// Head dimensions that the matrix-core kernels do not take (below 4, and 257 to 1024): a workgroup per row and
+// query head, its wavefronts four keys in turn each, lane l the columns l + 64 t; a score is a reduction over the
+// wavefront, four of them under way at a time.  Reads nothing that the row does not see.  Every row reads its
+// own K and V: 4 sequences of 2048 keys, 8 heads on 2, D 512, a token each: 1914 us with a wavefront per row and one
+// key at a time, 275 so; 64 tokens each 2241 and 831 (D 2: 787 and 130, 810 and 504).
 template <int T>
-__global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCall c, int tiles) {
+__global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCall c, int rows_per_seq) {
+  constexpr int U = 4;  // keys at a time
   __shared__ bch::TreeMasks tree;
-  const int b = blockIdx.x / tiles;
+  __shared__ float red_m[kAnyWaves], red_l[kAnyWaves], red_o[kAnyWaves][64 * T];
+  const int b = blockIdx.x / rows_per_seq, r = blockIdx.x % rows_per_seq;
   const Seq s = bch::load_seq(c.kv, c.seqs, b);
+  const int i = r / c.H, h = r - i * c.H, hk = h / (c.H / c.Hkv);
+  if (i >= s.n) return;
   if (c.parent) bch::tree_masks(tree, c.parent, s, c.window, c.sinks);
 
-  const int lane = threadIdx.x & 63;
-  const long long r = (long long)(blockIdx.x % tiles) * kAnyWaves + (threadIdx.x >> 6);
-  if (r >= (long long)s.n * c.H) return;
-  const int i = (int)(r / c.H), h = (int)(r % c.H), hk = h / (c.H / c.Hkv);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const float* kh = c.kv.k + hk * c.kv.kl.head;
   const float* vh = c.kv.v + hk * c.kv.vl.head;
   const long long row = s.row0 + i;
@@ -45,45 +49,83 @@ __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCal
     acc[t] = 0.0f;
   }
   float m = -INFINITY, l = 0.0f;
-  auto key = [&](int j) {
-    const bch::Slot sl = bch::key_slot(c.kv, b, j);
-    if (sl.page < 0) return;
-    const float* kr = kh + bch::slot_offset(c.kv.kl, sl);
-    const float* vr = vh + bch::slot_offset(c.kv.vl, sl);
-    float p = 0.0f, x[T];
+  // keys j .. min(j + U, end) - 1
+  auto some = [&](int j, int end) {
+    bool on[U];
+    float p[U], x[U][T];
 #pragma unroll
-    for (int t = 0; t < T; ++t) {
-      const int d = lane + 64 * t;
-      p = fmaf(qv[t], d < c.D ? kr[d] : 0.0f, p);
-      x[t] = d < c.D ? vr[d] : 0.0f;
+    for (int u = 0; u < U; ++u) {
+      bch::Slot sl{-1, 0};
+      if (j + u < end) sl = bch::key_slot(c.kv, b, j + u);
+      on[u] = sl.page >= 0;
+      if (!on[u]) sl = {0, 0};
+      const float* kr = kh + bch::slot_offset(c.kv.kl, sl);
+      const float* vr = vh + bch::slot_offset(c.kv.vl, sl);
+      p[u] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        const int d = lane + 64 * t;
+        p[u] = fmaf(qv[t], on[u] && d < c.D ? kr[d] : 0.0f, p[u]);
+        x[u][t] = on[u] && d < c.D ? vr[d] : 0.0f;
+      }
     }
-    p = bch::wave_allreduce(p, bch::OpSum());
-    if (p == -INFINITY) return;
-    const float mn = p > m ? p : m;  // NaN: the sum below becomes NaN and stays it
-    const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
-    const float e = __builtin_amdgcn_exp2f(p - (mn == -INFINITY ? 0.0f : mn));
-    m = mn;
-    l = l * a + e;
+    float mn = m;
 #pragma unroll
-    for (int t = 0; t < T; ++t) acc[t] = fmaf(e, x[t], acc[t] * a);
+    for (int u = 0; u < U; ++u) {
+      p[u] = bch::wave_allreduce(p[u], bch::OpSum());
+      if (!on[u]) p[u] = -INFINITY;
+      mn = p[u] > mn ? p[u] : mn;  // (NaN: its weight below is NaN, and so is the sum)
+    }
+    const float a = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn), use = mn == -INFINITY ? 0.0f : mn;
+    m = mn;
+    l *= a;
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[t] *= a;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p[u] == -INFINITY) continue;  // not seen: whatever its value
+      const float e = __builtin_amdgcn_exp2f(p[u] - use);
+      l += e;
+#pragma unroll
+      for (int t = 0; t < T; ++t) acc[t] = fmaf(e, x[u][t], acc[t]);
+    }
   };
 
   const int pos = s.first + (c.parent ? tree.depth[i] : i);
   const int hi = c.parent ? s.first : pos + 1;  // committed keys (or the chain's) below hi
-  const int lo = bch::window_begin(pos, c.window);
-  for (int j = 0; j < min(min(c.sinks, lo), hi); ++j) key(j);
-  for (int j = lo; j < hi; ++j) key(j);
-  if (c.parent)
+  const int lo = bch::window_begin(pos, c.window), s_hi = min(min(c.sinks, lo), hi);
+  for (int j = U * wave; j < s_hi; j += U * kAnyWaves) some(j, s_hi);
+  for (long long j = lo + U * wave; j < hi; j += U * kAnyWaves) some((int)j, hi);
+  if (c.parent) {
+    int turn = 0;
     for (int w = 0; w < 4; ++w)
       for (unsigned bits = tree.mask[i][w]; bits; bits &= bits - 1) {
         const int j = s.first + 32 * w + __ffs(bits) - 1;
-        if (j >= 0) key(j);
+        if (j >= 0 && turn++ % kAnyWaves == wave) some(j, j + 1);
       }
-  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  }
+  if (lane == 0) {
+    red_m[wave] = m;
+    red_l[wave] = l;
+  }
 #pragma unroll
-  for (int t = 0; t < T; ++t) {
-    const int d = lane + 64 * t;
-    if (d < c.D) o[d] = l == 0.0f ? 0.0f : acc[t] * inv;
+  for (int t = 0; t < T; ++t) red_o[wave][lane + 64 * t] = acc[t];
+  __syncthreads();
+  m = red_m[0];
+#pragma unroll
+  for (int w = 1; w < kAnyWaves; ++w) m = fmaxf(m, red_m[w]);
+  float f[kAnyWaves];
+  l = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kAnyWaves; ++w) {
+    f[w] = __builtin_amdgcn_exp2f(red_m[w] - (m == -INFINITY ? 0.0f : m));
+    l += f[w] * red_l[w];
+  }
+  for (int d = threadIdx.x; d < c.D; d += 64 * kAnyWaves) {
+    float x = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kAnyWaves; ++w) x = fmaf(f[w], red_o[w][d], x);
+    o[d] = l == 0.0f ? 0.0f : x / l;
   }
 }
 
@@ -186,8 +228,9 @@ __global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile,
   }
 }
 
-// Which kernels a call takes.  The tile kernel does 64 rows or fewer of a sequence as slowly as 256; a batch
-// may mix prompts and single tokens, so each kernel serves its own sequences.
+// Which kernels a call takes.  The tile kernel does a few rows of a sequence nearly as slowly as 256; a batch may
+// mix prompts and single tokens, so each kernel serves its own sequences (16 ragged trees of up to 64 drafts: 320
+// us on tiles alone, 282 on both, 118 with shares).
 struct Route {
   bool tile, rows;
   bch::SharePlan tile_plan, rows_plan;
@@ -235,10 +278,10 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     hipLaunchKernelGGL(paged_combine, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, c, a, b, only_few ? few : 0);
     return hipGetLastError();
   }
-  const long long tiles = ((long long)c.seqs.max_new * c.H + kAnyWaves - 1) / kAnyWaves;
-  if (!fits_grid(tiles * c.B, 64 * kAnyWaves)) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)(tiles * c.B)), block(64 * kAnyWaves);
-#define BCH_ANY(T_) hipLaunchKernelGGL(sdpa_paged_any_kernel<T_>, grid, block, 0, s, c, (int)tiles)
+  const long long rows = (long long)c.seqs.max_new * c.H;
+  if (rows > 0x7fffffffLL || !fits_grid(rows * c.B, 64 * kAnyWaves)) return hipErrorInvalidConfiguration;
+  const dim3 grid((unsigned)(rows * c.B)), block(64 * kAnyWaves);
+#define BCH_ANY(T_) hipLaunchKernelGGL(sdpa_paged_any_kernel<T_>, grid, block, 0, s, c, (int)rows)
   if (c.D <= 64) BCH_ANY(1);
   else if (c.D <= 128) BCH_ANY(2);
   else if (c.D <= 256) BCH_ANY(4);
