@@ -400,8 +400,11 @@ void launch_waves(hipStream_t s, const PagedCall& c, const SharePlan& p, float* 
 
 namespace bch {
 
-// A share is at least 128 keys.  Up to 512 keys a list, a workgroup takes it whole, which saves the second
-// launch.
+// A share is at least 128 keys.  A workgroup takes a list whole, which saves the second launch, up to 384 keys
+// of 128 floats, and up to 1024 where there is a list a CU; of narrower ones in proportion more.  Measured,
+// whole / shared, us a decode step (32 heads on 8, D 128): 8 lists of 256 / 384 / 512 keys 15.5 / 18.8 / 22.0
+// against 17.0 / 18.4 / 18.3; 256 lists of 512 / 1024 / 2048 28.6 / 45.8 / 96 against 36.8 / 54.3 / 107 (beyond,
+// lists of unequal lengths gain more from shares); 8 lists of 500 keys, D 64, 13.9 against 16.8.
 SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, bool may_split) {
   SharePlan p;
   const int group = c.H / c.Hkv;
@@ -412,7 +415,8 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
   p.part_rows = std::min(most, kRows);
   p.min_share = 8 + kOver;
   p.shares = 0;
-  if (may_split && p.tiles > 0 && most_keys(c, max_len) > 512) p.shares = resident(c.D);
+  const long long whole = lists_of(c, p) >= device_cu_count() ? 1024 : 384, width = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
+  if (may_split && p.tiles > 0 && most_keys(c, max_len) * width > whole * 128) p.shares = resident(c.D);
   return p;
 }
 

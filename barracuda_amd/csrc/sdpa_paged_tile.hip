@@ -624,8 +624,11 @@ void launch_dp(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws)
 
 namespace bch {
 
-// Fewer tiles than two a CU: equal shares of their key blocks, a workgroup each, a share eight blocks at
-// least.  More: a workgroup a tile.
+// Up to a tile for every second CU: equal shares of their key blocks, a workgroup each, a share four blocks
+// at least.  More: a workgroup a tile, last ones first; a prompt's lists differ in length, which shares do not
+// know.  Measured, a workgroup a tile / shares, us (32 heads on 8, D 128): 64 tiles of a 512-token prompt 84 / 66,
+// behind 3584 keys 514 / 202; 128 tiles, 1024 tokens 146 / 123 (window 512: 93 / 111); 256 tiles, 2048 tokens
+// 276 / 298, eight prompts of 256 55 / 76.
 SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) {
   SharePlan p;
   const int group = c.H / c.Hkv;
@@ -638,7 +641,7 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   p.min_share = 4 + kOver;
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
-  p.shares = may_split && rows / kTileRows < 2 * cu ? (int)cu : 0;
+  p.shares = may_split && rows / kTileRows <= cu / 2 ? (int)cu : 0;
   return p;
 }
 
