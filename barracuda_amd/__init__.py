@@ -1,5 +1,6 @@
 """barracuda_amd -- MI355X (gfx950) implementation of barraCuda's dense ML-ops
-hot path: f32 matmul / batched matmul, row softmax, fused attention forward.
+hot path: f32 matmul / batched matmul, row softmax, fused attention forward;
+and a paged key/value cache with windowed attention over it.
 
 The compute lives in libbarracuda_hip.so (C ABI: include/barracuda_hip.h);
 this package is the host side that mirrors the reference's op API.

@@ -133,7 +133,7 @@ __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCal
 // wavefront per row, lane s the maximum and sum of part s, lane d (and on by 64) the columns.  A part
 // without a key that the row sees has l = 0 and counts nothing; a row without any gives zeros.  Rows of a
 // list that was not cut are there already.  Trips to memory bound it: the rows of eight parts are loaded
-// before they are added.  Both kernels' rows in one launch, a wavefront per row of q that there is (with one
+// before they are added (32 decode steps 4.9 us, a tree of 64 rows in 32 parts 10.6).  Both kernels' rows in one launch, a wavefront per row of q that there is (with one
 // per row that a sequence might have, those with nothing to do took 12 of 20 us for seven ragged chunks).
 struct Combined {
   bch::SharePlan plan;

@@ -10,7 +10,7 @@ j % page_size of its page j // page_size.  Pages are counted: a fork shares its
 parent's, and a page that more than one sequence holds is copied before one of
 them writes into it.  The bookkeeping is on the host; what a step's kernels
 need of it (page table, starts, lengths, the drafts' parents) is uploaded once
-per step and serves every layer.
+per step and serves every layer.  A cache is for one thread at a time.
 
     cache = KvCache(layers, pages, page_size, kv_heads, head_dim)
     a = cache.new_sequence()
