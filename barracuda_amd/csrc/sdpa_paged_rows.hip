@@ -61,9 +61,12 @@ __device__ __forceinline__ float quad_sum(float x) {
 // in q (and count once in the scores), and come out twice, alike, in O.
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
+// (inside: known to be below D without looking; only the last 64 columns of a class of D need the comparison,
+// and the others' addresses no registers of their own: 4 x 2048 keys of 8 heads on 2, D 200, a token
+// each, 51 and 40 us)
 template <bool FULL>
-__device__ __forceinline__ int four(int d0, int D) {
-  return FULL ? d0 : min(d0, D - 4);
+__device__ __forceinline__ int four(int d0, int D, bool inside) {
+  return FULL || inside ? d0 : min(d0, D - 4);
 }
 __device__ __forceinline__ f32x4 load4(const float* p) { return *reinterpret_cast<const f32x4u*>(p); }
 template <bool FULL>
@@ -83,7 +86,7 @@ constexpr int kOver = 8;
 template <int DP, int kWaves, bool FULL, bool TREE>
 __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows_kernel(PagedCall c, SharePlan plan,
                                                                                       float* __restrict__ ws) {
-  constexpr int NC = DP / 16, NH = DP / 64;
+  constexpr int NC = DP / 16, NH = DP / 64, kIn = DP - 64;  // D > kIn
   __shared__ float red_m[kWaves][kRows], red_l[kWaves][kRows];
   __shared__ float red_o[kWaves - 1][kRows][DP + 4];
   __shared__ std::conditional_t<TREE, bch::TreeMasks, int> tree;
@@ -143,7 +146,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
       const int d0 = 16 * n + 4 * g;
-      qf[n] = once<FULL>(load4(qr + four<FULL>(d0, D)), d0, D) * c.qscale;
+      qf[n] = once<FULL>(load4(qr + four<FULL>(d0, D, 16 * n + 16 <= kIn)), d0, D) * c.qscale;
     }
 
     const int p_lo = TREE ? s.first : s.first + t_lo, p_hi = s.first + t_hi;
@@ -177,12 +180,12 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
       const float* kr = kh + bch::slot_offset(c.kv.kl, slot);
       voff = bch::slot_offset(c.kv.vl, slot);
 #pragma unroll
-      for (int x = 0; x < NC; ++x) kf[u][x] = load4(kr + four<FULL>(16 * x + 4 * g, D));
+      for (int x = 0; x < NC; ++x) kf[u][x] = load4(kr + four<FULL>(16 * x + 4 * g, D, 16 * x + 16 <= kIn));
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float* vr = vh + __shfl(voff, 4 * g + r);
 #pragma unroll
-        for (int h = 0; h < NH; ++h) vf[u][r * NH + h] = load4(vr + four<FULL>(4 * (i + 16 * h), D));
+        for (int h = 0; h < NH; ++h) vf[u][r * NH + h] = load4(vr + four<FULL>(4 * (i + 16 * h), D, 64 * h + 64 <= kIn));
       }
       fetch(next);
     };
@@ -269,7 +272,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
           for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int r2 = 0; r2 < 4; ++r2) {
-              const f32x4 x = load4(vr + four<FULL>(4 * (4 * g + r2 + 16 * h), D));
+              const f32x4 x = load4(vr + four<FULL>(4 * (4 * g + r2 + 16 * h), D, 64 * h + 64 <= kIn));
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 if (see) acc[4 * h + e][r2] = fmaf(p, x[e], acc[4 * h + e][r2]);
@@ -372,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, DP > 128 ? 1 : 2) void sdpa_paged_rows
             f32x4 x;
 #pragma unroll
             for (int e = 0; e < 4; ++e) x[e] = acc[4 * h + e][r] * inv;
-            if (FULL || d0 < D) *reinterpret_cast<f32x4u*>(dst + four<FULL>(d0, D)) = x;
+            if (FULL || d0 < D) *reinterpret_cast<f32x4u*>(dst + four<FULL>(d0, D, 64 * h + 64 <= kIn)) = x;
           }
       }
     }
@@ -417,7 +420,7 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
   p.part_rows = std::min(most, kRows);
   p.min_share = 8 + kOver;
   p.shares = 0;
-  const long long whole = lists_of(c, p) >= device_cu_count() ? 1024 : 384, width = c.D <= 64 ? 64 : c.D <= 128 ? 128 : 256;
+  const long long whole = lists_of(c, p) >= device_cu_count() ? 1024 : 384, width = c.D <= 64 ? 64 : c.D <= 128 ? 128 : c.D <= 192 ? 192 : 256;
   if (may_split && p.tiles > 0 && most_keys(c, max_len) * width > whole * 128) p.shares = resident(c.D);
   return p;
 }
@@ -432,6 +435,7 @@ hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const Share
   if (p.tiles == 0) return hipSuccess;  // a token alone has more rows than the limit
   if (c.D <= 64) launch_waves<64>(s, c, p, ws);
   else if (c.D <= 128) launch_waves<128>(s, c, p, ws);
+  else if (c.D <= 192) launch_waves<192>(s, c, p, ws);
   else launch_waves<256>(s, c, p, ws);
   return hipGetLastError();
 }
