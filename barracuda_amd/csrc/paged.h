@@ -372,7 +372,23 @@ __device__ __forceinline__ void note_list(float* ws, const PagedCall& c, const S
     note[1] = p.count;
   }
 }
-constexpr int kShortRows = 16, kTileRows = 256;  // rows of a row block of the two kernels
+constexpr int kShortRows = 16, kTileRows = 256, kWideRows = 128;  // rows of a row block of the kernels
+constexpr int kTileDim = 128;                                     // the bf16 parts' widest, f32 tiles from there on
+// What a list's beginning and end cost an f32 tile, in blocks: 13 tokens behind 2048 keys, 4 sequences, 8 heads on
+// 2, D 256, 50 us with 2, 67 with 4.
+constexpr int kWideOver = 2;
+// Where a workgroup takes a tile whole: tile and b * Hkv + hk of workgroup n, last tiles first (without a window the
+// longest), a tile's sequences and heads together; with Hkv a multiple of 8 the tiles of a head share an XCD's L2.
+// The sequences go round by one from tile to tile: workgroups are dealt out in turn to the XCDs and to the four
+// engines of one, and with B a multiple of 4 one engine would else get all tiles of the longest sequence.
+struct Tile {
+  int rb, bk;
+};
+__device__ __forceinline__ Tile tile_of(const PagedCall& c, const SharePlan& plan, unsigned n) {
+  const unsigned nbk = (unsigned)c.B * c.Hkv, at = n / nbk;
+  return {(int)(plan.tiles - 1 - at), (int)((n - at * nbk + at % c.B * c.Hkv) % nbk)};
+}
+inline int tile_rows(int D) { return D <= kTileDim ? kTileRows : kWideRows; }
 
 // The most keys that a row block of the call reads.
 inline long long most_keys(const PagedCall& c, int max_len) {
@@ -383,14 +399,17 @@ inline long long most_keys(const PagedCall& c, int max_len) {
 // the longest sequence, for the plan.
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
-// The sequences with more than kFewRows rows a key/value head, 8 <= D <= 128 (sdpa_paged_tile.hip), and the
+// The sequences with more than kFewRows rows a key/value head, 8 <= D <= 256 (sdpa_paged_tile.hip, above 128
+// sdpa_paged_wide.hip), and the
 // ones with up to row_limit, 4 <= D <= 256 (sdpa_paged_rows.hip).  A plan's workspace: share_bytes.
 // Measured, the first / the second kernel, us (8 sequences of 4096 keys, 32 heads on 8, D 128): 32 rows 113 / 90,
-// 48 117 / 128, 64 116 / 170; through a window of 512, 48 rows 40 / 34, 64 41 / 41.
+// 48 117 / 128, 64 116 / 170; through a window of 512, 48 rows 40 / 34, 64 41 / 41.  D 256:
+// 32 rows 185 by the second, 48 - / 299, 52 208 / -; 4 sequences of 2048 keys, 8 heads on 2, 48 - / 41, 52 50 / -.
 constexpr int kFewRows = 48;
 bool sdpa_paged_tile_applies(const PagedCall& c);
 SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split);
 hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws);
+hipError_t launch_sdpa_paged_wide(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws);
 bool sdpa_paged_rows_applies(const PagedCall& c, int row_limit);
 SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, bool may_split);
 hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws);

@@ -268,7 +268,7 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, r.tile_plan, tile_ws) : hipSuccess;
     if (e == hipSuccess && r.rows) e = launch_sdpa_paged_rows(s, c, r.rows_plan, rows_ws);
     if (e != hipSuccess || r.bytes == 0) return e;
-    const Combined a{r.tile_plan, kTileRows, tile_ws}, b{r.rows_plan, kShortRows, rows_ws};
+    const Combined a{r.tile_plan, tile_rows(c.D), tile_ws}, b{r.rows_plan, kShortRows, rows_ws};
     const long long rows = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
     // where only short sequences can have been cut, their first tokens, if those are fewer
     const int group = c.H / c.Hkv, few = std::min(kFewRows / group, c.seqs.max_new);

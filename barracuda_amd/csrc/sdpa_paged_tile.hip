@@ -113,11 +113,9 @@ __global__ __launch_bounds__(TileCfg<DP>::NT) void sdpa_paged_tile_kernel(PagedC
       if (mine.count == 0) break;
       if (wave == 0) Line::next(share, c, plan, lane, turn ^ 1);
     } else {
-      // a workgroup a tile, last ones first (without a window the longest), all heads of a tile together: with
-      // B * Hkv a multiple of 8 the tiles of a head share an XCD's L2
-      const int nbk = c.B * c.Hkv, bk = blockIdx.x % nbk;
-      mine = {bch::load_seq(c.kv, c.seqs, bk / c.Hkv), bk / c.Hkv, bk % c.Hkv, (int)(plan.tiles - 1 - blockIdx.x / nbk),
-              0, 0, 0, 1, 1};
+      const bch::Tile own = bch::tile_of(c, plan, blockIdx.x);
+      const int of = own.bk / c.Hkv;
+      mine = {bch::load_seq(c.kv, c.seqs, of), of, own.bk - of * c.Hkv, own.rb, 0, 0, 0, 1, 1};
       more = false;
     }
     const int b = mine.b, hk = mine.hk, tile = mine.rb;
@@ -640,26 +638,27 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   p.row_min = kFewRows + 1;
   p.row_max = 0x7fffffff;
   const int most = c.seqs.max_new * group;
-  p.tiles = (most - 1) / kTileRows + 1;
-  p.part_rows = std::min(most, kTileRows);
-  p.min_share = 4 + kOver;
+  p.tiles = (most - 1) / tile_rows(c.D) + 1;
+  p.part_rows = std::min(most, tile_rows(c.D));
+  p.min_share = c.D <= kTileDim ? 4 + kOver : 2 + kWideOver;
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
-  p.shares = may_split && rows / kTileRows <= cu / 2 ? (int)cu : 0;
+  p.shares = may_split && rows / tile_rows(c.D) <= cu / 2 ? (int)cu : 0;
   return p;
 }
 
 bool sdpa_paged_tile_applies(const PagedCall& c) {
   const long long rows = (long long)c.seqs.max_new * (c.H / c.Hkv);
-  return c.D >= 8 && c.D <= 128 && rows > kFewRows && rows <= 0x7fffffff - 256 &&
-         fits_grid((long long)c.B * c.Hkv * ((rows + 255) / 256), TileCfg<32>::NT);
+  return c.D >= 8 && c.D <= 256 && rows > kFewRows && rows <= 0x7fffffff - 256 &&
+         fits_grid((long long)c.B * c.Hkv * ((rows - 1) / tile_rows(c.D) + 1), TileCfg<32>::NT);
 }
 
 hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {
   if (c.D <= 32) launch_dp<32>(s, c, p, ws);
   else if (c.D <= 64) launch_dp<64>(s, c, p, ws);
   else if (c.D <= 96) launch_dp<96>(s, c, p, ws);
-  else launch_dp<128>(s, c, p, ws);
+  else if (c.D <= kTileDim) launch_dp<128>(s, c, p, ws);
+  else return launch_sdpa_paged_wide(s, c, p, ws);
   return hipGetLastError();
 }
 
