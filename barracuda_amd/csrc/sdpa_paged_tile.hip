@@ -628,9 +628,12 @@ namespace bch {
 
 // Up to a tile for every second CU: equal shares of their key blocks, a workgroup each, a share four blocks
 // at least.  More: a workgroup a tile, last ones first; a prompt's lists differ in length, which shares do not
-// know.  Measured, a workgroup a tile / shares, us (32 heads on 8, D 128): 64 tiles of a 512-token prompt 84 / 66,
+// know.  Up to two tiles a CU shares too where that hardly matters (keys more than twice the new tokens) and the
+// lists are long: whole ones leave CUs idle where sequences differ.  Measured, a workgroup a tile / shares, us (32 heads on 8, D 128): 64 tiles of a 512-token prompt 84 / 66,
 // behind 3584 keys 514 / 202; 128 tiles, 1024 tokens 146 / 123 (window 512: 93 / 111); 256 tiles, 2048 tokens
-// 276 / 298, eight prompts of 256 55 / 76.
+// 276 / 298, eight prompts of 256 55 / 76.  Chunks: four of up to 700 tokens, 2048 keys, 271 / 201; eight of up to 256,
+// 4096 keys, 509 / 191, all of 256 627 / 654; sixteen of 128, window 512, 109 / 126.  Four prompts of up to 2048 tokens
+// 281 / 359 (D 256, three chunks of up to 600, 5000 keys: 1378 / 886).
 SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) {
   SharePlan p;
   const int group = c.H / c.Hkv;
@@ -643,7 +646,9 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   p.min_share = c.D <= kTileDim ? 4 + kOver : 2 + kWideOver;
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
-  p.shares = may_split && rows / tile_rows(c.D) <= cu / 2 ? (int)cu : 0;
+  const long long full = rows / tile_rows(c.D), keys = most_keys(c, max_len);
+  const bool alike = keys >= 1024 && keys > 2LL * c.seqs.max_new;
+  p.shares = may_split && full <= (alike ? 2 * cu : cu / 2) ? (int)cu : 0;
   return p;
 }
 
