@@ -193,7 +193,7 @@ __device__ __forceinline__ KeyList key_list(const Seq& s, int t_lo, int t_hi, in
 // instead and a workgroup has one of them: no workgroup then begins two.
 struct SharePlan {
   int row_min, row_max;  // rows a key/value head of the sequences served
-  int tiles;             // row blocks of the longest of them
+  int rows, tiles;       // rows of a row block, row blocks of the longest sequence
   int part_rows;         // rows of a part: a row block's, if any sequence has as many
   int shares;            // workgroups of the line; 0 (no workspace): a workgroup a list
   int min_share;

@@ -137,11 +137,10 @@ __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCal
 // per row that a sequence might have, those with nothing to do took 12 of 20 us for seven ragged chunks).
 struct Combined {
   bch::SharePlan plan;
-  int block_rows;
   const float* ws;
 };
 // most > 0: the tokens of a sequence that are looked at; else all rows of q.
-__global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile, Combined rows16, int most) {
+__global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile, Combined few, int most) {
   const int lane = threadIdx.x & 63;
   const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   int tok0 = (int)(at / c.H);
@@ -175,13 +174,12 @@ __global__ __launch_bounds__(256) void paged_combine(PagedCall c, Combined tile,
   const int group = c.H / c.Hkv, hk = h / group;
   const long long rows = (long long)n * group, row = (long long)tok * group + h - hk * group;
   const bool is_tile = tile.plan.shares > 0 && rows >= tile.plan.row_min;
-  if (!is_tile && (rows16.plan.shares == 0 || rows > rows16.plan.row_max)) return;
-  const int block_rows = is_tile ? tile.block_rows : rows16.block_rows;
-  bch::SharePlan plan = rows16.plan;
+  if (!is_tile && (few.plan.shares == 0 || rows > few.plan.row_max)) return;
+  bch::SharePlan plan = few.plan;
   if (is_tile) plan = tile.plan;
-  const float* const ws = is_tile ? tile.ws : rows16.ws;
-  const long long list = ((long long)b * c.Hkv + hk) * plan.tiles + row / block_rows;
-  const int r = (int)(row % block_rows);
+  const float* const ws = is_tile ? tile.ws : few.ws;
+  const long long list = ((long long)b * c.Hkv + hk) * plan.tiles + row / plan.rows;
+  const int r = (int)(row % plan.rows);
   // (starts that do not ascend name lists that nobody noted: still no more than there is room for)
   const int2 note = reinterpret_cast<const int2*>(ws)[list];
   const int first = min(max(note.x, 0), plan.shares - 1), count = min(note.y, plan.shares - first);
@@ -268,7 +266,7 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, r.tile_plan, tile_ws) : hipSuccess;
     if (e == hipSuccess && r.rows) e = launch_sdpa_paged_rows(s, c, r.rows_plan, rows_ws);
     if (e != hipSuccess || r.bytes == 0) return e;
-    const Combined a{r.tile_plan, tile_rows(c.D), tile_ws}, b{r.rows_plan, kShortRows, rows_ws};
+    const Combined a{r.tile_plan, tile_ws}, b{r.rows_plan, rows_ws};
     const long long rows = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
     // where only short sequences can have been cut, their first tokens, if those are fewer
     const int group = c.H / c.Hkv, few = std::min(kFewRows / group, c.seqs.max_new);

@@ -641,12 +641,13 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   p.row_min = kFewRows + 1;
   p.row_max = 0x7fffffff;
   const int most = c.seqs.max_new * group;
-  p.tiles = (most - 1) / tile_rows(c.D) + 1;
-  p.part_rows = std::min(most, tile_rows(c.D));
+  p.rows = tile_rows(c.D);
+  p.tiles = (most - 1) / p.rows + 1;
+  p.part_rows = std::min(most, p.rows);
   p.min_share = c.D <= kTileDim ? 4 + kOver : 2 + kWideOver;
   // full tiles that there are: a batch's rows, or every sequence's
   const long long rows = (long long)c.Hkv * group * (c.seqs.start ? c.seqs.total : (long long)c.B * c.seqs.max_new);
-  const long long full = rows / tile_rows(c.D), keys = most_keys(c, max_len);
+  const long long full = rows / p.rows, keys = most_keys(c, max_len);
   const bool alike = keys >= 1024 && keys > 2LL * c.seqs.max_new;
   p.shares = may_split && full <= (alike ? 2 * cu : cu / 2) ? (int)cu : 0;
   return p;
