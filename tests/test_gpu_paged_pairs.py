@@ -31,7 +31,7 @@ def test_many_sequences(dev):
 
 
 @pytest.mark.parametrize("window,sinks", [(0, 0), (3, 2900), (2200, 4)])
-@pytest.mark.parametrize("d", [50, 64, 128])
+@pytest.mark.parametrize("d", [50, 64, 100, 128])
 def test_tree(dev, d, window, sinks):
     rng = np.random.default_rng(d + window)
     for lens, news, h, hkv in (([3000, 2777, 900], [8, 12, 5], 8, 2), ([2800, 60], [40, 33], 2, 2)):
