@@ -402,8 +402,9 @@ size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
 // The sequences with more than kFewRows rows a key/value head, 8 <= D <= 256 (sdpa_paged_tile.hip, above 128
 // sdpa_paged_wide.hip), and the
 // ones with up to row_limit, 4 <= D <= 256 (sdpa_paged_rows.hip).  A plan's workspace: share_bytes.
-// Measured, the first / the second kernel, us (8 sequences of 4096 keys, 32 heads on 8, D 128): 32 rows 113 / 90,
-// 48 117 / 128, 64 116 / 170; through a window of 512, 48 rows 40 / 34, 64 41 / 41.  D 256:
+// Measured, the first / the second kernel, us (8 sequences of 4096 keys, 32 heads on 8, D 128): 32 rows 113 / 63,
+// 48 117 / 103 (90 and 128 with 16 rows a workgroup, as in batches with longer chunks; 64 so 116 / 170); through a
+// window of 512, 48 rows 40 / 34, 64 41 / 41.  D 256:
 // 32 rows 185 by the second, 48 - / 299, 52 208 / -; 4 sequences of 2048 keys, 8 heads on 2, 48 - / 41, 52 50 / -.
 constexpr int kFewRows = 48;
 bool sdpa_paged_tile_applies(const PagedCall& c);
