@@ -92,6 +92,7 @@ SIGNATURES = {
                             AttnLayout]),
     "bch_sdpa_window": (_i, [_vp, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, AttnLayout, _vp, AttnLayout, _vp,
                              AttnLayout, _vp, AttnLayout]),
+    "bch_sdpa_paged_kernel_name": (C.c_char_p, [C.POINTER(KvPages), C.POINTER(KvBatch), _i, _i, _i]),
     "bch_kv_append": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, AttnLayout, _vp, AttnLayout]),
     "bch_kv_copy_pages": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, C.POINTER(_i), C.POINTER(_i)]),
     "bch_kv_keep": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, _i, _vp, _vp, _vp]),

@@ -1204,6 +1204,16 @@ const char* bch_layer_norm_kernel_name(long long rows, long long cols, const flo
   return bch::layer_norm_kernel_name(rows, cols, in, out);
 }
 
+const char* bch_sdpa_paged_kernel_name(const bch_kv_pages* kv, const bch_kv_batch* batch, int H, int window, int sinks) {
+  const char* op = "bch_sdpa_paged_kernel_name";
+  if (check_pages(nullptr, op, kv, true) != BCH_OK || check_batch(nullptr, op, batch) != BCH_OK || H < 1 ||
+      H % kv->Hkv != 0 || window < 0 || sinks < 0 || kv->D > kPagedMaxD)
+    return "";
+  const bch::PagedCall c{batch->B, H, kv->Hkv, kv->D, 1.0f, window, sinks, nullptr, pages_of(*kv), seqs_of(*batch),
+                         nullptr, nullptr, {0, 0, 0}, {0, 0, 0}};
+  return c.B == 0 || c.seqs.max_new == 0 ? "" : bch::sdpa_paged_kernel_name(c, batch->max_len);
+}
+
 }  // extern "C"
 
 namespace bch {

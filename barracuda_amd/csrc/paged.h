@@ -399,6 +399,8 @@ inline long long most_keys(const PagedCall& c, int max_len) {
 // the longest sequence, for the plan.
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes);
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len);
+// The kernels of the call, rows of a row block and shares (the least of one in blocks) of each; with a workspace.
+const char* sdpa_paged_kernel_name(const PagedCall& c, int max_len);
 // The sequences with more than kFewRows rows a key/value head, 8 <= D <= 256 (sdpa_paged_tile.hip, above 128
 // sdpa_paged_wide.hip), and the
 // ones with up to row_limit, 4 <= D <= 256 (sdpa_paged_rows.hip).  A plan's workspace: share_bytes.

@@ -7,6 +7,7 @@
 #include "paged.h"
 
 #include <math.h>
+#include <stdio.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -256,6 +257,23 @@ Route route(const PagedCall& c, int max_len, bool may_split) {
 namespace bch {
 
 size_t sdpa_paged_workspace_bytes(const PagedCall& c, int max_len) { return route(c, max_len, true).bytes; }
+
+const char* sdpa_paged_kernel_name(const PagedCall& c, int max_len) {
+  thread_local char text[256];
+  const Route r = route(c, max_len, true);
+  int at = 0;
+  auto add = [&](const char* name, const SharePlan& p) {
+    at += snprintf(text + at, sizeof text - at, "%s%s rows=%d", at > 0 ? " + " : "", name, p.rows);
+    if (p.shares > 0) at += snprintf(text + at, sizeof text - at, " shares=%d least=%d", p.shares, p.min_share);
+    else at += snprintf(text + at, sizeof text - at, " whole");
+  };
+  text[0] = 0;
+  if (r.tile) add(c.D <= kTileDim ? "sdpa_paged_tile_kernel" : "sdpa_paged_wide_kernel", r.tile_plan);
+  if (r.rows && r.rows_plan.tiles > 0) add("sdpa_paged_rows_kernel", r.rows_plan);
+  if (r.bytes > 0) snprintf(text + at, sizeof text - at, " + paged_combine");
+  else if (at == 0) snprintf(text, sizeof text, "sdpa_paged_any_kernel");
+  return text;
+}
 
 hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, void* ws, size_t ws_bytes) {
   Route r = route(c, max_len, true);

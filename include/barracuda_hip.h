@@ -512,6 +512,15 @@ const char *bch_layer_norm_kernel_name(long long rows, long long cols,
 const char *bch_softmax_rows_f64_kernel_name(long long rows, long long cols,
                                              const double *in,
                                              const double *out);
+/* The kernels of a bch_sdpa_paged call (the host's part of kv and batch; their
+ * buffers are not looked at), joined by " + ": for each the rows that a
+ * workgroup takes together ("rows=") and whether lists of keys are taken
+ * "whole" or shared by "shares=" workgroups, "least=" key blocks a share, as
+ * with a workspace.  "" for a call that launches nothing or is refused.  The
+ * text is the calling thread's until its next call of this. */
+const char *bch_sdpa_paged_kernel_name(const bch_kv_pages *kv,
+                                       const bch_kv_batch *batch, int H,
+                                       int window, int sinks);
 
 #ifdef __cplusplus
 }
