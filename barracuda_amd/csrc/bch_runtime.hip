@@ -903,6 +903,8 @@ bch_status check_batch(bch_ctx* ctx, const char* op, const bch_kv_batch* batch) 
   if (batch->B < 0 || batch->total < 0 || batch->max_new < 0 || batch->max_len < 0)
     return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (B=%d, total=%d, max_new=%d, max_len=%d)", op, batch->B,
                 batch->total, batch->max_new, batch->max_len);
+  if (batch->B > bch::kMaxSeqs)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d sequences, at most %d", op, batch->B, bch::kMaxSeqs);
   return BCH_OK;
 }
 bch_status check_layers(bch_ctx* ctx, const char* op, const bch_kv_pages* kv, int layers, long long k_stride,
@@ -984,6 +986,7 @@ bch_status bch_sdpa_window(bch_ctx* ctx, int B, int H, int Hkv, int Sq, int Skv,
   if (st == BCH_OK) st = check_layout(ctx, op, "o", ol, D);
   if (st != BCH_OK) return st;
   if (D > kPagedMaxD) return fail(ctx, BCH_E_UNSUPPORTED, "%s: head dimension %d > %d", op, D, kPagedMaxD);
+  if (B > bch::kMaxSeqs) return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d sequences, at most %d", op, B, bch::kMaxSeqs);
   if (Skv > bch::kMaxKeys || Sq > bch::kMaxKeys)
     return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d queries, %d keys, at most %lld", op, Sq, Skv, bch::kMaxKeys);
   if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);

@@ -21,6 +21,8 @@ namespace bch {
 
 constexpr int kMaxDrafts = 128;  // rows of one sequence's tree: its ancestor masks are four words
 
+constexpr int kMaxSeqs = 1 << 24;  // of a call: workgroups look through them 64 at a time
+
 constexpr long long kMaxKeys = 0x7fffff00;  // of a sequence: a block's last key still has a 32-bit number
 
 struct KvPages {
@@ -190,13 +192,16 @@ __device__ __forceinline__ KeyList key_list(const Seq& s, int t_lo, int t_hi, in
 // into equal shares, a workgroup each, whatever the lengths of the sequences.  A share may hold the end of
 // one list, whole ones and the beginning of another; the parts of a list that was cut meet in
 // paged_combine.  Where there are few lists or little to do, each list is cut into equal parts by itself
-// instead and a workgroup has one of them: no workgroup then begins two.
+// instead and a workgroup has one of them: no workgroup then begins two.  And where lists are to be taken whole
+// but there might be more than a grid has workgroups (most of them empty: a list for each row block that a
+// sequence might have), the lists that there are stand in the line, each with length 1.
 struct SharePlan {
   int row_min, row_max;  // rows a key/value head of the sequences served
   int rows, tiles;       // rows of a row block, row blocks of the longest sequence
   int part_rows;         // rows of a part: a row block's, if any sequence has as many
   int shares;            // workgroups of the line; 0 (no workspace): a workgroup a list
   int min_share;
+  int whole;  // the line's lists are not cut (no workspace either)
 };
 // Workspace: for every list the workgroup of its first part and the number of its parts (in that workgroup and
 // the ones behind it), then two parts a workgroup, the one that ends a list begun before its share and the one
@@ -210,9 +215,17 @@ inline long long lists_of(const PagedCall& c, const SharePlan& p) { return (long
 // A grid has fewer than 2^32 threads.
 inline bool fits_grid(long long workgroups, int threads) { return workgroups < (1LL << 32) / threads; }
 inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
-  if (p.shares == 0) return 0;
+  if (p.shares == 0 || p.whole) return 0;
   const long long lists = lists_of(c, p);
   return sizeof(float) * (size_t)(notes_floats(lists) + 2LL * p.shares * part_floats(p, c.D));
+}
+
+// Lists taken whole by workgroups of `threads`: through a line of `workgroups` where a grid cannot have one a list.
+inline void deal_whole(const PagedCall& c, SharePlan& p, int threads, int workgroups) {
+  if (p.shares > 0 || fits_grid(lists_of(c, p), threads)) return;
+  p.shares = workgroups;
+  p.min_share = 1;
+  p.whole = 1;
 }
 
 // The lists of 64 sequences from b0 on, one sequence a lane.
@@ -283,8 +296,9 @@ struct Shares {
   static __device__ __forceinline__ void begin(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
     Lane64 seqs;
     long long total = 0, lists = 0;
+    int part = plan.whole ? 0x7fffffff : 0;  // (that many blocks are any list)
     for (int b0 = 0; b0 < c.B; b0 += 64) {
-      seqs = line(c, plan, b0, lane, 0);
+      seqs = line(c, plan, b0, lane, part);
       total += uniform(__shfl(seqs.sum, 63));
       int n = seqs.tiles;
 #pragma unroll
@@ -295,14 +309,13 @@ struct Shares {
     long long share = max((long long)plan.min_share, quotient(total + grid - 1, grid));
     // parts of one list each: ceil(w / part) <= w / part + 1 of them, in all no more than workgroups; up to a
     // twentieth longer than the shares
-    int part = 0;
-    if (lists < grid) {
+    if (!plan.whole && lists < grid) {
       const long long p = max((long long)plan.min_share, quotient(total + grid - lists - 1, grid - lists));
       if (20 * p <= 21 * share && p <= 0x7fffffff) part = (int)p;
     }
     if (part || c.B > 64) seqs = line(c, plan, 0, lane, part);
     f.seqs[lane] = seqs;
-    if (part) {
+    if (part && !plan.whole) {
       share = 1;
       total = 0;
       for (int b0 = 0; b0 < c.B; b0 += 64)
@@ -366,7 +379,7 @@ __device__ __forceinline__ float* part_of(float* ws, const PagedCall& c, const S
          part_at(plan, (int)blockIdx.x - p.slot, p.slot, c.D);
 }
 __device__ __forceinline__ void note_list(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
-  if (plan.shares > 0 && p.slot == 0) {
+  if (plan.shares > 0 && !plan.whole && p.slot == 0) {
     int* note = reinterpret_cast<int*>(ws) + 2 * (((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb);
     note[0] = blockIdx.x;
     note[1] = p.count;

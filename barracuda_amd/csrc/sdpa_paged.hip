@@ -239,7 +239,8 @@ Route route(const PagedCall& c, int max_len, bool may_split) {
   const long long all = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
   if (!bch::fits_grid(all / 4 + 1, 256)) may_split = false;  // paged_combine's
   Route r{};
-  r.tile = bch::sdpa_paged_tile_applies(c);
+  // (a batch's short sequences are the other kernel's)
+  r.tile = bch::sdpa_paged_tile_applies(c) && (!c.seqs.start || bch::sdpa_paged_rows_applies(c, bch::kFewRows));
   const int row_limit = r.tile ? bch::kFewRows : 0x7fffffff;
   // dense operands: every sequence has max_new rows
   r.rows = bch::sdpa_paged_rows_applies(c, row_limit) && !(r.tile && !c.seqs.start);
@@ -264,7 +265,8 @@ const char* sdpa_paged_kernel_name(const PagedCall& c, int max_len) {
   int at = 0;
   auto add = [&](const char* name, const SharePlan& p) {
     at += snprintf(text + at, sizeof text - at, "%s%s rows=%d", at > 0 ? " + " : "", name, p.rows);
-    if (p.shares > 0) at += snprintf(text + at, sizeof text - at, " shares=%d least=%d", p.shares, p.min_share);
+    if (p.whole) at += snprintf(text + at, sizeof text - at, " dealt=%d", p.shares);
+    else if (p.shares > 0) at += snprintf(text + at, sizeof text - at, " shares=%d least=%d", p.shares, p.min_share);
     else at += snprintf(text + at, sizeof text - at, " whole");
   };
   text[0] = 0;
@@ -284,11 +286,13 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, r.tile_plan, tile_ws) : hipSuccess;
     if (e == hipSuccess && r.rows) e = launch_sdpa_paged_rows(s, c, r.rows_plan, rows_ws);
     if (e != hipSuccess || r.bytes == 0) return e;
-    const Combined a{r.tile_plan, tile_ws}, b{r.rows_plan, rows_ws};
+    Combined a{r.tile_plan, tile_ws}, b{r.rows_plan, rows_ws};
+    if (a.plan.whole) a.plan.shares = 0;  // nothing of it to join
+    if (b.plan.whole) b.plan.shares = 0;
     const long long rows = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
     // where only short sequences can have been cut, their first tokens, if those are fewer
     const int group = c.H / c.Hkv, few = std::min(kFewRows / group, c.seqs.max_new);
-    const bool only_few = r.tile && r.tile_plan.shares == 0 && (long long)c.B * few * c.H < rows;
+    const bool only_few = r.tile && a.plan.shares == 0 && (long long)c.B * few * c.H < rows;
     const long long waves = only_few ? (long long)c.B * few * c.H : rows;
     if (waves == 0) return hipSuccess;
     hipLaunchKernelGGL(paged_combine, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, c, a, b, only_few ? few : 0);

@@ -475,13 +475,15 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
     p.shares = resident(c.D, p.rows);
   }
   p.part_rows = std::min(most, p.rows);
+  p.whole = 0;
+  deal_whole(c, p, 512, resident(c.D, p.rows));
   return p;
 }
 
 bool sdpa_paged_rows_applies(const PagedCall& c, int row_limit) {
   const long long rows = std::min((long long)c.seqs.max_new * (c.H / c.Hkv), (long long)row_limit);
   return c.D >= 4 && c.D <= 256 && rows <= 0x7fffffff - kRows &&
-         fits_grid((long long)c.B * c.Hkv * ((rows + kRows - 1) / kRows), 512);
+         (long long)c.Hkv * ((rows + kRows - 1) / kRows) <= 0x7fffffff;
 }
 
 hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {

@@ -650,13 +650,15 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   const long long full = rows / p.rows, keys = most_keys(c, max_len);
   const bool alike = keys >= 1024 && keys > 2LL * c.seqs.max_new;
   p.shares = may_split && full <= (alike ? 2 * cu : cu / 2) ? (int)cu : 0;
+  p.whole = 0;
+  deal_whole(c, p, TileCfg<32>::NT, (int)cu);
   return p;
 }
 
 bool sdpa_paged_tile_applies(const PagedCall& c) {
   const long long rows = (long long)c.seqs.max_new * (c.H / c.Hkv);
   return c.D >= 8 && c.D <= 256 && rows > kFewRows && rows <= 0x7fffffff - 256 &&
-         fits_grid((long long)c.B * c.Hkv * ((rows - 1) / tile_rows(c.D) + 1), TileCfg<32>::NT);
+         (long long)c.Hkv * ((rows - 1) / tile_rows(c.D) + 1) <= 0x7fffffff;
 }
 
 hipError_t launch_sdpa_paged_tile(hipStream_t s, const PagedCall& c, const SharePlan& p, float* ws) {

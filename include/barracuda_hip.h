@@ -393,7 +393,7 @@ typedef struct bch_kv_pages {
  * rows there are in all (starts are clamped to 0 .. total), the most new
  * tokens of one sequence (rows beyond max_new are left as they were), and the
  * most keys of one sequence (max_len: for planning alone; a longer sequence is
- * computed all the same). */
+ * computed all the same).  B is at most 2^24 (BCH_E_UNSUPPORTED). */
 typedef struct bch_kv_batch {
   int B;
   int total;
@@ -429,7 +429,7 @@ bch_status bch_sdpa_paged(bch_ctx *ctx, const bch_kv_pages *kv,
 /* The same over dense operands (layouts as bch_sdpa_fwd_ex): row i of Sq stands
  * at position Skv - Sq + i, so with Sq < Skv the queries are the last ones of
  * their sequence, and with Sq > Skv the first Sq - Skv rows see nothing and get
- * zeros.  window 0 is causal attention; no tree.  D <= 1024. */
+ * zeros.  window 0 is causal attention; no tree.  D <= 1024, B <= 2^24. */
 bch_status bch_sdpa_window(bch_ctx *ctx, int B, int H, int Hkv, int Sq, int Skv,
                            int D, float scale, int window, int sinks,
                            const float *q, bch_attn_layout q_layout,
@@ -515,8 +515,9 @@ const char *bch_softmax_rows_f64_kernel_name(long long rows, long long cols,
 /* The kernels of a bch_sdpa_paged call (the host's part of kv and batch; their
  * buffers are not looked at), joined by " + ": for each the rows that a
  * workgroup takes together ("rows=") and whether lists of keys are taken
- * "whole" or shared by "shares=" workgroups, "least=" key blocks a share, as
- * with a workspace.  "" for a call that launches nothing or is refused.  The
+ * "whole", a workgroup each, are "dealt=" out whole to so many workgroups, or
+ * shared by "shares=" workgroups, "least=" key blocks a share, as with a
+ * workspace.  "" for a call that launches nothing or is refused.  The
  * text is the calling thread's until its next call of this. */
 const char *bch_sdpa_paged_kernel_name(const bch_kv_pages *kv,
                                        const bch_kv_batch *batch, int H,

@@ -1,0 +1,99 @@
+"""Calls over so many sequences, with one long chunk among them, that a grid cannot have a workgroup for each place
+that the longest chunk's length gives every sequence.  The single tokens share a few pages; a sample of the rows is
+compared with plain forms in 64 bits, and every row has to be written."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from barracuda_amd import Tensor
+from barracuda_amd import _native as N
+from barracuda_amd.kv_cache import _I32
+from tests.kv_model import attend, visible
+from tests.test_gpu_paged import compare, tolerance
+from tests.test_paged_route import kernels
+
+pytestmark = pytest.mark.gpu
+
+
+class Crowd:
+    """b sequences of a token each, but `at` with `new` of them behind `before` keys."""
+
+    def __init__(self, dev, b, at, new, before, h, hkv, d, page=8, window=0, sinks=0, tree=None):
+        rng = np.random.default_rng(b + d)
+        self.dev, self.h, self.hkv, self.d, self.page = dev, h, hkv, d, page
+        self.window, self.sinks, self.tree, self.at = window, sinks, tree, at
+        news = np.ones(b, np.int64)
+        news[at] = new
+        self.start = np.concatenate([[0], np.cumsum(news)])
+        self.total = int(self.start[-1])
+        self.lens = rng.integers(1, 2 * page + 1, b).astype(np.int32)
+        self.lens[at] = before + new
+        held = -(-(before + new) // page)
+        self.width, self.num = max(2, held), held + 50
+        self.table = np.full((b, self.width), -1, np.int32)
+        self.table[:, :2] = rng.integers(held, self.num, (b, 2))
+        self.table[at, :held] = rng.permutation(held)
+        self.k, self.v = (rng.standard_normal((self.num, hkv, page, d), dtype=np.float32) for _ in range(2))
+        self.q = rng.standard_normal((self.total, h, d), dtype=np.float32)
+        parents = []
+        if tree is not None:
+            parents = np.full(self.total, -1, np.int32)
+            parents[self.start[at]:self.start[at + 1]] = tree
+        self.tk, self.tv, self.tq = (Tensor.from_data(x, list(x.shape), dev) for x in (self.k, self.v, self.q))
+        self.to = Tensor.from_data(np.full(self.q.shape, 7.0, np.float32), list(self.q.shape), dev)
+        self.i32 = _I32(dev, self.start, self.lens, self.table, parents)
+        lay = N.AttnLayout(hkv * page * d, page * d, d)
+        self.kv = N.KvPages(self.tk.ptr, self.tv.ptr, lay, lay, self.num, page, hkv, d, self.i32.ptrs[2], self.width)
+        self.batch = N.KvBatch(b, self.total, new, int(self.lens.max()), self.i32.ptrs[0], self.i32.ptrs[1])
+        self.row = N.AttnLayout(0, d, h * d)
+
+    def keys(self, s, pool):
+        j = np.arange(self.lens[s])
+        return pool[self.table[s, j // self.page], :, j % self.page]
+
+    def check(self, some):
+        dev = self.dev
+        parent = C.c_void_p(self.i32.ptrs[3]) if self.tree is not None else None
+        scale = float(1.0 / np.sqrt(self.d))
+        dev.check(dev._lib.bch_sdpa_paged(dev.ctx, self.kv, self.batch, self.h, scale, self.window, self.sinks, parent,
+                                          C.c_void_p(self.tq.ptr), self.row, C.c_void_p(self.to.ptr), self.row),
+                  "attention")
+        got = self.to.to_numpy().reshape(self.q.shape)
+        assert not np.any(got[..., 0] == 7.0), "rows left as they were"
+        rng = np.random.default_rng(1)
+        b = self.batch.B
+        for s in [0, self.at, b - 1] + list(rng.integers(0, b, some)):
+            first, n = int(self.lens[s] - (self.start[s + 1] - self.start[s])), int(self.start[s + 1] - self.start[s])
+            k, v = self.keys(s, self.k), self.keys(s, self.v)
+            i = np.arange(n) if n <= 128 else np.unique(np.concatenate([[0, 1, n - 1], rng.integers(0, n, 60)]))
+            if self.tree is not None:
+                see = visible(first, n, self.window, self.sinks, list(self.tree) if s == self.at else [-1])
+            else:
+                back = (first + i)[:, None] - np.arange(len(k))[None, :]
+                see = back >= 0
+                if self.window:
+                    see &= (back < self.window) | (np.arange(len(k)) < self.sinks)[None, :]
+            rows = self.start[s] + i
+            compare(got[rows], attend(self.q[rows], k, v, see, scale),
+                    tolerance(self.q[rows], k, v, scale, len(k)))
+
+
+@pytest.mark.parametrize("tree", [False, True])
+def test_three_million_sequences(dev, tree):
+    """Where once the short sequences' kernel did not run and their rows were left as they were."""
+    b, new = 3000000, 16
+    drafts = [-1, 0, 0, 1, 3, 2, 2, -1, 7, 8, 8, 5, 0, 12, 12, 9] if tree else None
+    print(f"crowd b={b} tree={tree} {kernels(b, b + new - 1, new, 20, 4, 1, 8)}", flush=True)
+    Crowd(dev, b, b // 3, new, 4, 4, 1, 8, tree=drafts).check(500)
+
+
+@pytest.mark.parametrize("b,new,h,hkv,d,window,sinks", [(8192, 8192, 32, 4, 8, 64, 2), (8192, 8192, 32, 4, 131, 50, 0),
+                                                        (16384, 1024, 8, 1, 5, 0, 0)])
+def test_a_long_chunk_beside_many_sequences(dev, b, new, h, hkv, d, window, sinks):
+    k = kernels(b, b + new - 1, new, new + 33, h, hkv, d, window, sinks)
+    print(f"crowd b={b} new={new} h={h} hkv={hkv} d={d} {k}", flush=True)
+    assert any(x is not True and x[1] < 0 for x in k.values()), "lists are not dealt out"
+    Crowd(dev, b, b // 2, new, 33, h, hkv, d, page=16, window=window, sinks=sinks).check(200)
