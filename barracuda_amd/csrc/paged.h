@@ -84,6 +84,26 @@ __device__ __forceinline__ Seq load_seq(const KvPages& kv, const KvSeqs& s, int 
   return r;
 }
 
+// a / b of a >= 0, b > 0; the 64-bit division takes a microsecond.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+
+// The sequence that row `row` of q is one of, by 64 lanes: the first that ends behind it, or the last (where starts
+// do not ascend, any of the call's).
+__device__ __forceinline__ int seq_of_row(const KvSeqs& s, int B, long long row, int lane) {
+  if (!s.start) return (int)quotient(row, s.max_new);
+  int lo = 0, n = B;  // it is one of lo .. lo + n - 1, or the last
+  while (n > 1) {
+    const int step = (n - 1) / 64 + 1;  // lane l asks whether sequence lo + (l + 1) step - 1 ends at or before the row
+    const int at = (lane + 1) * step;
+    const int below = __popcll(__ballot(at < n && s.start[lo + min(at, n)] <= row));
+    lo += below * step;
+    n = min(step, n - below * step);
+  }
+  return lo;
+}
+
 // The first key that the window leaves a row at position pos (negative: a row that sees nothing).
 __device__ __forceinline__ int window_begin(int pos, int window) {
   return window > 0 && pos >= window ? pos - window + 1 : 0;
@@ -257,11 +277,6 @@ struct Share {
 __device__ __forceinline__ long long uniform(long long v) {
   return (long long)(((unsigned long long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
                      (unsigned)__builtin_amdgcn_readfirstlane((int)v));
-}
-
-// a / b of a >= 0, b > 0; the 64-bit division takes a microsecond.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
 }
 
 // BLK keys a block, ROWS rows a block, OVER blocks for a list's beginning and end.

@@ -19,20 +19,24 @@ using bch::Seq;
 
 constexpr int kAnyWaves = 4;
 
-// Head dimensions that the matrix-core kernels do not take (below 4, and 257 to 1024): a workgroup per row and
-// query head, its wavefronts four keys in turn each, lane l the columns l + 64 t; a score is a reduction over the
+// Head dimensions that the matrix-core kernels do not take (below 4, and 257 to 1024): a workgroup per row of q
+// and query head, which looks for the row's sequence; its wavefronts four keys in turn each, lane l the columns l + 64 t; a score is a reduction over the
 // wavefront, four of them under way at a time.  Reads nothing that the row does not see.  Every row reads its
 // own K and V: 4 sequences of 2048 keys, 8 heads on 2, D 512, a token each: 1914 us with a wavefront per row and one
-// key at a time, 275 so; 64 tokens each 2241 and 831 (D 2: 787 and 130, 810 and 504).
+// key at a time, 275 so; 64 tokens each 2241 and 837 (D 2: 787 and 131, 810 and 511).
 template <int T>
-__global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCall c, int rows_per_seq) {
+__global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCall c, long long at0) {
   constexpr int U = 4;  // keys at a time
   __shared__ bch::TreeMasks tree;
   __shared__ float red_m[kAnyWaves], red_l[kAnyWaves], red_o[kAnyWaves][64 * T];
-  const int b = blockIdx.x / rows_per_seq, r = blockIdx.x % rows_per_seq;
+  const long long at = at0 + blockIdx.x;  // row of q * H + query head
+  const long long of = bch::quotient(at, c.H);
+  const int h = (int)(at - of * c.H), hk = h / (c.H / c.Hkv);
+  const int b = __builtin_amdgcn_readfirstlane(bch::seq_of_row(c.seqs, c.B, of, threadIdx.x & 63));
   const Seq s = bch::load_seq(c.kv, c.seqs, b);
-  const int i = r / c.H, h = r - i * c.H, hk = h / (c.H / c.Hkv);
-  if (i >= s.n) return;
+  const long long i_ = of - (c.seqs.start ? s.row0 : (long long)b * c.seqs.max_new);
+  if (i_ < 0 || i_ >= s.n) return;
+  const int i = (int)i_;
   if (c.parent) bch::tree_masks(tree, c.parent, s, c.window, c.sinks);
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -298,18 +302,20 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
     hipLaunchKernelGGL(paged_combine, dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, c, a, b, only_few ? few : 0);
     return hipGetLastError();
   }
-  const long long rows = (long long)c.seqs.max_new * c.H;
-  if (rows > 0x7fffffffLL || !fits_grid(rows * c.B, 64 * kAnyWaves)) return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)(rows * c.B)), block(64 * kAnyWaves);
-#define BCH_ANY(T_) hipLaunchKernelGGL(sdpa_paged_any_kernel<T_>, grid, block, 0, s, c, (int)rows)
-  if (c.D <= 64) BCH_ANY(1);
-  else if (c.D <= 128) BCH_ANY(2);
-  else if (c.D <= 256) BCH_ANY(4);
-  else if (c.D <= 512) BCH_ANY(8);
-  else if (c.D <= 1024) BCH_ANY(16);
-  else return hipErrorInvalidValue;
-#undef BCH_ANY
-  return hipGetLastError();
+  // the rows that there are, 2^23 workgroups a launch
+  auto any = c.D <= 64    ? sdpa_paged_any_kernel<1>
+             : c.D <= 256 ? nullptr  // the other kernels'
+             : c.D <= 512 ? sdpa_paged_any_kernel<8>
+                          : sdpa_paged_any_kernel<16>;
+  const long long tokens = c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new, most = 1LL << 23;
+  if (!any || c.D > 1024 || tokens > (1LL << 40) / c.H) return hipErrorInvalidConfiguration;
+  for (long long at = 0; at < tokens * c.H; at += most) {
+    const dim3 grid((unsigned)std::min(most, tokens * c.H - at)), block(64 * kAnyWaves);
+    hipLaunchKernelGGL(any, grid, block, 0, s, c, at);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace bch

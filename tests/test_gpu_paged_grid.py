@@ -97,3 +97,27 @@ def test_a_long_chunk_beside_many_sequences(dev, b, new, h, hkv, d, window, sink
     print(f"crowd b={b} new={new} h={h} hkv={hkv} d={d} {k}", flush=True)
     assert any(x is not True and x[1] < 0 for x in k.values()), "lists are not dealt out"
     Crowd(dev, b, b // 2, new, 33, h, hkv, d, page=16, window=window, sinks=sinks).check(200)
+
+
+@pytest.mark.parametrize("d", [2, 300])
+def test_a_chunk_beside_many_sequences_at_other_widths(dev, d):
+    """Widths that take a workgroup a row and head: 2^24 and more of them by the longest chunk's length."""
+    b, new, h, hkv = 1100, 8192, 2, 1
+    print(f"crowd b={b} new={new} d={d} {kernels(b, b + new - 1, new, new + 5, h, hkv, d, 40, 1)}", flush=True)
+    Crowd(dev, b, 700, new, 5, h, hkv, d, page=16, window=40, sinks=1).check(200)
+    # and more rows that there are than one launch takes
+    if d == 2:
+        Crowd(dev, 1 << 22, 5, 7, 5, 4, 2, d, page=4).check(500)
+
+
+def test_dense_batches_beyond_one_launch(dev):
+    b, h, sq, d = 1 << 20, 3, 3, 2
+    rng = np.random.default_rng(2)
+    q, k, v = (rng.standard_normal((b, h, sq, d), dtype=np.float32) for _ in range(3))
+    t = [Tensor.from_data(x, list(x.shape), dev) for x in (q, k, v)]
+    got = t[0].sliding_window_attention(t[1], t[2], 2, 1).to_numpy().reshape(q.shape)
+    scale = float(np.float32(1.0) / np.sqrt(np.float32(d)))
+    see = visible(0, sq, 2, 1)
+    for i in [0, b - 1] + list(rng.integers(0, b, 300)):
+        want = attend(*(x[i].transpose(1, 0, 2) for x in (q, k, v)), see, scale)
+        compare(got[i].transpose(1, 0, 2), want, tolerance(q[i], k[i], v[i], scale, sq))
