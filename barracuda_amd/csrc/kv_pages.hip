@@ -34,20 +34,38 @@ struct Elem<4> {
 // 5.6 TB/s; through them, four tokens 29; past them, one token 28.8, four 24.9).
 constexpr int kAppend = 2;
 
-template <int VEC>
-__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* k, float* v, KvSeqs seqs, int tiles,
-                                                             int Hkv, int D, const float* __restrict__ nk,
-                                                             SdpaLayout nkl, const float* __restrict__ nv,
-                                                             SdpaLayout nvl) {
+// FIND: kAppend rows of all that there are (from the at0'th kAppend on), whose sequences it looks for: where batch
+// times the longest sequence's new tokens is beyond a grid.  In ordinary batches the search costs some: a workgroup a
+// sequence and kAppend of its tokens / all rows, 8 ragged prompts 23.9 / 24.6 us, 16 sequences of up to 64 drafts in four
+// layers, with their keep, 28.5 / 29.7.
+template <int VEC, bool FIND>
+__global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* k, float* v, KvSeqs seqs, int B,
+                                                             int tiles, long long at0, int Hkv, int D,
+                                                             const float* __restrict__ nk, SdpaLayout nkl,
+                                                             const float* __restrict__ nv, SdpaLayout nvl) {
   typedef typename Elem<VEC>::type T;
-  const int b = blockIdx.x / tiles, i0 = (blockIdx.x % tiles) * kAppend;
-  const bch::Seq s = bch::load_seq(kv, seqs, b);
-  if (i0 >= s.n) return;
   bch::Slot slot[kAppend];
+  long long rows[kAppend];
+  if constexpr (FIND) {
 #pragma unroll
-  for (int u = 0; u < kAppend; ++u) {
-    const int j = s.first + i0 + u;
-    slot[u] = i0 + u < s.n && j >= 0 ? bch::key_slot(kv, b, j) : bch::Slot{-1, 0};
+    for (int u = 0; u < kAppend; ++u) {
+      const long long at = (at0 + blockIdx.x) * kAppend + u;
+      rows[u] = min(at, (long long)seqs.total - 1);
+      const int b = __builtin_amdgcn_readfirstlane(bch::seq_of_row(seqs, B, rows[u], threadIdx.x & 63));
+      const bch::Seq s = bch::load_seq(kv, seqs, b);
+      const long long i = rows[u] - s.row0, j = s.first + i;
+      slot[u] = at < seqs.total && i >= 0 && i < s.n && j >= 0 ? bch::key_slot(kv, b, (int)j) : bch::Slot{-1, 0};
+    }
+  } else {
+    const int b = blockIdx.x / tiles, i0 = (blockIdx.x % tiles) * kAppend;
+    const bch::Seq s = bch::load_seq(kv, seqs, b);
+    if (i0 >= s.n) return;
+#pragma unroll
+    for (int u = 0; u < kAppend; ++u) {
+      const int j = s.first + i0 + u;
+      slot[u] = i0 + u < s.n && j >= 0 ? bch::key_slot(kv, b, j) : bch::Slot{-1, 0};
+      rows[u] = s.row0 + min(i0 + u, s.n - 1);
+    }
   }
   const int dv = D / VEC;
   for (int e = threadIdx.x; e < Hkv * dv; e += kThreads) {
@@ -55,9 +73,8 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* 
     T x[kAppend], y[kAppend];
 #pragma unroll
     for (int u = 0; u < kAppend; ++u) {
-      const long long row = s.row0 + min(i0 + u, s.n - 1);
-      x[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(nk + row * nkl.row + h * nkl.head + d));
-      y[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(nv + row * nvl.row + h * nvl.head + d));
+      x[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(nk + rows[u] * nkl.row + h * nkl.head + d));
+      y[u] = __builtin_nontemporal_load(reinterpret_cast<const T*>(nv + rows[u] * nvl.row + h * nvl.head + d));
     }
 #pragma unroll
     for (int u = 0; u < kAppend; ++u)
@@ -176,16 +193,21 @@ namespace bch {
 
 hipError_t launch_kv_append(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B, int Hkv,
                             int D, const float* nk, const SdpaLayout& nkl, const float* nv, const SdpaLayout& nvl) {
-  const int tiles = (seqs.max_new + kAppend - 1) / kAppend;
-  if ((long long)tiles * B > 0x7fffffffLL || (long long)Hkv * D > 0x7fffffffLL - kThreads)
-    return hipErrorInvalidConfiguration;
-  const dim3 grid((unsigned)(tiles * B)), block(kThreads);
-  if (vec4(kv, k, v, D) && aligned16(nk) && aligned16(nv) && nkl.row % 4 == 0 && nkl.head % 4 == 0 &&
-      nvl.row % 4 == 0 && nvl.head % 4 == 0)
-    hipLaunchKernelGGL(kv_append_kernel<4>, grid, block, 0, s, kv, k, v, seqs, tiles, Hkv, D, nk, nkl, nv, nvl);
-  else
-    hipLaunchKernelGGL(kv_append_kernel<1>, grid, block, 0, s, kv, k, v, seqs, tiles, Hkv, D, nk, nkl, nv, nvl);
-  return hipGetLastError();
+  if ((long long)Hkv * D > 0x7fffffffLL - kThreads) return hipErrorInvalidConfiguration;
+  const int tiles = (seqs.max_new - 1) / kAppend + 1;
+  const bool vec = vec4(kv, k, v, D) && aligned16(nk) && aligned16(nv) && nkl.row % 4 == 0 && nkl.head % 4 == 0 &&
+                   nvl.row % 4 == 0 && nvl.head % 4 == 0;
+  const bool find = !fits_grid((long long)tiles * B, kThreads);
+  const long long all = find ? (seqs.total - 1LL) / kAppend + 1 : (long long)tiles * B, most = find ? 1 << 23 : all;
+  auto kern = find ? (vec ? kv_append_kernel<4, true> : kv_append_kernel<1, true>)
+                   : (vec ? kv_append_kernel<4, false> : kv_append_kernel<1, false>);
+  for (long long at = 0; at < all; at += most) {
+    const dim3 grid((unsigned)std::min(most, all - at)), block(kThreads);
+    hipLaunchKernelGGL(kern, grid, block, 0, s, kv, k, v, seqs, B, tiles, at, Hkv, D, nk, nkl, nv, nvl);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 hipError_t launch_kv_copy_pages(hipStream_t s, const KvPages& kv, float* k, float* v, int layers, long long k_layer,

@@ -121,3 +121,42 @@ def test_dense_batches_beyond_one_launch(dev):
     for i in [0, b - 1] + list(rng.integers(0, b, 300)):
         want = attend(*(x[i].transpose(1, 0, 2) for x in (q, k, v)), see, scale)
         compare(got[i].transpose(1, 0, 2), want, tolerance(q[i], k[i], v[i], scale, sq))
+
+
+@pytest.mark.parametrize("b,new,d", [(4096, 8193, 3), (4096, 8193, 4), (1 << 22, 9, 3), (1 << 22, 9, 4), (3, 1 << 25, 3)])
+def test_append_of_batches_beyond_a_grid(dev, b, new, d):
+    """2^24 and more places of two tokens by the longest chunk's length: every key into its page, bit for bit, and
+    nothing beside them."""
+    print(f"append b={b} new={new} d={d}", flush=True)
+    rng = np.random.default_rng(b)
+    page, at = 16, b // 2
+    news = np.ones(b, np.int64)
+    news[at] = new
+    news[rng.integers(0, b, b // 5)] = 0
+    news[[0, at]] = [1, new]
+    start = np.concatenate([[0], np.cumsum(news)])
+    total = int(start[-1])
+    lens = np.minimum(news + rng.integers(0, 9, b), page)
+    lens[at] = new + 21
+    # every sequence has a page of its own, the long one as many as it needs
+    held = -(-int(lens[at]) // page)
+    table = np.full((b, held), -1, np.int32)
+    table[:, 0] = rng.permutation(b)
+    table[at] = [table[at, 0]] + list(range(b, b + held - 1))
+    num = b + held
+    new_k = rng.standard_normal((total, d), dtype=np.float32)
+    new_v = new_k[::-1].copy()
+    pool = [Tensor.from_data(np.full((num, page, d), 5.0, np.float32), [num, page, d], dev) for _ in range(2)]
+    t = [Tensor.from_data(x, [total, d], dev) for x in (new_k, new_v)]
+    i32 = _I32(dev, start, lens, table)
+    lay, row = N.AttnLayout(page * d, page * d, d), N.AttnLayout(0, d, d)
+    kv = N.KvPages(pool[0].ptr, pool[1].ptr, lay, lay, num, page, 1, d, i32.ptrs[2], held)
+    batch = N.KvBatch(b, total, new, int(lens.max()), i32.ptrs[0], i32.ptrs[1])
+    dev.check(dev._lib.bch_kv_append(dev.ctx, kv, batch, C.c_void_p(t[0].ptr), row, C.c_void_p(t[1].ptr), row), "append")
+    which = np.repeat(np.arange(b), news)
+    j = (lens - news - start[:-1])[which] + np.arange(total)
+    p, slot = table[which, j // page], j % page
+    for got, x in zip(pool, (new_k, new_v)):
+        want = np.full((num, page, d), 5.0, np.float32)
+        want[p, slot] = x
+        assert np.array_equal(got.to_numpy().reshape(want.shape).view(np.uint32), want.view(np.uint32))
