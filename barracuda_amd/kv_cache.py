@@ -40,6 +40,7 @@ from .tensor import HipDevice, Tensor, _Buffer, _I32_MAX, get_device
 __all__ = ["KvCache", "KvStep"]
 
 MAX_DRAFTS = 128  # of one sequence's tree
+_KEEP_SEQUENCES, _KEEP_LAYERS = 65535, 32767  # of one bch_kv_keep
 
 
 class _I32:
@@ -418,12 +419,17 @@ class KvCache:
                 table[i, :len(s.pages)] = s.pages
             start = np.concatenate([[0], np.cumsum([len(p) for _, _, p in moving])])
             arrays = _I32(self.device, start, [x for _, _, p in moving for x in p], [to for _, to, _ in moving], table)
-            kv = N.KvPages(self.k.ptr, self.v.ptr, self._layout, self._layout, self.num_pages, self.page_size,
-                           self.kv_heads, self.head_dim, arrays.ptrs[3], width)
+            starts, keep, tos, tables = arrays.ptrs
             dev = self.device
-            with dev._lock:
-                dev.check(dev._lib.bch_kv_keep(dev.ctx, kv, self.layers, self._layer, self._layer, len(moving),
-                                               int(start[-1]), C.c_void_p(arrays.ptrs[0]), C.c_void_p(arrays.ptrs[1]),
-                                               C.c_void_p(arrays.ptrs[2])), "kv_keep")
+            for b0 in range(0, len(moving), _KEEP_SEQUENCES):
+                b1 = min(b0 + _KEEP_SEQUENCES, len(moving))
+                for l0 in range(0, self.layers, _KEEP_LAYERS):
+                    at = 4 * l0 * self._layer
+                    kv = N.KvPages(self.k.ptr + at, self.v.ptr + at, self._layout, self._layout, self.num_pages,
+                                   self.page_size, self.kv_heads, self.head_dim, tables + 4 * b0 * width, width)
+                    with dev._lock:
+                        dev.check(dev._lib.bch_kv_keep(dev.ctx, kv, min(_KEEP_LAYERS, self.layers - l0), self._layer,
+                                                       self._layer, b1 - b0, int(start[b1]), C.c_void_p(starts + 4 * b0),
+                                                       C.c_void_p(keep), C.c_void_p(tos + 4 * b0)), "kv_keep")
         for seq, to, positions in moves:
             self._cut(self._seqs[seq], to + len(positions))

@@ -459,7 +459,8 @@ bch_status bch_kv_copy_pages(bch_ctx *ctx, const bch_kv_pages *kv, int layers,
  * drafts of a verification step, or what an eviction leaves).  start [B+1],
  * keep [total] and to [B] are device memory.  A sequence's keep must ascend,
  * with keep[start[b]+i] >= to[b]+i; keys that would move up, and keys of pages
- * that are not held, stay.  The pages written must not be shared. */
+ * that are not held, stay.  The pages written must not be shared.  At most
+ * 65535 sequences and 32767 layers a call (BCH_E_UNSUPPORTED). */
 bch_status bch_kv_keep(bch_ctx *ctx, const bch_kv_pages *kv, int layers,
                        long long k_layer_stride, long long v_layer_stride,
                        int B, int total, const int *start, const int *keep,

@@ -408,3 +408,41 @@ def test_c_calls_refuse_before_any_device_call():
     assert keep(b=-1) == S and keep(total=-1) == S and keep(layers=-1) == S and keep(stride=-1) == S
     assert keep(b=65536) == U and keep(layers=32768) == U
     assert keep(kv=_pages(table_width=0)) == S
+
+
+class _LimitedLib(_HostLib):
+    """Refuses what bch_kv_keep refuses."""
+
+    def bch_kv_keep(self, ctx, kv, layers, ks, vs, b, total, start, keep, to):
+        if b > 65535 or layers > 32767:
+            return N.BCH_E_UNSUPPORTED
+        return super().bch_kv_keep(ctx, kv, layers, ks, vs, b, total, start, keep, to)
+
+
+def test_keep_of_more_sequences_than_one_call_takes():
+    """As many as one step may have; the ones with nothing to move among them."""
+    cache = _cache(layers=1, pages=140000, page=1, heads=1, d=1)
+    cache.device._lib = _LimitedLib()
+    seqs = [cache.new_sequence() for _ in range(70000)]
+    step = cache.batch([(s, 2) for s in seqs])
+    _append(cache, step, 0)
+    kept = [[] if s % 50 == 7 else [s % 3 // 2] for s in seqs]
+    cache.keep(step, kept)
+    k = cache.k.to_numpy().reshape(-1)
+    for s, ids in zip(seqs, kept):
+        assert [k[p] for p in cache.pages(s)] == [2 * s + x for x in ids]
+    assert cache.device._lib.calls.count("keep") == 2
+
+
+def test_keep_in_more_layers_than_one_call_takes():
+    cache = _cache(layers=40000, pages=3, page=1, heads=1, d=1)
+    cache.device._lib = _LimitedLib()
+    a = cache.new_sequence()
+    step = cache.batch([(a, 2)])
+    old, new = cache.pages(a)
+    for pool in (cache.k, cache.v):
+        x = np.ctypeslib.as_array(C.cast(pool.ptr, C.POINTER(C.c_float)), (cache.layers, 3))
+        x[:, new] = np.arange(cache.layers)
+    cache.keep(step, [[1]])
+    for pool in (cache.k, cache.v):
+        assert np.array_equal(pool.to_numpy().reshape(-1, 3)[:, old], np.arange(cache.layers))
