@@ -410,7 +410,6 @@ class KvCache:
                 raise InvalidOperation("KvCache", "a page that kept keys move into has been evicted")
             written += [(s, i) for i in pages]
         self._own_pages(written)
-        self._generation += 1
         moving = [(self._seqs[seq], to, positions) for seq, to, positions in moves if positions]
         if any(positions != list(range(to, to + len(positions))) for _, to, positions in moving):
             width = max(len(s.pages) for s, _, _ in moving)
@@ -421,6 +420,7 @@ class KvCache:
             arrays = _I32(self.device, start, [x for _, _, p in moving for x in p], [to for _, to, _ in moving], table)
             starts, keep, tos, tables = arrays.ptrs
             dev = self.device
+            self._generation += 1  # (not before: until here the step may be tried again)
             for b0 in range(0, len(moving), _KEEP_SEQUENCES):
                 b1 = min(b0 + _KEEP_SEQUENCES, len(moving))
                 for l0 in range(0, self.layers, _KEEP_LAYERS):
@@ -431,5 +431,6 @@ class KvCache:
                         dev.check(dev._lib.bch_kv_keep(dev.ctx, kv, min(_KEEP_LAYERS, self.layers - l0), self._layer,
                                                        self._layer, b1 - b0, int(start[b1]), C.c_void_p(starts + 4 * b0),
                                                        C.c_void_p(keep), C.c_void_p(tos + 4 * b0)), "kv_keep")
+        self._generation += 1
         for seq, to, positions in moves:
             self._cut(self._seqs[seq], to + len(positions))

@@ -446,3 +446,18 @@ def test_keep_in_more_layers_than_one_call_takes():
     cache.keep(step, [[1]])
     for pool in (cache.k, cache.v):
         assert np.array_equal(pool.to_numpy().reshape(-1, 3)[:, old], np.arange(cache.layers))
+
+
+def test_a_failed_upload_leaves_a_step_that_can_be_kept():
+    cache = _cache()
+    a = cache.new_sequence()
+    step = cache.batch([(a, 5)], [[-1, 0, 0, 1, 1]])
+    _append(cache, step, 0)
+    cache.device.fail_uploads = True
+    with pytest.raises(OutOfMemory):
+        cache.keep(step, [[0, 2, 4]])
+    cache.device.fail_uploads = False
+    assert cache.length(a) == 5
+    cache.keep(step, [[0, 2, 4]])
+    assert _read(cache, a) == [0, 2, 4]
+    _check_pages(cache)
