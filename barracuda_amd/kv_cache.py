@@ -82,15 +82,23 @@ class KvStep:
         self._batch = N.KvBatch(len(lens), self.total, max([0] + self.counts), max([0] + lens), start, length)
         self._table, self._width = tab, width
         self._parents = C.c_void_p(par) if parents is not None else None
+        # of each sequence with new tokens the evicted keys: the first, the end, and the keys before the new tokens
+        self._gone = []
+        for s, n, length in zip(sequences, counts, lens):
+            if n and cache._seqs[s].evicted:
+                at = [i for i, p in enumerate(cache._seqs[s].pages) if p < 0]
+                if at:
+                    self._gone.append((at[0] * cache.page_size, (at[-1] + 1) * cache.page_size, length - n))
         self._generation = cache._generation
 
 
 class _Sequence:
-    __slots__ = ("pages", "length")
+    __slots__ = ("pages", "length", "evicted")
 
     def __init__(self):
         self.pages: list[int] = []  # -1: given back by evict
         self.length = 0
+        self.evicted = False  # whether there may be such pages
 
 
 class KvCache:
@@ -126,7 +134,7 @@ class KvCache:
         """A sequence with the same keys, its pages shared until one of the two
         writes into them."""
         s, f = self._seq(sequence), self.new_sequence()
-        self._seqs[f].pages, self._seqs[f].length = list(s.pages), s.length
+        self._seqs[f].pages, self._seqs[f].length, self._seqs[f].evicted = list(s.pages), s.length, s.evicted
         for p in s.pages:
             if p >= 0:
                 self._refs[p] += 1
@@ -212,7 +220,8 @@ class KvCache:
         with heads a multiple of kv_heads, scale 1/sqrt(head_dim) unless given.
         A row sees the keys up to its own (a draft: the committed ones, its
         ancestors and itself); with window > 0 only those less than `window`
-        positions back and the first `sinks`."""
+        positions back and the first `sinks`.  InvalidOperation if one of them
+        has been evicted."""
         self._check_step("KvCache.attention", step, layer)
         shape = q.shape()
         if len(shape) != 3 or shape[0] != step.total or shape[2] != self.head_dim:
@@ -222,6 +231,10 @@ class KvCache:
             raise InvalidInput(f"num_q_heads ({heads}) must be divisible by num_kv_heads ({self.kv_heads})")
         if window < 0 or sinks < 0:
             raise InvalidInput(f"window ({window}) and sinks ({sinks}) must not be negative")
+        for begin, end, committed in step._gone:
+            if window == 0 or begin < sinks or end > committed - window + 1:
+                raise InvalidOperation("KvCache.attention", f"a row would see keys that have been evicted (of {begin} to "
+                                       f"{end - 1}, {committed} keys before its own, window {window}, sinks {sinks})")
         self._own(q)
         out = Tensor.empty(shape, self.device)
         if step.total == 0:
@@ -267,7 +280,8 @@ class KvCache:
         self._move([(sequence, same, positions[same:])])
 
     def truncate(self, sequence: int, length: int) -> None:
-        """Give up all but the first `length` keys."""
+        """Give up all but the first `length` keys.  Windows then reach further
+        back than before: into evicted pages, where attention is refused."""
         s = self._seq(sequence)
         if not 0 <= length <= s.length:
             raise InvalidInput(f"KvCache.truncate: length {length} of a sequence of {s.length}")
@@ -277,7 +291,9 @@ class KvCache:
     def evict(self, sequence: int, window: int, sinks: int = 0) -> int:
         """Give back the pages whose keys no later token sees through this
         window and these sinks; the other keys keep their positions.  Returns
-        the number of pages given back."""
+        the number of pages given back.  Attention of a later token that would
+        see one of their keys all the same (through a larger window, with more
+        sinks, or after truncate) is refused."""
         s = self._seq(sequence)
         if window < 1 or sinks < 0:
             raise InvalidInput(f"KvCache.evict: window ({window}) must be at least 1, sinks ({sinks}) not negative")
@@ -289,6 +305,7 @@ class KvCache:
                 s.pages[i] = -1
                 n += 1
         if n:
+            s.evicted = True
             self._generation += 1
         return n
 

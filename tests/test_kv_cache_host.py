@@ -13,6 +13,7 @@ import pytest
 from barracuda_amd import _native as N
 from barracuda_amd import KvCache, SlidingWindowAttention, Tensor
 from barracuda_amd.error import InvalidInput, InvalidOperation, OutOfMemory, ShapeMismatch
+from tests.kv_model import visible
 
 
 class _HostLib:
@@ -461,3 +462,82 @@ def test_a_failed_upload_leaves_a_step_that_can_be_kept():
     cache.keep(step, [[0, 2, 4]])
     assert _read(cache, a) == [0, 2, 4]
     _check_pages(cache)
+
+
+class _SeenLib(_HostLib):
+    """Attention that only notes that it was called."""
+
+    def bch_sdpa_paged(self, ctx, kv, batch, h, scale, window, sinks, parent, q, ql, o, ol):
+        self.calls.append(("attention", window, sinks))
+        return N.BCH_OK
+
+
+def _attends(cache, step, window, sinks):
+    """Whether attention through this window takes the step, and that it does in every layer or in none."""
+    q = Tensor.from_data(np.zeros((step.total, 2, 3)), [step.total, 2, 3], cache.device)
+    took = []
+    for layer in range(cache.layers):
+        n = len(cache.device._lib.calls)
+        try:
+            cache.attention(step, layer, q, window, sinks)
+            took.append(True)
+        except InvalidOperation as e:
+            assert "evict" in str(e)
+            took.append(False)
+        assert (len(cache.device._lib.calls) > n) == (took[-1] and step.total > 0)
+    assert len(set(took)) == 1
+    return took[0]
+
+
+def test_attention_that_would_see_evicted_keys_is_refused():
+    """Evicted keys may not silently count as nothing: after a truncation, through a larger window or with more
+    sinks than evict was told of, a row would see them."""
+    cache = _cache(page=4)
+    cache.device._lib = _SeenLib()
+    a, b = cache.new_sequence(), cache.new_sequence()
+    _append(cache, cache.batch([(a, 21), (b, 9)]), 0)
+    assert cache.evict(a, window=8, sinks=3) == 2  # pages 1 and 2: keys 4 .. 11; the next token sees 14 on
+    step = cache.batch([(a, 1), (b, 2)])
+    assert _attends(cache, step, 8, 3) and _attends(cache, step, 10, 4) and _attends(cache, step, 1, 0)
+    for window, sinks in ((0, 0), (11, 0), (2**40, 0), (8, 5), (8, 2**40)):
+        assert not _attends(cache, step, window, sinks), (window, sinks)
+    assert _attends(cache, cache.batch([(a, 0), (b, 1)]), 0, 0)  # no row of the sequence
+    f = cache.fork(a)
+    cache.truncate(a, 17)
+    step = cache.batch([(a, 2), (f, 2)], [[-1, 0], [-1, -1]])  # now key 17 would see 10 and 11 through 8
+    assert not _attends(cache, step, 8, 3) and _attends(cache, step, 6, 3)
+    assert _attends(cache, cache.batch([(f, 1)]), 8, 3)
+    cache.retain(a, [0, 1, 2, 3])
+    step = cache.batch([(a, 1)])
+    assert _attends(cache, step, 0, 0)
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_attention_is_refused_exactly_where_an_evicted_key_would_be_seen(seed):
+    rng = np.random.default_rng(seed)
+    cache = _cache(page=int(rng.integers(1, 5)), pages=60)
+    cache.device._lib = _SeenLib()
+    for _ in range(40):
+        seqs = [cache.new_sequence() for _ in range(2)]
+        _append(cache, cache.batch([(s, int(rng.integers(1, 30))) for s in seqs]), 0)
+        for s in seqs:
+            for _ in range(int(rng.integers(0, 3))):
+                cache.evict(s, int(rng.integers(1, 12)), int(rng.integers(0, 6)))
+            if rng.random() < 0.4:
+                cache.truncate(s, int(rng.integers(0, cache.length(s) + 1)))
+        counts = [int(rng.integers(0, 4)) for _ in seqs]
+        parents = [[int(rng.integers(-1, j)) if j else -1 for j in range(n)] for n in counts] if rng.random() < 0.5 else None
+        try:
+            step = cache.batch(zip(seqs, counts), parents)
+        except InvalidOperation:
+            counts = [0, 0]
+            step = cache.batch(zip(seqs, counts))
+            parents = None
+        window, sinks = int(rng.integers(0, 14)), int(rng.integers(0, 8))
+        hidden = False
+        for i, (s, n) in enumerate(zip(seqs, counts)):
+            see = visible(cache.length(s) - n, n, window, sinks, parents[i] if parents else None).any(0)
+            hidden |= any(x and cache.pages(s)[j // cache.page_size] < 0 for j, x in enumerate(see))
+        assert _attends(cache, step, window, sinks) == (not hidden), (window, sinks)
+        for s in seqs:
+            cache.free(s)
