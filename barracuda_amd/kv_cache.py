@@ -40,6 +40,7 @@ from .tensor import HipDevice, Tensor, _Buffer, _I32_MAX, get_device
 __all__ = ["KvCache", "KvStep"]
 
 MAX_DRAFTS = 128  # of one sequence's tree
+_MAX_KEYS = 2**31 - 256  # of a sequence
 _KEEP_SEQUENCES, _KEEP_LAYERS = 65535, 32767  # of one bch_kv_keep
 
 
@@ -171,7 +172,7 @@ class KvCache:
         if len({s for s, _ in items}) != len(items):
             raise InvalidInput("KvCache.batch: a sequence is named twice")
         for s, n in items:
-            if n < 0 or self._seqs[s].length + n > _I32_MAX:
+            if n < 0 or self._seqs[s].length + n > _MAX_KEYS:
                 raise InvalidInput(f"KvCache.batch: {n} new tokens for sequence {s}")
         if sum(n for _, n in items) > _I32_MAX:
             raise InvalidInput("KvCache.batch: too many new tokens")
