@@ -545,7 +545,7 @@ def test_attention_is_refused_exactly_where_an_evicted_key_would_be_seen(seed):
 
 def test_sequences_longer_than_the_kernels_count_are_refused():
     """2^31 - 256 keys: a longer length counts as that many, and its last tokens would go astray."""
-    cache = _cache(page=2**20, pages=1, heads=1, d=1, layers=1)
+    cache = _cache(page=1, pages=1, heads=1, d=1, layers=1)
     a = cache.new_sequence()
     cache._seqs[a].length = 2**31 - 256 - 2
     with pytest.raises(InvalidInput):
