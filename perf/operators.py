@@ -284,9 +284,6 @@ def _handles(case, x):
         own_state["o"] = torch.empty_like(x["q"])
     if "new_k" in x:
         own_state["new"] = _native.AttnLayout(0, d, hkv * d)
-    if case["kind"] == "fork":
-        own_state["src"] = (ctypes.c_int * len(x["src"]))(*x["src"])
-        own_state["dst"] = (ctypes.c_int * len(x["dst"]))(*x["dst"])
     return own_state
 
 
@@ -324,8 +321,8 @@ def _run_own(s):
             dev.check(lib.bch_kv_append(dev.ctx, kv[i], s["batch"], _p(x["new_k"][i]), s["new"], _p(x["new_v"][i]),
                                         s["new"]), "append")
     if kind == "fork":
-        dev.check(lib.bch_kv_copy_pages(dev.ctx, kv[0], len(kv), stride, stride, len(s["src"]), s["src"], s["dst"]),
-                  "copy_pages")
+        src, dst = (x[p].ctypes.data_as(ctypes.POINTER(ctypes.c_int)) for p in ("src", "dst"))
+        dev.check(lib.bch_kv_copy_pages(dev.ctx, kv[0], len(kv), stride, stride, len(x["src"]), src, dst), "copy_pages")
     elif kind == "keep":
         dev.check(lib.bch_kv_keep(dev.ctx, kv[0], len(kv), stride, stride, len(x["to"]), len(x["keep"]),
                                   _p(x["keep_start"]), _p(x["keep"]), _p(x["to"])), "keep")
