@@ -220,8 +220,8 @@ struct SharePlan {
   int rows, tiles;       // rows of a row block, row blocks of the longest sequence
   int part_rows;         // rows of a part: a row block's, if any sequence has as many
   int shares;            // workgroups of the line; 0 (no workspace): a workgroup a list
-  int min_share;
-  int whole;  // the line's lists are not cut (no workspace either)
+  int min_share;         // of a share, in blocks; 0: the line's lists are not cut (no workspace either)
+  __host__ __device__ bool whole() const { return min_share == 0; }
 };
 // Workspace: for every list the workgroup of its first part and the number of its parts (in that workgroup and
 // the ones behind it), then two parts a workgroup, the one that ends a list begun before its share and the one
@@ -235,7 +235,7 @@ inline long long lists_of(const PagedCall& c, const SharePlan& p) { return (long
 // A grid has fewer than 2^32 threads.
 inline bool fits_grid(long long workgroups, int threads) { return workgroups < (1LL << 32) / threads; }
 inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
-  if (p.shares == 0 || p.whole) return 0;
+  if (p.shares == 0 || p.whole()) return 0;
   const long long lists = lists_of(c, p);
   return sizeof(float) * (size_t)(notes_floats(lists) + 2LL * p.shares * part_floats(p, c.D));
 }
@@ -244,8 +244,7 @@ inline size_t share_bytes(const PagedCall& c, const SharePlan& p) {
 inline void deal_whole(const PagedCall& c, SharePlan& p, int threads, int workgroups) {
   if (p.shares > 0 || fits_grid(lists_of(c, p), threads)) return;
   p.shares = workgroups;
-  p.min_share = 1;
-  p.whole = 1;
+  p.min_share = 0;
 }
 
 // The lists of 64 sequences from b0 on, one sequence a lane.
@@ -311,7 +310,7 @@ struct Shares {
   static __device__ __forceinline__ void begin(Share& f, const PagedCall& c, const SharePlan& plan, int lane) {
     Lane64 seqs;
     long long total = 0, lists = 0;
-    int part = plan.whole ? 0x7fffffff : 0;  // (that many blocks are any list)
+    int part = plan.whole() ? 0x7fffffff : 0;  // (that many blocks are any list)
     for (int b0 = 0; b0 < c.B; b0 += 64) {
       seqs = line(c, plan, b0, lane, part);
       total += uniform(__shfl(seqs.sum, 63));
@@ -321,16 +320,16 @@ struct Shares {
       lists += (long long)c.Hkv * __builtin_amdgcn_readfirstlane(n);
     }
     const long long grid = gridDim.x;
-    long long share = max((long long)plan.min_share, quotient(total + grid - 1, grid));
+    long long share = max((long long)max(plan.min_share, 1), quotient(total + grid - 1, grid));
     // parts of one list each: ceil(w / part) <= w / part + 1 of them, in all no more than workgroups; up to a
     // twentieth longer than the shares
-    if (!plan.whole && lists < grid) {
+    if (!plan.whole() && lists < grid) {
       const long long p = max((long long)plan.min_share, quotient(total + grid - lists - 1, grid - lists));
       if (20 * p <= 21 * share && p <= 0x7fffffff) part = (int)p;
     }
     if (part || c.B > 64) seqs = line(c, plan, 0, lane, part);
     f.seqs[lane] = seqs;
-    if (part && !plan.whole) {
+    if (part && !plan.whole()) {
       share = 1;
       total = 0;
       for (int b0 = 0; b0 < c.B; b0 += 64)
@@ -388,13 +387,14 @@ __device__ __forceinline__ Piece read_piece(const Piece& f) {
   return {{u(f.seq.row0), u(f.seq.n), u(f.seq.len), u(f.seq.first)}, u(f.b), u(f.hk), u(f.rb), u(f.p0), u(f.p1),
           u(f.slot), u(f.count), u(f.parts)};
 }
-// Where a workgroup leaves its part of a list that was cut, and (the first part's) the list's note.
+// Where a workgroup leaves its part of a list that was cut, and (the first part's) the list's note; ws is null where
+// no list is.
 __device__ __forceinline__ float* part_of(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
   return ws + notes_floats((long long)c.B * c.Hkv * plan.tiles) +
          part_at(plan, (int)blockIdx.x - p.slot, p.slot, c.D);
 }
 __device__ __forceinline__ void note_list(float* ws, const PagedCall& c, const SharePlan& plan, const Piece& p) {
-  if (plan.shares > 0 && !plan.whole && p.slot == 0) {
+  if (ws && p.slot == 0) {
     int* note = reinterpret_cast<int*>(ws) + 2 * (((long long)p.b * c.Hkv + p.hk) * plan.tiles + p.rb);
     note[0] = blockIdx.x;
     note[1] = p.count;

@@ -269,7 +269,7 @@ const char* sdpa_paged_kernel_name(const PagedCall& c, int max_len) {
   int at = 0;
   auto add = [&](const char* name, const SharePlan& p) {
     at += snprintf(text + at, sizeof text - at, "%s%s rows=%d", at > 0 ? " + " : "", name, p.rows);
-    if (p.whole) at += snprintf(text + at, sizeof text - at, " dealt=%d", p.shares);
+    if (p.whole()) at += snprintf(text + at, sizeof text - at, " dealt=%d", p.shares);
     else if (p.shares > 0) at += snprintf(text + at, sizeof text - at, " shares=%d least=%d", p.shares, p.min_share);
     else at += snprintf(text + at, sizeof text - at, " whole");
   };
@@ -285,14 +285,14 @@ hipError_t launch_sdpa_paged(hipStream_t s, const PagedCall& c, int max_len, voi
   Route r = route(c, max_len, true);
   if (ws_bytes < r.bytes) r = route(c, max_len, false);
   if (r.tile || r.rows) {
-    float* tile_ws = static_cast<float*>(ws);
-    float* rows_ws = tile_ws + r.tile_bytes / sizeof(float);
+    float* tile_ws = r.tile_bytes > 0 ? static_cast<float*>(ws) : nullptr;
+    float* rows_ws = r.bytes > r.tile_bytes ? static_cast<float*>(ws) + r.tile_bytes / sizeof(float) : nullptr;
     hipError_t e = r.tile ? launch_sdpa_paged_tile(s, c, r.tile_plan, tile_ws) : hipSuccess;
     if (e == hipSuccess && r.rows) e = launch_sdpa_paged_rows(s, c, r.rows_plan, rows_ws);
     if (e != hipSuccess || r.bytes == 0) return e;
     Combined a{r.tile_plan, tile_ws}, b{r.rows_plan, rows_ws};
-    if (a.plan.whole) a.plan.shares = 0;  // nothing of it to join
-    if (b.plan.whole) b.plan.shares = 0;
+    if (a.plan.whole()) a.plan.shares = 0;  // nothing of it to join
+    if (b.plan.whole()) b.plan.shares = 0;
     const long long rows = (c.seqs.start ? (long long)c.seqs.total : (long long)c.B * c.seqs.max_new) * c.H;
     // where only short sequences can have been cut, their first tokens, if those are fewer
     const int group = c.H / c.Hkv, few = std::min(kFewRows / group, c.seqs.max_new);

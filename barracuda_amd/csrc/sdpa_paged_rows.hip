@@ -475,7 +475,6 @@ SharePlan sdpa_paged_rows_plan(const PagedCall& c, int max_len, int row_limit, b
     p.shares = resident(c.D, p.rows);
   }
   p.part_rows = std::min(most, p.rows);
-  p.whole = 0;
   deal_whole(c, p, 512, resident(c.D, p.rows));
   return p;
 }

@@ -650,7 +650,6 @@ SharePlan sdpa_paged_tile_plan(const PagedCall& c, int max_len, bool may_split) 
   const long long full = rows / p.rows, keys = most_keys(c, max_len);
   const bool alike = keys >= 1024 && keys > 2LL * c.seqs.max_new;
   p.shares = may_split && full <= (alike ? 2 * cu : cu / 2) ? (int)cu : 0;
-  p.whole = 0;
   deal_whole(c, p, TileCfg<32>::NT, (int)cu);
   return p;
 }
