@@ -30,14 +30,15 @@ struct Elem<4> {
 
 // ---- append: row i of sequence b is key len[b] - n + i ----
 // A workgroup takes kAppend tokens of one sequence; a thread the same columns of each, K and V, with
-// all of its loads ahead of its stores, past the caches (8 ragged prompts, 8391 tokens of 8 KB, 133 MB: 23.8 us,
+// all of its loads ahead of its stores, past the caches (8 ragged prompts, 8128 tokens of 8 KB, 133 MB: 23.8 us,
 // 5.6 TB/s; through them, four tokens 29; past them, one token 28.8, four 24.9).
 constexpr int kAppend = 2;
 
 // FIND: kAppend rows of all that there are (from the at0'th kAppend on), whose sequences it looks for: where batch
 // times the longest sequence's new tokens is beyond a grid.  In ordinary batches the search costs some: a workgroup a
 // sequence and kAppend of its tokens / all rows, 8 ragged prompts 23.9 / 24.6 us, 16 sequences of up to 64 drafts in four
-// layers, with their keep, 28.5 / 29.7.
+// layers, with their keep, 28.5 / 29.7.  (Beside a long chunk it would save: 127 tokens and a chunk of 8192 take 207 us
+// by sequence, 7 and 23 apart.)
 template <int VEC, bool FIND>
 __global__ __launch_bounds__(kThreads) void kv_append_kernel(KvPages kv, float* k, float* v, KvSeqs seqs, int B,
                                                              int tiles, long long at0, int Hkv, int D,

@@ -19,11 +19,11 @@ using bch::Seq;
 
 constexpr int kAnyWaves = 4;
 
-// Head dimensions that the matrix-core kernels do not take (below 4, and 257 to 1024): a workgroup per row of q
-// and query head, which looks for the row's sequence; its wavefronts four keys in turn each, lane l the columns l + 64 t; a score is a reduction over the
-// wavefront, four of them under way at a time.  Reads nothing that the row does not see.  Every row reads its
-// own K and V: 4 sequences of 2048 keys, 8 heads on 2, D 512, a token each: 1914 us with a wavefront per row and one
-// key at a time, 275 so; 64 tokens each 2241 and 837 (D 2: 787 and 131, 810 and 511).
+// Head dimensions that the matrix-core kernels do not take (below 4, and 257 to 1024): a workgroup per row of q and
+// query head, which looks for the row's sequence; its wavefronts four keys in turn each, lane l the columns l + 64 t;
+// a score is a reduction over the wavefront, four of them under way at a time.  Reads nothing that the row does not
+// see.  Every row reads its own K and V: 4 sequences of 2048 keys, 8 heads on 2, D 512, a token each: 1914 us with a
+// wavefront per row and one key at a time, 276 so; 64 tokens each 2241 and 837 (D 2: 787 and 131, 810 and 511).
 template <int T>
 __global__ __launch_bounds__(64 * kAnyWaves) void sdpa_paged_any_kernel(PagedCall c, long long at0) {
   constexpr int U = 4;  // keys at a time

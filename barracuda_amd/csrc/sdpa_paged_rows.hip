@@ -1,8 +1,8 @@
 // sdpa_paged_rows.hip -- attention over a paged cache for few rows a sequence: a decode step, a small
 // tree of drafts, a short chunk (paged.h says which keys a row sees).
 //
-// What bounds it: reading the visible K and V once: 4 sequences of 65536 keys, 8 heads of 128, 2.15 GB, 365 us,
-// 5.9 TB/s; 32 of 256 to 20000 keys through a window of 4096, 389 MB, 83 us, 4.7 TB/s, where the beginnings of
+// What bounds it: reading the visible K and V once: 4 sequences of 65536 keys, 8 heads of 128, 2.15 GB, 369 us,
+// 5.8 TB/s; 32 of up to 16384 keys through a window of 4096, 389 MB, 84 us, 4.6 TB/s, where the beginnings of
 // 256 lists count.  As in sdpa_decode.hip:
 //   * Rows: token t, query head hk * group + g of a key/value head is row t * group + g (tokens outermost,
 //     so that the rows of a block stand close together and share the ends of their windows), taken 16 or 32

@@ -2,7 +2,7 @@
 // them, large trees of drafts (paged.h says which keys a row sees).  8 <= D <= 128.
 //
 // What bounds it: the matrix cores at the clock that the power limit leaves them: a 16384-token prompt, window
-// 4096, 32 heads on 8, D 128, 4.55 ms, 212 TFLOP/s of f32 products, matrix cores busy 61% of the cycles at 1.92
+// 4096, 32 heads on 8, D 128, 4.56 ms, 211 TFLOP/s of f32 products, matrix cores busy 61% of the cycles at 1.92
 // GHz.  A list's beginning and end cost about 16 us, most of the time of a list of six blocks.
 //
 // Both products on the bf16 matrix cores, three exact bf16 parts per f32 and six part products

@@ -3,7 +3,7 @@
 //
 // At these widths the bf16 parts of q, K and V leave no room in registers and LDS for two wavefronts a SIMD
 // (sdpa_paged_tile.hip), so the products are f32 ones, v_mfma_f32_16x16x4_f32, whose rate bounds it: a prompt of
-// 4096 tokens, 32 heads on 8, D 256, 2.38 ms, 115 TFLOP/s, 73% of the instruction's peak (D 192 1.75 ms); 9.4 and
+// 4096 tokens, 32 heads on 8, D 256, 2.37 ms, 116 TFLOP/s, 74% of the instruction's peak (D 192 1.75 ms); 9.4 and
 // 4.9 ms with the 16-row kernel, which reads K and V from L2 for every 16 rows.
 //   * A workgroup = eight wavefronts of 16 rows of one key/value head (token t, query head hk * group + g is
 //     row t * group + g); q and O stay in registers, D / 4 floats a lane each.  K and V in blocks of 32 keys
@@ -12,8 +12,9 @@
 //   * S^T = K Q^T, chains sb = 0, 1 of 16 keys: lane (g = l / 16, i = l % 16) holds K[16 sb + i][16 x + 4 g ..
 //     + 3] and q[row i] alike; value r of the result is key 16 sb + 4 g + r of row i.  O^T += V^T P^T: step
 //     (sb, r) contracts that key; the lane holds V[key][4 (i + 16 h) .. + 3], component e feeding O block
-//     4 h + e, whose value r' is d = 4 (4 g + r' + 16 h) + e.  All reads of LDS are 128 bits without conflicts
-//     (a row of K is 4 floats longer), each feeding four matrix instructions.
+//     4 h + e, whose value r' is d = 4 (4 g + r' + 16 h) + e.  All reads of LDS are 128 bits (a row of
+//     K is 4 floats longer against bank conflicts, which are a quarter of LDS's busy cycles, and those are a sixth
+//     of the kernel's), each feeding four matrix instructions.
 //   * Online softmax with a lazily moved reference maximum; a wavefront passes over blocks that none of its
 //     rows sees.  Lists of blocks, shares and their joining as in the other two kernels.
 //   * Columns in fours; one that would reach past D is the row's last one, with the columns that the four
