@@ -12,6 +12,7 @@ from . import ipc, linalg, nn
 from .kv_cache import KvCache, KvStep
 from .linalg import F64Buffer, GemmCachedF64, GemmF64
 from .nn import Activation, fused_mlp
+from .rotary import Rotary, RotaryPositions, rotary_freqs
 from .session import AttentionDims, SessionTensor, TensorSession
 from .tensor import (GELU, Attention, BatchMatMul, CausalAttention, FlashAttention, GroupedQueryAttention,
                      HipDevice, LayerNorm, LcgStream, MatMul, MatmulTiled, MultiHeadAttention, ReLU,
@@ -25,5 +26,5 @@ __all__ = [
     "Attention", "BatchMatMul", "CausalAttention", "FlashAttention", "GroupedQueryAttention", "HipDevice",
     "MatMul", "MultiHeadAttention",
     "MatmulTiled", "ScaledDotProductAttention", "SlidingWindowAttention", "Softmax", "Tensor", "get_device", "LcgStream",
-    "ReLU", "GELU", "LayerNorm", "KvCache", "KvStep",
+    "ReLU", "GELU", "LayerNorm", "KvCache", "KvStep", "Rotary", "RotaryPositions", "rotary_freqs",
 ]

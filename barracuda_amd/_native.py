@@ -52,6 +52,11 @@ class KvBatch(C.Structure):
     _fields_ = [("B", _i), ("total", _i), ("max_new", _i), ("max_len", _i), ("start", _vp), ("len", _vp)]
 
 
+class Rotary(C.Structure):
+    """bch_rotary_plan: which columns are turned, and by what a position; freq is a device address."""
+    _fields_ = [("dim", _i), ("interleaved", _i), ("scale", _f), ("freq", _vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "bch_device_count": (_i, [C.POINTER(_i)]),
@@ -96,6 +101,9 @@ SIGNATURES = {
     "bch_kv_append": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, AttnLayout, _vp, AttnLayout]),
     "bch_kv_copy_pages": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, C.POINTER(_i), C.POINTER(_i)]),
     "bch_kv_keep": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, _i, _vp, _vp, _vp]),
+    "bch_rotary": (_i, [_vp, _i, _i, _i, _i, C.POINTER(Rotary), _i, _ll, _vp, _vp, AttnLayout, _vp, AttnLayout]),
+    "bch_kv_append_rotary": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, C.POINTER(Rotary), _i, _vp, AttnLayout,
+                                  _vp, AttnLayout, _vp, AttnLayout, _vp, AttnLayout]),
     "bch_launch_code_object": (_i, [_vp, _vp, _sz, C.c_char_p, C.POINTER(C.c_uint),
                                     C.POINTER(C.c_uint), C.POINTER(_vp), _sz, _sz]),
     "bch_event_create": (_i, [_vp, C.POINTER(_vp)]),

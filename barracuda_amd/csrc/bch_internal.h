@@ -292,6 +292,19 @@ long long row_launches(long long rows);
 hipError_t launch_head_permute(hipStream_t s, bool concat, int B, int S, int H, int D, const float* in,
                                float* out);
 
+struct SdpaLayout;
+
+// Rotary positions (rotary.hip): the pairs of a row's first `dim` columns turned by position * freq[pair], backwards with
+// inverse, and multiplied by scale.
+struct RotaryPlan {
+  int dim, interleaved, inverse;
+  float scale;
+  const double* freq;
+};
+// Row i of [B][H][S][D] operands stands at positions[b * S + i], or without positions at first + i.
+hipError_t launch_rotary(hipStream_t s, int B, int H, int S, int D, const RotaryPlan& r, long long first,
+                         const int* positions, const float* x, const SdpaLayout& xl, float* o, const SdpaLayout& ol);
+
 // Device-to-device copy (16-byte path when aligned).
 hipError_t launch_copy(hipStream_t s, void* dst, const void* src, size_t bytes);
 

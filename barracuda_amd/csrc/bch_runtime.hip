@@ -1019,6 +1019,79 @@ bch_status bch_kv_append(bch_ctx* ctx, const bch_kv_pages* kv, const bch_kv_batc
                   "kv_append launch");
 }
 
+namespace {
+
+bch_status check_rotary(bch_ctx* ctx, const char* op, const bch_rotary_plan* r, int D) {
+  if (!r) return fail(ctx, BCH_E_INVALID, "%s: plan is NULL", op);
+  if (r->dim < 2 || r->dim % 2 != 0 || r->dim > D)
+    return fail(ctx, BCH_E_SHAPE, "%s: %d columns to turn of D = %d (needs an even number from 2 to D)", op, r->dim, D);
+  if (r->interleaved != 0 && r->interleaved != 1)
+    return fail(ctx, BCH_E_INVALID, "%s: interleaved must be 0 or 1 (got %d)", op, r->interleaved);
+  return BCH_OK;
+}
+
+}  // namespace
+
+bch_status bch_rotary(bch_ctx* ctx, int B, int H, int S, int D, const bch_rotary_plan* plan, int inverse,
+                      long long first, const int* positions, const float* x, bch_attn_layout xl, float* o,
+                      bch_attn_layout ol) {
+  const char* op = "rotary";
+  if (B < 0 || H < 0 || S < 0 || D < 1)
+    return fail(ctx, BCH_E_SHAPE, "%s: negative or empty dimension (B=%d, H=%d, S=%d, D=%d)", op, B, H, S, D);
+  bch_status st = check_rotary(ctx, op, plan, D);
+  if (st != BCH_OK) return st;
+  if (inverse != 0 && inverse != 1) return fail(ctx, BCH_E_INVALID, "%s: inverse must be 0 or 1 (got %d)", op, inverse);
+  st = check_layout(ctx, op, "x", xl, D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "o", ol, D);
+  if (st != BCH_OK) return st;
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (B == 0 || H == 0 || S == 0) return BCH_OK;
+  if (!x || !o || !plan->freq) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  if (x == o && (xl.batch_stride != ol.batch_stride || xl.head_stride != ol.head_stride || xl.row_stride != ol.row_stride))
+    return fail(ctx, BCH_E_INVALID, "%s: in place, x and o need the same layout", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  const bch::RotaryPlan r{plan->dim, plan->interleaved, inverse, plan->scale, plan->freq};
+  return from_hip(ctx, bch::launch_rotary(ctx->stream, B, H, S, D, r, first, positions, x, layout(xl), o, layout(ol)),
+                  "rotary launch");
+}
+
+bch_status bch_kv_append_rotary(bch_ctx* ctx, const bch_kv_pages* kv, const bch_kv_batch* batch, const int* parent,
+                                const bch_rotary_plan* plan, int H, const float* q, bch_attn_layout ql, float* o,
+                                bch_attn_layout ol, const float* k, bch_attn_layout kl, const float* v,
+                                bch_attn_layout vl) {
+  const char* op = "kv_append_rotary";
+  bch_status st = check_pages(ctx, op, kv, true);
+  if (st == BCH_OK) st = check_batch(ctx, op, batch);
+  if (st == BCH_OK) st = check_rotary(ctx, op, plan, kv->D);
+  if (st != BCH_OK) return st;
+  if (H < 0) return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (H=%d)", op, H);
+  if (H > 0) st = check_layout(ctx, op, "q", ql, kv->D);
+  if (H > 0 && st == BCH_OK) st = check_layout(ctx, op, "o", ol, kv->D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "new k", kl, kv->D);
+  if (st == BCH_OK) st = check_layout(ctx, op, "new v", vl, kv->D);
+  if (st != BCH_OK) return st;
+  if ((long long)H + 2LL * kv->Hkv > 0x7fffffff / 4)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d query and %d key/value heads", op, H, kv->Hkv);
+  const int max_new = std::min(batch->max_new, batch->total);
+  if (parent && max_new > bch::kMaxDrafts)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d drafts in one tree, at most %d", op, max_new, bch::kMaxDrafts);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (batch->B == 0 || max_new == 0) return BCH_OK;
+  if (!kv->k || !kv->v || !kv->table || !batch->start || !batch->len || !k || !v || !plan->freq || (H > 0 && (!q || !o)))
+    return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  if (H > 0 && q == o && (ql.head_stride != ol.head_stride || ql.row_stride != ol.row_stride))
+    return fail(ctx, BCH_E_INVALID, "%s: in place, q and o need the same layout", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  const bch::RotaryPlan r{plan->dim, plan->interleaved, 0, plan->scale, plan->freq};
+  return from_hip(ctx,
+                  bch::launch_kv_append_rotary(ctx->stream, pages_of(*kv), kv->k, kv->v, seqs_of(*batch), batch->B,
+                                               parent, r, H, kv->Hkv, kv->D, q, layout(ql), o, layout(ol), k,
+                                               layout(kl), v, layout(vl)),
+                  "kv_append_rotary launch");
+}
+
 bch_status bch_kv_copy_pages(bch_ctx* ctx, const bch_kv_pages* kv, int layers, long long k_layer_stride,
                              long long v_layer_stride, int n, const int* src, const int* dst) {
   const char* op = "kv_copy_pages";

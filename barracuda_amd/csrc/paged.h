@@ -448,6 +448,11 @@ hipError_t launch_sdpa_paged_rows(hipStream_t s, const PagedCall& c, const Share
 // ---- the cache's own calls (kv_pages.hip) ----
 hipError_t launch_kv_append(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B, int Hkv,
                             int D, const float* nk, const SdpaLayout& nkl, const float* nv, const SdpaLayout& nvl);
+// The same with rotary positions (rotary.hip): k turned on its way into the pages, and H heads of q turned into o.
+hipError_t launch_kv_append_rotary(hipStream_t s, const KvPages& kv, float* k, float* v, const KvSeqs& seqs, int B,
+                                   const int* parent, const RotaryPlan& r, int H, int Hkv, int D, const float* q,
+                                   const SdpaLayout& ql, float* o, const SdpaLayout& ol, const float* nk,
+                                   const SdpaLayout& nkl, const float* nv, const SdpaLayout& nvl);
 // Pages dst[x] = src[x], of `layers` layers; host arrays.
 hipError_t launch_kv_copy_pages(hipStream_t s, const KvPages& kv, float* k, float* v, int layers, long long k_layer,
                                 long long v_layer, int Hkv, int D, int n, const int* src, const int* dst);

@@ -16,7 +16,8 @@ per step and serves every layer.  A cache is for one thread at a time.
     a = cache.new_sequence()
     step = cache.batch([(a, 512)])                 # room for 512 new tokens
     for layer in range(layers):
-        cache.append(step, layer, k, v)            # [total, kv_heads, head_dim]
+        cache.append(step, layer, k, v)            # [total, kv_heads, head_dim]; or, with rotary positions,
+        # q = cache.append_rotary(step, layer, rotary, q, k, v)
         o = cache.attention(step, layer, q, window=4096, sinks=4)
     b = cache.fork(a)
     step = cache.batch([(a, 5), (b, 1)], parents=[[-1, 0, 0, 1, 1], [-1]])
@@ -214,6 +215,38 @@ class KvCache:
         with dev._lock:
             dev.check(dev._lib.bch_kv_append(dev.ctx, self._pages(step, layer), step._batch, C.c_void_p(k.ptr), row,
                                              C.c_void_p(v.ptr), row), "kv_append")
+
+    def append_rotary(self, step: KvStep, layer: int, rotary, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+        """append with the keys turned by their positions (a Rotary of head_dim),
+        and q [total, heads, head_dim] turned by the same: the result is for
+        attention.  A draft stands behind its parent.  Keys stay turned as they
+        were appended: after retain has closed them up, distances over the gap
+        are as before."""
+        self._check_step("KvCache.append_rotary", step, layer)
+        shape = [step.total, self.kv_heads, self.head_dim]
+        for t in (k, v):
+            if t.shape() != shape:
+                raise ShapeMismatch(shape, t.shape())
+        qs = q.shape()
+        if len(qs) != 3 or qs[0] != step.total or qs[2] != self.head_dim:
+            raise ShapeMismatch(shape, qs)
+        if rotary.head_dim != self.head_dim:
+            raise ShapeMismatch([self.head_dim], [rotary.head_dim])
+        self._own(q, k, v)
+        if rotary.device is not self.device:
+            raise DeviceError("tensors live on different devices")
+        out = Tensor.empty(qs, self.device)
+        if step.total == 0:
+            return out
+        heads = qs[1]
+        row = N.AttnLayout(0, self.head_dim, self.kv_heads * self.head_dim)
+        q_row = N.AttnLayout(0, self.head_dim, max(1, heads) * self.head_dim)
+        dev = self.device
+        with dev._lock:
+            dev.check(dev._lib.bch_kv_append_rotary(dev.ctx, self._pages(step, layer), step._batch, step._parents,
+                                                    rotary._plan, heads, C.c_void_p(q.ptr), q_row, C.c_void_p(out.ptr), q_row,
+                                                    C.c_void_p(k.ptr), row, C.c_void_p(v.ptr), row), "kv_append_rotary")
+        return out
 
     def attention(self, step: KvStep, layer: int, q: Tensor, window: int = 0, sinks: int = 0,
                   scale: float | None = None) -> Tensor:

@@ -302,6 +302,10 @@ class Tensor:
     def sliding_window_attention(self, key: "Tensor", value: "Tensor", window: int, sinks: int = 0) -> "Tensor":
         return SlidingWindowAttention(self, key, value, window, sinks).execute()
 
+    def rotary(self, rotary, first: int = 0, positions=None, inverse: bool = False, heads_last: bool = False) -> "Tensor":
+        from .rotary import RotaryPositions
+        return RotaryPositions(self, rotary, first, positions, inverse, heads_last).execute()
+
     def multi_head_attention(self, key: "Tensor", value: "Tensor", w_q: "Tensor", w_k: "Tensor",
                              w_v: "Tensor", w_o: "Tensor", num_heads: int) -> "Tensor":
         return MultiHeadAttention(self, key, value, w_q, w_k, w_v, w_o, num_heads).execute()

@@ -466,6 +466,49 @@ bch_status bch_kv_keep(bch_ctx *ctx, const bch_kv_pages *kv, int layers,
                        int B, int total, const int *start, const int *keep,
                        const int *to);
 
+/* ---- rotary positions ----
+ * The reference's attention has none; these stand beside it and beside the
+ * cache's append. */
+
+/* How a head's columns are turned: of its first `dim` columns (even, 2 .. D)
+ * the pair i < dim/2 is columns i and i + dim/2, or with interleaved = 1
+ * columns 2i and 2i + 1.  At position p a pair (a, b) becomes
+ *   scale (a cos t - b sin t), scale (a sin t + b cos t),  t = p freq[i];
+ * columns from dim on stay.  freq [dim/2], radians a position, is device
+ * memory.  Angles are products in 64 bits. */
+typedef struct bch_rotary_plan {
+  int dim;
+  int interleaved;
+  float scale;
+  const double *freq;
+} bch_rotary_plan;
+
+/* o = x turned; layouts as bch_sdpa_fwd_ex.  Row i of batch b stands at position
+ * positions[b*S + i] (device, [B][S]), or with positions NULL at first + i.
+ * inverse = 1 turns by -t: what the gradient of o gives for x.  o may be x (the same
+ * layout); they must not overlap otherwise.  B, H or S of 0: nothing happens. */
+bch_status bch_rotary(bch_ctx *ctx, int B, int H, int S, int D,
+                      const bch_rotary_plan *plan, int inverse, long long first,
+                      const int *positions, const float *x,
+                      bch_attn_layout x_layout, float *o,
+                      bch_attn_layout o_layout);
+
+/* bch_kv_append with the keys turned on their way into the pages, and H heads of
+ * the new tokens' q turned into o (row r, head h at r*row_stride + h*head_stride;
+ * o may be q).  Row i of sequence b's n new tokens stands at position len[b]-n+i, or with
+ * `parent` (as bch_sdpa_paged) behind its parent: where bch_sdpa_paged puts it.
+ * Its key's place in the pages is that of the len[b]-n+i'th, as for
+ * bch_kv_append; keys of pages that are not held, and keys before the
+ * sequence's beginning, are not written (q is turned all the same).  H of 0: q and o
+ * are not looked at.  A tree has at most 128 drafts a sequence. */
+bch_status bch_kv_append_rotary(bch_ctx *ctx, const bch_kv_pages *kv,
+                                const bch_kv_batch *batch, const int *parent,
+                                const bch_rotary_plan *plan, int H,
+                                const float *q, bch_attn_layout q_layout,
+                                float *o, bch_attn_layout o_layout,
+                                const float *k, bch_attn_layout k_layout,
+                                const float *v, bch_attn_layout v_layout);
+
 /* ---- seeded synthetic inputs, generated in HBM ---- */
 
 /* Fill dst[0..n) from the reference's seeded generators: uniform [lo, hi)
