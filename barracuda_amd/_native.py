@@ -57,6 +57,11 @@ class Rotary(C.Structure):
     _fields_ = [("dim", _i), ("interleaved", _i), ("scale", _f), ("freq", _vp)]
 
 
+class W4(C.Structure):
+    """bch_w4: the packed 4-bit weights of a linear layer; data is a device address."""
+    _fields_ = [("n", _i), ("k", _i), ("group", _i), ("data", _vp)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "bch_device_count": (_i, [C.POINTER(_i)]),
@@ -101,6 +106,9 @@ SIGNATURES = {
     "bch_kv_append": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, AttnLayout, _vp, AttnLayout]),
     "bch_kv_copy_pages": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, C.POINTER(_i), C.POINTER(_i)]),
     "bch_kv_keep": (_i, [_vp, C.POINTER(KvPages), _i, _ll, _ll, _i, _i, _vp, _vp, _vp]),
+    "bch_w4_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),
+    "bch_w4_pack": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp]),
+    "bch_w4_linear": (_i, [_vp, _i, C.POINTER(W4), _vp, _i, _vp, _i, _vp, _i]),
     "bch_rotary": (_i, [_vp, _i, _i, _i, _i, C.POINTER(Rotary), _i, _ll, _vp, _vp, AttnLayout, _vp, AttnLayout]),
     "bch_kv_append_rotary": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, C.POINTER(Rotary), _i, _vp, AttnLayout,
                                   _vp, AttnLayout, _vp, AttnLayout, _vp, AttnLayout]),

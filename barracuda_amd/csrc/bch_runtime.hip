@@ -28,6 +28,7 @@
 #include "../../include/barracuda_hip.h"
 #include "bch_internal.h"
 #include "paged.h"
+#include "w4.h"
 
 // Fixed scratch of bch_sgemm_noalloc (no hipMalloc on that path): the
 // skinny GEMM's split-k partials.  Each device that loads the library holds
@@ -1148,6 +1149,68 @@ bch_status bch_kv_keep(bch_ctx* ctx, const bch_kv_pages* kv, int layers, long lo
                   bch::launch_kv_keep(ctx->stream, pages_of(*kv), kv->k, kv->v, layers, k_layer_stride, v_layer_stride,
                                       kv->Hkv, kv->D, B, total, start, keep, to),
                   "kv_keep launch");
+}
+
+namespace {
+
+// Outputs whose 16-row tiles a kernel's grid can number, and inputs whose blocks' first numbers fit 32 bits.
+constexpr int kW4MaxN = 1 << 27, kW4MaxK = 0x7fffff00;
+
+bch_status check_w4(bch_ctx* ctx, const char* op, int n, int k, int group) {
+  if (n < 1 || k < 1 || group < 1)
+    return fail(ctx, BCH_E_SHAPE, "%s: empty dimension (n=%d, k=%d, group=%d)", op, n, k, group);
+  if (group % 32 != 0) return fail(ctx, BCH_E_INVALID, "%s: groups of %d inputs (needs a multiple of 32)", op, group);
+  if (n > kW4MaxN || k > kW4MaxK)
+    return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d outputs (at most %d) of %d inputs (at most %d)", op, n, kW4MaxN, k, kW4MaxK);
+  return BCH_OK;
+}
+
+}  // namespace
+
+bch_status bch_w4_bytes(int n, int k, int group, size_t* bytes) {
+  if (!bytes) return fail(nullptr, BCH_E_INVALID, "w4_bytes: bytes is NULL");
+  bch_status st = check_w4(nullptr, "w4_bytes", n, k, group);
+  if (st == BCH_OK) *bytes = bch::w4_bytes(n, k, group);
+  return st;
+}
+
+bch_status bch_w4_pack(bch_ctx* ctx, int n, int k, int group, const unsigned char* codes, int ld, const float* scale,
+                       const unsigned char* zero, void* out) {
+  const char* op = "w4_pack";
+  bch_status st = check_w4(ctx, op, n, k, group);
+  if (st != BCH_OK) return st;
+  if (ld < (k - 1) / 2 + 1) return fail(ctx, BCH_E_SHAPE, "%s: rows of %d bytes for %d codes", op, ld, k);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (!codes || !scale || !out) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  if (reinterpret_cast<uintptr_t>(out) & 15) return fail(ctx, BCH_E_INVALID, "%s: out must be 16-byte aligned", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx, bch::launch_w4_pack(ctx->stream, bch::w4_of(n, k, group, out), codes, ld, scale, zero, out),
+                  "w4_pack launch");
+}
+
+bch_status bch_w4_linear(bch_ctx* ctx, int m, const bch_w4* w, const float* x, int ldx, const float* bias, int act,
+                         float* y, int ldy) {
+  const char* op = "linear4";
+  if (!w) return fail(ctx, BCH_E_INVALID, "%s: weights are NULL", op);
+  bch_status st = check_w4(ctx, op, w->n, w->k, w->group);
+  if (st != BCH_OK) return st;
+  if (act != BCH_ACT_NONE && act != BCH_ACT_RELU && act != BCH_ACT_GELU)
+    return fail(ctx, BCH_E_INVALID, "%s: unknown activation %d", op, act);
+  if (m < 0) return fail(ctx, BCH_E_SHAPE, "%s: negative dimension (m=%d)", op, m);
+  if (ldx < w->k || ldy < w->n)
+    return fail(ctx, BCH_E_SHAPE, "%s: leading dimension too small (ldx=%d k=%d, ldy=%d n=%d)", op, ldx, w->k, ldy, w->n);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (m == 0) return BCH_OK;
+  if (!w->data || !x || !y) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  if (reinterpret_cast<uintptr_t>(w->data) & 15) return fail(ctx, BCH_E_INVALID, "%s: weights must be 16-byte aligned", op);
+  st = use(ctx);
+  if (st != BCH_OK) return st;
+  const bch::W4 v = bch::w4_of(w->n, w->k, w->group, w->data);
+  st = size_ws(ctx, bch::w4_linear_workspace_bytes(m, v), 0);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx, bch::launch_w4_linear(ctx->stream, m, v, x, ldx, bias, act, y, ldy, ctx->ws, ctx->ws_bytes),
+                  "linear4 launch");
 }
 
 bch_status bch_fill_uniform(bch_ctx* ctx, float* dst, size_t n, unsigned long long* state, double lo,

@@ -203,6 +203,40 @@ bch_status bch_sgemm_ex(bch_ctx *ctx, int transb, int m, int n, int k,
                         const float *A, int lda, const float *B, int ldb,
                         const float *bias, int act, float *C, int ldc);
 
+/* ---- linear layers with 4-bit weights ----
+ * The reference's linear layer (shaders/misc/linear_f64.wgsl) has f32 weights;
+ * this stands beside bch_sgemm_ex for layers whose weights are most of what a
+ * step reads.  A weight is
+ *   W[o][i] = scale[o][i / group] * (code[o][i] - zero[o][i / group]),
+ * code and zero whole numbers 0 .. 15, group a multiple of 32 (one that is k or
+ * more: a scale an output). */
+
+/* The packed weights of a layer with k inputs and n outputs take *bytes. */
+bch_status bch_w4_bytes(int n, int k, int group, size_t *bytes);
+
+/* Weights laid out once for bch_w4_linear, all in device memory: codes [n][ld
+ * bytes], two inputs a byte, the even one in the low half; scale and zero (a
+ * byte each; NULL: 8 everywhere) [n][ceil(k / group)]; out bch_w4_bytes, 16-byte aligned.
+ * n <= 2^27. */
+bch_status bch_w4_pack(bch_ctx *ctx, int n, int k, int group,
+                       const unsigned char *codes, int ld, const float *scale,
+                       const unsigned char *zero, void *out);
+
+typedef struct bch_w4 {
+  int n;
+  int k;
+  int group;
+  const void *data; /* what bch_w4_pack wrote */
+} bch_w4;
+
+/* y[m,n] = act(x[m,k] W^T + bias), x and y f32 row-major (ldx >= k, ldy >= n),
+ * bias nullable, act as bch_sgemm_ex; y must not overlap the others.  Sums are f32.  A code that is
+ * its zero point contributes nothing (0 * infinity: NaN, as in f32). 
+ */
+bch_status bch_w4_linear(bch_ctx *ctx, int m, const bch_w4 *w, const float *x,
+                         int ldx, const float *bias, int act, float *y,
+                         int ldy);
+
 /* C[b] = A[b] . B[b] for b < batch; A[b] starts at A + b*strideA (elements),
  * leading dimensions k, n, n.  Replaces BatchMatMul::execute
  * (ops/batch_matmul.rs:47-144, kernel K5 batch_matmul_f64.wgsl). */
