@@ -13,6 +13,7 @@ from .kv_cache import KvCache, KvStep
 from .linalg import F64Buffer, GemmCachedF64, GemmF64
 from .nn import Activation, fused_mlp
 from .rotary import Rotary, RotaryPositions, rotary_freqs
+from .sampling import Sample, Sampled, Sampling
 from .session import AttentionDims, SessionTensor, TensorSession
 from .tensor import (GELU, Attention, BatchMatMul, CausalAttention, FlashAttention, GroupedQueryAttention,
                      HipDevice, LayerNorm, LcgStream, MatMul, MatmulTiled, MultiHeadAttention, ReLU,
@@ -27,4 +28,5 @@ __all__ = [
     "MatMul", "MultiHeadAttention",
     "MatmulTiled", "ScaledDotProductAttention", "SlidingWindowAttention", "Softmax", "Tensor", "get_device", "LcgStream",
     "ReLU", "GELU", "LayerNorm", "KvCache", "KvStep", "Rotary", "RotaryPositions", "rotary_freqs",
+    "Sample", "Sampled", "Sampling",
 ]

@@ -62,6 +62,11 @@ class W4(C.Structure):
     _fields_ = [("n", _i), ("k", _i), ("group", _i), ("data", _vp)]
 
 
+class Sampling(C.Structure):
+    """bch_sampling: how a token is chosen from a row of logits."""
+    _fields_ = [("temperature", _f), ("top_k", _i), ("top_p", _f), ("min_p", _f)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "bch_device_count": (_i, [C.POINTER(_i)]),
@@ -109,6 +114,7 @@ SIGNATURES = {
     "bch_w4_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),
     "bch_w4_pack": (_i, [_vp, _i, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "bch_w4_linear": (_i, [_vp, _i, C.POINTER(W4), _vp, _i, _vp, _i, _vp, _i]),
+    "bch_sample": (_i, [_vp, _i, _i, _vp, _ll, C.POINTER(Sampling), _vp, _vp, _vp, _vp]),
     "bch_rotary": (_i, [_vp, _i, _i, _i, _i, C.POINTER(Rotary), _i, _ll, _vp, _vp, AttnLayout, _vp, AttnLayout]),
     "bch_kv_append_rotary": (_i, [_vp, C.POINTER(KvPages), C.POINTER(KvBatch), _vp, C.POINTER(Rotary), _i, _vp, AttnLayout,
                                   _vp, AttnLayout, _vp, AttnLayout, _vp, AttnLayout]),

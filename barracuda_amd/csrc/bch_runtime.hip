@@ -28,6 +28,7 @@
 #include "../../include/barracuda_hip.h"
 #include "bch_internal.h"
 #include "paged.h"
+#include "sample.h"
 #include "w4.h"
 
 // Fixed scratch of bch_sgemm_noalloc (no hipMalloc on that path): the
@@ -1211,6 +1212,41 @@ bch_status bch_w4_linear(bch_ctx* ctx, int m, const bch_w4* w, const float* x, i
   if (st != BCH_OK) return st;
   return from_hip(ctx, bch::launch_w4_linear(ctx->stream, m, v, x, ldx, bias, act, y, ldy, ctx->ws, ctx->ws_bytes),
                   "linear4 launch");
+}
+
+static_assert(sizeof(bch_sampling) == sizeof(bch::SampleRule), "a row's rule in device memory");
+
+bch_status bch_sample(bch_ctx* ctx, int rows, int vocab, const float* logits, long long row_stride,
+                      const bch_sampling* rule, const bch_sampling* row_rules, const float* u, int* tokens,
+                      float* probs) {
+  const char* op = "sample";
+  if (rows < 0 || vocab < 1) return fail(ctx, BCH_E_SHAPE, "%s: negative or empty dimension (rows=%d, vocab=%d)", op, rows, vocab);
+  if (row_stride < vocab) return fail(ctx, BCH_E_SHAPE, "%s: rows %lld apart of %d logits", op, row_stride, vocab);
+  if (vocab > 0x7ffff000) return fail(ctx, BCH_E_UNSUPPORTED, "%s: %d logits a row, at most %d", op, vocab, 0x7ffff000);
+  if (!rule && !row_rules) return fail(ctx, BCH_E_INVALID, "%s: rule is NULL", op);
+  if (!row_rules && !(rule->temperature >= 0.0f && rule->top_k >= 0 && rule->top_p >= 0.0f && rule->top_p <= 1.0f &&
+                      rule->min_p >= 0.0f && rule->min_p <= 1.0f))
+    return fail(ctx, BCH_E_INVALID,
+                "%s: temperature (%g) and top_k (%d) must not be negative, top_p (%g) and min_p (%g) from 0 to 1", op,
+                rule->temperature, rule->top_k, rule->top_p, rule->min_p);
+  if (!ctx) return fail(ctx, BCH_E_INVALID, "%s: ctx is NULL", op);
+  if (rows == 0) return BCH_OK;
+  if (!logits || !u || !tokens) return fail(ctx, BCH_E_INVALID, "%s: NULL buffer", op);
+  bch_status st = use(ctx);
+  if (st != BCH_OK) return st;
+  bch::SampleCall c{};
+  c.vocab = vocab;
+  c.unit_log = bch::sample_unit_log(vocab);
+  c.stride = row_stride;
+  if (!row_rules) c.rule = {rule->temperature, rule->top_k, rule->top_p, rule->min_p};
+  c.rules = reinterpret_cast<const bch::SampleRule*>(row_rules);
+  c.logits = logits;
+  c.u = u;
+  c.tokens = tokens;
+  c.probs = probs;
+  st = size_ws(ctx, bch::sample_workspace_bytes(c), 0);
+  if (st != BCH_OK) return st;
+  return from_hip(ctx, bch::launch_sample(ctx->stream, c, rows, ctx->ws, ctx->ws_bytes), "sample launch");
 }
 
 bch_status bch_fill_uniform(bch_ctx* ctx, float* dst, size_t n, unsigned long long* state, double lo,

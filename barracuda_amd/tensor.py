@@ -306,6 +306,10 @@ class Tensor:
         from .rotary import RotaryPositions
         return RotaryPositions(self, rotary, first, positions, inverse, heads_last).execute()
 
+    def sample(self, u, rule=None):
+        from .sampling import Sample, Sampling
+        return Sample(self, u, Sampling() if rule is None else rule).execute()
+
     def multi_head_attention(self, key: "Tensor", value: "Tensor", w_q: "Tensor", w_k: "Tensor",
                              w_v: "Tensor", w_o: "Tensor", num_heads: int) -> "Tensor":
         return MultiHeadAttention(self, key, value, w_q, w_k, w_v, w_o, num_heads).execute()

@@ -543,6 +543,37 @@ bch_status bch_kv_append_rotary(bch_ctx *ctx, const bch_kv_pages *kv,
                                 const float *k, bch_attn_layout k_layout,
                                 const float *v, bch_attn_layout v_layout);
 
+/* ---- sampling ----
+ * The reference ends at the softmax (ops/softmax.rs); this chooses tokens from
+ * the logits. */
+
+/* With m a row's largest logit a token weighs w = exp((x - m) / temperature).  In
+ * the order of descending logits, equal ones by ascending index: top_k leaves the
+ * first k (0: all), top_p of these the shortest beginning that holds that part
+ * of their weight (1: all; 0: the first), min_p of these the ones with w >= min_p.
+ * Temperature 0 leaves the first alone. */
+typedef struct bch_sampling {
+  float temperature;
+  int top_k;
+  float top_p;
+  float min_p;
+} bch_sampling;
+
+/* tokens[r] (device, [rows]) = of what the rule leaves of row r of logits
+ * (row_stride >= vocab floats apart) the first token in index order whose cumulative
+ * weight exceeds u[r] times the whole; u (device, [rows]) are numbers from 0 to below 1 (below 0 and NaN
+ * count as 0, from 1 on the last token is taken).  probs (device, [rows], nullable): its share of
+ * that weight.  `rule` (host) is every row's, or with row_rules (device, [rows], read when
+ * the kernels run) each row has its own; there what is out of range is taken as the nearest that is in it, and
+ * NaN as 0 for a temperature or min_p, as 1 for a top_p.  NaN logits count as -inf, which is never chosen;
+ * a row of nothing else gives token -1, probability 0.  Tokens of +inf share all weight.  Weights are added up as whole numbers of 2^-U, U =
+ * min(51, 62 - bits of vocab), to which they are rounded (44 for 131072 tokens): the same logits give the same
+ * token whatever else is in the batch. */
+bch_status bch_sample(bch_ctx *ctx, int rows, int vocab, const float *logits,
+                      long long row_stride, const bch_sampling *rule,
+                      const bch_sampling *row_rules, const float *u, int *tokens,
+                      float *probs);
+
 /* ---- seeded synthetic inputs, generated in HBM ---- */
 
 /* Fill dst[0..n) from the reference's seeded generators: uniform [lo, hi)
