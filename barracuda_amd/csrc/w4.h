@@ -49,4 +49,10 @@ hipError_t launch_w4_linear(hipStream_t s, int m, const W4& w, const float* x, l
                             float* y, long long ldy, void* ws, size_t ws_bytes);
 size_t w4_linear_workspace_bytes(int m, const W4& w);
 
+
+// More rows, on the matrix cores (w4_tile.hip): ws holds w4_parts_bytes(m, w).
+size_t w4_parts_bytes(int m, const W4& w);
+hipError_t launch_w4_tile(hipStream_t s, int m, const W4& w, const float* x, long long ldx, const float* bias, int act,
+                          float* y, long long ldy, void* ws);
+
 }  // namespace bch

@@ -129,10 +129,32 @@ hipError_t launch_w4_pack(hipStream_t s, const W4& w, const unsigned char* codes
   return hipGetLastError();
 }
 
-size_t w4_linear_workspace_bytes(int m, const W4& w) { return 0; }
+// Rows from which the matrix cores' tiles are taken.
+constexpr int kTileFrom = 64;
+// Scratch of a call: the parts of its rows, or of as many as take this much.
+constexpr size_t kPartsMost = (size_t)256 << 20;
+
+// The rows whose parts ws_bytes hold, in whole tiles of 128 where that is not all of them.
+int rows_in(int m, const W4& w, size_t ws_bytes) {
+  if (w4_parts_bytes(m, w) <= ws_bytes) return m;
+  const long long fit = (long long)(ws_bytes / (w4_parts_bytes(128, w) / 128 + 1)) / 128 * 128;
+  return (int)std::min<long long>(fit, m);
+}
+
+size_t w4_linear_workspace_bytes(int m, const W4& w) {
+  if (m < kTileFrom) return 0;
+  return std::min(w4_parts_bytes(m, w), std::max(kPartsMost, 2 * w4_parts_bytes(128, w)));
+}
 
 hipError_t launch_w4_linear(hipStream_t s, int m, const W4& w, const float* x, long long ldx, const float* bias, int act,
                             float* y, long long ldy, void* ws, size_t ws_bytes) {
+  const int fit = m < kTileFrom ? 0 : rows_in(m, w, ws_bytes);
+  if (fit > 0) {
+    for (int at = 0; at < m; at += fit) {
+      const hipError_t e = launch_w4_tile(s, std::min(fit, m - at), w, x + at * ldx, ldx, bias, act, y + at * ldy, ldy, ws);
+      if (e != hipSuccess || m - at <= fit) return e;
+    }
+  }
   const bool vec = w.k % 4 == 0 && ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
   const int mt = m >= 8 ? 8 : m >= 4 ? 4 : m >= 2 ? 2 : 1;
   const long long per = (1LL << 23) / w.tiles * mt;  // rows a launch
