@@ -40,7 +40,7 @@ SOURCES = ["bch_runtime.hip", "softmax_rows.hip", "sgemm_mfma.hip",
            "sgemm_reserve.hip", "sgemm_skinny.hip", "sdpa_fwd.hip", "sdpa_decode.hip", "sdpa_wide.hip", "dgemm_mfma.hip",
            "rng_fill.hip", "copy.hip", "elementwise.hip", "layer_norm.hip", "head_permute.hip",
            "softmax_f64.hip", "sdpa_paged.hip", "sdpa_paged_rows.hip",
-           "sdpa_paged_tile.hip", "sdpa_paged_wide.hip", "kv_pages.hip", "rotary.hip", "w4_linear.hip", "w4_tile.hip", "sample.hip"]
+           "sdpa_paged_tile.hip", "sdpa_paged_wide.hip", "kv_pages.hip", "rotary.hip", "w4_linear.hip", "w4_skinny.hip", "w4_tile.hip", "sample.hip"]
 # Per-file code-generation flags.  The skinny GEMM keeps its MFMA
 # accumulators in VGPRs: with the default heuristics the compiler parks them
 # in AGPRs and copies them back and forth inside the k loop (measured: 716

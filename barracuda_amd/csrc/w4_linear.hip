@@ -48,69 +48,6 @@ __global__ __launch_bounds__(kThreads) void w4_pack_scales(W4 w, const float* __
   }
 }
 
-// ---- a few rows of x: f32 multiplications ----
-// A workgroup takes 16 outputs and MT rows; its wavefronts share the blocks of inputs.  A lane holds 32 codes of its output,
-// and its sums over a group's codes before they are scaled.
-template <int MT>
-__global__ __launch_bounds__(kThreads) void w4_rows_kernel(W4 w, int m, const float* __restrict__ x, long long ldx,
-                                                           bool vec, const float* __restrict__ bias, int act, float* y,
-                                                           long long ldy) {
-  __shared__ float part[4][MT][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, kb = lane >> 4;
-  const int tile = blockIdx.x % w.tiles;
-  const long long m0 = (long long)(blockIdx.x / w.tiles) * MT;
-  float acc[MT] = {};
-  for (int b = wave; b < w.blocks; b += 4) {
-    const bch::u32x4 c = w.codes[((long long)tile * w.blocks + b) * 64 + lane];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i0 = 128 * b + 32 * j + 8 * kb;
-      const long long g = (long long)tile * w.groups + (128 * b + 32 * j) / w.group;
-      const float s = w.scale[16 * g + r];
-      const int z = w.zero[16 * g + r];
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = (float)((int)((c[j] >> (4 * (e / 2 + 4 * (e % 2)))) & 15) - z);
-#pragma unroll
-      for (int u = 0; u < MT; ++u) {
-        const float* row = x + min(m0 + u, (long long)m - 1) * ldx;
-        float q[8];
-        if (vec) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float4 t = i0 + 4 * h < w.k ? *reinterpret_cast<const float4*>(row + i0 + 4 * h) : make_float4(0, 0, 0, 0);
-            q[4 * h] = t.x;
-            q[4 * h + 1] = t.y;
-            q[4 * h + 2] = t.z;
-            q[4 * h + 3] = t.w;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) q[e] = i0 + e < w.k ? row[i0 + e] : 0.0f;
-        }
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(v[e], q[e], sum);
-        acc[u] = fmaf(s, sum, acc[u]);
-      }
-    }
-  }
-#pragma unroll
-  for (int u = 0; u < MT; ++u) {
-    acc[u] += __shfl_xor(acc[u], 16);
-    acc[u] += __shfl_xor(acc[u], 32);
-    if (kb == 0) part[wave][u][r] = acc[u];
-  }
-  __syncthreads();
-  for (int t = threadIdx.x; t < 16 * MT; t += kThreads) {
-    const int u = t >> 4, rr = t & 15, o = 16 * tile + rr;
-    if (m0 + u >= m || o >= w.n) continue;
-    float sum = (part[0][u][rr] + part[1][u][rr]) + (part[2][u][rr] + part[3][u][rr]);
-    if (bias) sum += bias[o];
-    y[(m0 + u) * ldy + o] = bch::activate(sum, act);
-  }
-}
-
 }  // namespace
 
 namespace bch {
@@ -129,42 +66,57 @@ hipError_t launch_w4_pack(hipStream_t s, const W4& w, const unsigned char* codes
   return hipGetLastError();
 }
 
-// Rows from which the matrix cores' tiles are taken.
-constexpr int kTileFrom = 64;
-// Scratch of a call: the parts of its rows, or of as many as take this much.
-constexpr size_t kPartsMost = (size_t)256 << 20;
+namespace {
 
-// The rows whose parts ws_bytes hold, in whole tiles of 128 where that is not all of them.
-int rows_in(int m, const W4& w, size_t ws_bytes) {
-  if (w4_parts_bytes(m, w) <= ws_bytes) return m;
-  const long long fit = (long long)(ws_bytes / (w4_parts_bytes(128, w) / 128 + 1)) / 128 * 128;
-  return (int)std::min<long long>(fit, m);
+// Scratch that a call of many rows asks for at most; more rows go through it in turn.
+constexpr size_t kMostBytes = (size_t)256 << 20;
+
+// The rows that go together, and how: kernels for few rows as long as their models say that they are done earlier.
+struct Way {
+  int rows;
+  bool tile;
+  W4Plan plan;
+  size_t bytes;
+};
+Way way_of(int m, const W4& w, size_t most) {
+  const int cus = device_cu_count(), few = std::min(m, kW4Few);
+  for (const bool split : {true, false}) {
+    const W4Plan f = w4_skinny_plan(few, w, cus, split), t = m > kW4Few ? w4_tile_plan(m, w, cus, split) : W4Plan{};
+    if (m <= kW4Few || f.cost * ((m - 1) / few + 1) < t.cost) {
+      if (w4_skinny_bytes(few, w, f) <= most) return {few, false, f, w4_skinny_bytes(few, w, f)};
+    } else if (w4_tile_bytes(m, w, t) <= most) {
+      return {m, true, t, w4_tile_bytes(m, w, t)};
+    }
+  }
+  // as many rows as the scratch holds, in whole tiles where it holds one
+  int rows = (int)std::min<long long>(m, (long long)(most / (w4_parts_bytes(128, w) / 128 + 1)));
+  if (rows >= 128) {
+    rows = rows / 128 * 128;
+    return {rows, true, w4_tile_plan(rows, w, cus, false), w4_parts_bytes(rows, w)};
+  }
+  rows = std::min(rows / 8 * 8 - 8, kW4Few);
+  if (rows < 8) return {0, false, {}, 0};
+  const W4Plan p = w4_skinny_plan(rows, w, cus, false);
+  return w4_skinny_bytes(rows, w, p) <= most ? Way{rows, false, p, w4_skinny_bytes(rows, w, p)} : Way{0, false, {}, 0};
 }
 
-size_t w4_linear_workspace_bytes(int m, const W4& w) {
-  if (m < kTileFrom) return 0;
-  return std::min(w4_parts_bytes(m, w), std::max(kPartsMost, 2 * w4_parts_bytes(128, w)));
-}
+}  // namespace
+
+size_t w4_linear_workspace_bytes(int m, const W4& w) { return m <= 2 ? 0 : way_of(m, w, kMostBytes).bytes; }
 
 hipError_t launch_w4_linear(hipStream_t s, int m, const W4& w, const float* x, long long ldx, const float* bias, int act,
                             float* y, long long ldy, void* ws, size_t ws_bytes) {
-  const int fit = m < kTileFrom ? 0 : rows_in(m, w, ws_bytes);
-  if (fit > 0) {
-    for (int at = 0; at < m; at += fit) {
-      const hipError_t e = launch_w4_tile(s, std::min(fit, m - at), w, x + at * ldx, ldx, bias, act, y + at * ldy, ldy, ws);
-      if (e != hipSuccess || m - at <= fit) return e;
-    }
-  }
-  const bool vec = w.k % 4 == 0 && ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  const int mt = m >= 8 ? 8 : m >= 4 ? 4 : m >= 2 ? 2 : 1;
-  const long long per = (1LL << 23) / w.tiles * mt;  // rows a launch
-  for (long long at = 0; at < m; at += per) {
-    const int mm = (int)std::min<long long>(per, m - at);
-    const dim3 grid((unsigned)((long long)w.tiles * ((mm - 1) / mt + 1))), block(kThreads);
-    auto kern = mt == 8 ? w4_rows_kernel<8> : mt == 4 ? w4_rows_kernel<4> : mt == 2 ? w4_rows_kernel<2> : w4_rows_kernel<1>;
-    hipLaunchKernelGGL(kern, grid, block, 0, s, w, mm, x + at * ldx, ldx, vec, bias, act, y + at * ldy, ldy);
-    const hipError_t e = hipGetLastError();
+  for (int at = 0; at < m;) {
+    const int left = m - at;
+    const Way way = left <= 2 ? Way{0, false, {}, 0} : way_of(left, w, std::min(ws_bytes, kMostBytes));
+    const float* xs = x + at * ldx;
+    float* ys = y + at * ldy;
+    const int rows = way.rows > 0 ? std::min(left, way.rows) : std::min(left, 2);
+    const hipError_t e = way.rows == 0 ? launch_w4_line(s, rows, w, xs, ldx, bias, act, ys, ldy)
+                         : way.tile    ? launch_w4_tile(s, rows, w, xs, ldx, bias, act, ys, ldy, ws, way.plan)
+                                       : launch_w4_skinny(s, rows, w, xs, ldx, bias, act, ys, ldy, ws, way.plan);
     if (e != hipSuccess) return e;
+    at += rows;
   }
   return hipSuccess;
 }
