@@ -1244,7 +1244,7 @@ bch_status bch_sample(bch_ctx* ctx, int rows, int vocab, const float* logits, lo
   c.u = u;
   c.tokens = tokens;
   c.probs = probs;
-  st = size_ws(ctx, bch::sample_workspace_bytes(c), 0);
+  st = size_ws(ctx, bch::sample_workspace_bytes(c, rows), 0);
   if (st != BCH_OK) return st;
   return from_hip(ctx, bch::launch_sample(ctx->stream, c, rows, ctx->ws, ctx->ws_bytes), "sample launch");
 }

@@ -8,7 +8,9 @@
 //
 // Weights are whole numbers of 2^-U (2^-44 for 131072 tokens; 62 bits hold their sum): from 64-bit arithmetic, rounded once.  Sums of
 // them are exact, so neither the order in which threads add nor how a row is cut up changes a choice, and the
-// roundings move a border by 2^-45 of the largest weight a token.  What is below half of 2^-U is never drawn.
+// roundings move a border by 2^-45 of the largest weight a token.  What is below half of 2^-U is never drawn.  (The whole
+// weight of a row of which nothing but top_p, or nothing at all, leaves some is added up from spans of 512 logits, whole
+// numbers of 2^-51 of each span's largest: the same spans and order for every row of that length.)
 #include "sample.h"
 
 #include <algorithm>
@@ -64,10 +66,13 @@ __device__ __forceinline__ u64 units(const Scale& s, double w) {
 }
 
 // ---- sums over a workgroup ----
+// A workgroup goes through most of its code once, and much of its time is the fetching of that code.  So what a thread has several
+// of goes through loops in turn, with one copy of weight_of in each (16 rows of 50021 logits, 4900 of them finite, top_p 0.98: the
+// last step takes 25 us, and 48 with the loops unrolled and eight weights a thread in scratch memory).
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
 
 __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {  // inclusive
-#pragma unroll
+#pragma unroll 1
   for (int d = 1; d < 64; d *= 2) {
     const u64 o = __shfl_up(v, d);
     if (lane >= d) v += o;
@@ -75,48 +80,72 @@ __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {  // inclusive
   return v;
 }
 
+typedef u64 Sums[2][kWaves];
+
+// Exclusive sum of v over the threads, and the total.
+__device__ __forceinline__ u64 block_scan(Sums& sums, u64 v, u64& all) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const u64 in = wave_scan(v, lane);
+  __syncthreads();
+  if (lane == 63) sums[0][wave] = in;
+  __syncthreads();
+  u64 before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const u64 one = sums[0][w];
+    before += w < wave ? one : 0;
+    all += one;
+  }
+  return before + in - v;
+}
+
+// ---- rules ----
+
+__device__ __forceinline__ bool one_token(const SampleRule& rule) {
+  return !(rule.temperature > 0.0f) || rule.top_k == 1 || rule.top_p <= 0.0f;
+}
+__device__ __forceinline__ bool by_count(const SampleRule& rule, int vocab) { return rule.top_k > 0 && rule.top_k < vocab; }
+__device__ __forceinline__ bool by_weight(const SampleRule& rule) { return rule.top_p < 1.0f; }
+__device__ __forceinline__ Scale scale_of(const SampleCall& c, const SampleRule& rule, float m) {
+  return {m, 1.44269504088896340736 / (double)rule.temperature, rule.min_p > 0.0f ? fmin((double)rule.min_p, 1.0) : 0.0,
+          c.unit_log};
+}
+// The part of `whole` that u is.  NaN counts as 0.
+__device__ __forceinline__ double draw_at(const SampleCall& c, long long r, double whole) {
+  const double u = c.u[r];
+  return u > 0.0 ? fmin(u, 1.0) * whole : 0.0;
+}
+__device__ __forceinline__ u64 draw_units(const SampleCall& c, long long r, u64 whole) {
+  return min((u64)draw_at(c, r, (double)whole), whole - 1);
+}
+// The weight that top_p asks for of `of` units.
+__device__ __forceinline__ u64 part_units(const SampleRule& rule, double of) {
+  return max((u64)1, (u64)ceil((double)rule.top_p * of));
+}
+__device__ __forceinline__ void answer(const SampleCall& c, long long r, int token, double prob) {
+  c.tokens[r] = token;
+  if (c.probs) c.probs[r] = (float)prob;
+}
+
+// ---- a row by one workgroup, whatever its rule and its logits ----
 struct Cut {
   unsigned key;  // tokens above it stay,
   unsigned ties; // and of those on it the first so many
 };
 
-struct Shared {
+struct General {
   u64 weight[kBins];
   unsigned count[kBins];
-  u64 sums[2][kWaves];
   u64 found[4];
   int bin;
 };
-
-// Exclusive sums of a and b over the threads, and their totals.
-__device__ __forceinline__ void block_scan(Shared& s, u64& a, u64& b, u64& all_a, u64& all_b) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 ia = wave_scan(a, lane), ib = wave_scan(b, lane);
-  __syncthreads();
-  if (lane == 63) {
-    s.sums[0][wave] = ia;
-    s.sums[1][wave] = ib;
-  }
-  __syncthreads();
-  u64 ba = 0, bb = 0;
-  all_a = all_b = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) {
-      ba = all_a;
-      bb = all_b;
-    }
-    all_a += s.sums[0][w];
-    all_b += s.sums[1][w];
-  }
-  a = ba + ia - a;
-  b = bb + ib - b;
-}
 
 // The cut behind the shortest beginning of the order that holds `target` tokens (BY_COUNT), or units of weight: the key's digits
 // from the top, each by a histogram of the tokens that share the digits before it.  total: the weight of what the search is in; the
 // target is given for it by `aim`.  Returns the weight that the cut leaves.
 template <bool BY_COUNT, typename Aim>
-__device__ u64 find_cut(Shared& s, const float* row, int vocab, const Scale& sc, Aim aim, Cut& cut) {
+__device__ u64 find_cut(General& s, Sums& sums, const float* row, int vocab, const Scale& sc, Aim aim, Cut& cut) {
   unsigned prefix = 0;
   u64 target = 0, above_weight = 0, tie_weight = 0;
   constexpr int kShift[4] = {32, 21, 10, 0};
@@ -147,7 +176,8 @@ __device__ u64 find_cut(Shared& s, const float* row, int vocab, const Scale& sc,
       w += s.weight[b];
     }
     u64 all_c, all_w;
-    block_scan(s, c, w, all_c, all_w);
+    c = block_scan(sums, c, all_c);
+    w = block_scan(sums, w, all_w);
     if (level == 0) target = aim(all_w);
     for (int b = hi; b > hi - per; --b) {
       const u64 before = BY_COUNT ? c : w, in = BY_COUNT ? s.count[b] : s.weight[b];
@@ -172,42 +202,19 @@ __device__ u64 find_cut(Shared& s, const float* row, int vocab, const Scale& sc,
   return above_weight + cut.ties * tie_weight;
 }
 
-// ---- one workgroup a row ----
-__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c) {
-  __shared__ Shared s;
-  const long long r = blockIdx.x;
+// For a rule that leaves more than one token.
+__device__ void general_row(General& s, Sums& sums, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc) {
   const float* row = c.logits + r * c.stride;
-  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the largest logit, of equal ones the lowest index
-  u64 top = 0;
-  for (int i = threadIdx.x; i < c.vocab; i += kThreads)
-    top = max(top, (u64)key_of(clean(row[i])) << 32 | (0xffffffffu - (unsigned)i));
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) top = max(top, __shfl_xor(top, d));
-  if (lane == 0) s.sums[0][wave] = top;
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) top = max(top, s.sums[0][w]);
-  const unsigned top_key = (unsigned)(top >> 32);
-  const bool nothing = top_key == kNothing, one = !(rule.temperature > 0.0f) || rule.top_k == 1 || rule.top_p <= 0.0f;
-  if (nothing || one) {
-    if (threadIdx.x == 0) {
-      c.tokens[r] = nothing ? -1 : (int)(0xffffffffu - (unsigned)top);
-      if (c.probs) c.probs[r] = nothing ? 0.0f : 1.0f;
-    }
-    return;
-  }
-  const Scale sc{logit_of(top_key), 1.44269504088896340736 / (double)rule.temperature,
-                 rule.min_p > 0.0f ? fmin((double)rule.min_p, 1.0) : 0.0, c.unit_log};
   Cut cut{0, 0};
   u64 left = 0;
-  const bool by_count = rule.top_k > 0 && rule.top_k < c.vocab;
-  if (by_count) left = find_cut<true>(s, row, c.vocab, sc, [&](u64) { return (u64)rule.top_k; }, cut);
-  if (rule.top_p < 1.0f)
-    find_cut<false>(s, row, c.vocab, sc,
+  const bool count_cut = by_count(rule, c.vocab);
+  if (count_cut) left = find_cut<true>(s, sums, row, c.vocab, sc, [&](u64) { return (u64)rule.top_k; }, cut);
+  if (by_weight(rule))
+    find_cut<false>(s, sums, row, c.vocab, sc,
                     [&](u64 all) {
-                      const u64 of = by_count ? left : all;
-                      return min(of, max((u64)1, (u64)ceil((double)rule.top_p * (double)of)));
+                      const u64 of = count_cut ? left : all;
+                      return min(of, part_units(rule, (double)of));
                     },
                     cut);
   // the draw: the part of the row that the target falls into, sixteen times smaller each time
@@ -240,8 +247,8 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c) {
     }
     __syncthreads();
     if (lane == 0) {
-      s.sums[0][wave] = sum;
-      s.sums[1][wave] = on;
+      sums[0][wave] = sum;
+      sums[1][wave] = on;
     }
     __syncthreads();
     u64 part[kWaves];
@@ -250,17 +257,15 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c) {
     u64 all = 0;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
-      const unsigned n = (unsigned)s.sums[1][w];
+      const unsigned n = (unsigned)sums[1][w];
       const unsigned keep = cut.ties > before[w] ? min(n, cut.ties - before[w]) : 0;
       before[w + 1] = before[w] + n;
-      part[w] = s.sums[0][w] + keep * tie_weight;
+      part[w] = sums[0][w] + keep * tie_weight;
       all += part[w];
     }
     if (first) {
       whole = all;
-      const double u = c.u[r];  // NaN counts as 0
-      target = u > 0.0 ? (u64)(fmin(u, 1.0) * (double)whole) : 0;
-      target = min(target, whole - 1);
+      target = draw_units(c, r, whole);
     }
     int pick = 0;
     bool found = false;
@@ -297,10 +302,682 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c) {
     const u64 run = wave_scan(w, lane);
     const u64 beyond = __ballot(run > target);
     if (beyond && lane == __ffsll(beyond) - 1) {
-      c.tokens[r] = i;
-      if (c.probs) c.probs[r] = (float)((double)w / (double)whole);
+      answer(c, r, i, (double)w / (double)whole);
     }
   }
+}
+
+// ---- the same from the largest logits of every 512 ----
+// Most rules leave few tokens of many.  A wavefront takes 512 logits, read once: it notes its largest, what its weights add up to
+// against that (where the rule needs it), and a list of its largest: those from its lanes' R-th largest maximum on.  All of the
+// row's tokens from the largest such bound of any wavefront on (`tau`) then are on lists, and where the rule's cuts are found
+// among them, they alone decide.  Where they are not (flat rows with a top_p near 1, thousands of equal logits),
+// general_row does.
+constexpr int kSpan = 512, kListMost = 128, kSortMost = 2048;
+constexpr int kSpanUnit = 51;  // 512 weights in units of 2^-51 stay below 2^61
+
+struct Record {
+  unsigned top, tau;  // keys; tau 0xffffffff: the list is not whole
+  int count, first;   // of the list; the lowest index of the largest
+  u64 weight;
+};
+
+// How many of a wavefront's lanes are to hold a token from tau on: the largest of the wavefronts' bounds then leaves a good deal more
+// than top_k tokens of the row, or some hundreds.
+__device__ __forceinline__ int list_rank(const SampleRule& rule, int vocab, int spans) {
+  if (one_token(rule)) return 1;
+  if (by_count(rule, vocab)) return (int)min(48LL, 5 + (4LL * rule.top_k + spans - 1) / spans);
+  return min(32, max(8, 1024 / spans));
+}
+__device__ __forceinline__ bool needs_whole(const SampleRule& rule, int vocab) {
+  return !one_token(rule) && !by_count(rule, vocab) && (by_weight(rule) || !(rule.min_p > 0.0f));
+}
+
+// f of each of eight values, one copy of it.
+template <typename F>
+__device__ __forceinline__ void each(const float (&x)[8], F f) {
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = x[e];
+#pragma unroll 1
+  for (int n = 0; n < 8; ++n) {
+    f(y[0]);
+#pragma unroll
+    for (int e = 0; e < 7; ++e) y[e] = y[e + 1];
+  }
+}
+
+// Four logits from index i on, wherever they lie (16-byte loads need 4-byte alignment); -inf behind the last.
+__device__ __forceinline__ void load_four(const SampleCall& c, const float* row, int i, float* x) {
+  typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
+  if (i + 3 < c.vocab) {
+    const f32x4_any t = *reinterpret_cast<const f32x4_any*>(row + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = clean(t[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float t = row[min(i + e, c.vocab - 1)];
+      x[e] = i + e < c.vocab ? clean(t) : -INFINITY;
+    }
+  }
+}
+// The logits of a span: this lane's 4 lane .. + 3 and 256 + 4 lane .. + 3.
+__device__ __forceinline__ void load_span(const SampleCall& c, const float* row, int base, float (&x)[8]) {
+  const int lane = threadIdx.x & 63;
+  load_four(c, row, base + 4 * lane, x);
+  load_four(c, row, base + 256 + 4 * lane, x + 4);
+}
+__device__ __forceinline__ void load_eight(const SampleCall& c, const float* row, int i, float (&x)[8]) {
+  load_four(c, row, i, x);
+  load_four(c, row, i + 4, x + 4);
+}
+__device__ __forceinline__ int span_index(int base, int e) {
+  return base + 256 * (e / 4) + 4 * (int)(threadIdx.x & 63) + e % 4;
+}
+
+// Span `at` of a row, by one wavefront: its record, and its list (keys in the upper half, 2^32 - 1 - index in the lower).
+__device__ __forceinline__ void list_span(const SampleCall& c, const float* row, const SampleRule& rule, int spans, int at,
+                                          Record* record, u64* list) {
+  const int lane = threadIdx.x & 63, base = at * kSpan;
+  float x[8];
+  load_span(c, row, base, x);
+  unsigned key[8], mine = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    key[e] = key_of(x[e]);
+    mine = max(mine, key[e]);
+  }
+  const unsigned top = key_of(bch::wave_allreduce(logit_of(mine), bch::OpMax()));
+  int first = 0x7fffffff;
+  if (one_token(rule)) {
+#pragma unroll
+    for (int e = 7; e >= 0; --e)
+      if (key[e] == top) first = span_index(base, e);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d));
+  }
+  unsigned tau = top;
+  int count = 0;
+  if (!one_token(rule)) {
+    // the R-th largest of the lanes' maxima, bit by bit (the upper half of them: a little below it is as good)
+    const int rank = list_rank(rule, c.vocab, spans);
+    tau = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 16; --bit) {
+      const unsigned next = tau | 1u << bit;
+      if (__popcll(__ballot(mine >= next)) >= rank) tau = next;
+    }
+    tau = max(tau, kNothing + 1);  // -inf is never chosen
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const bool on = key[e] >= tau;
+      const u64 mask = __ballot(on);
+      const int slot = count + __popcll(mask & ((1ull << lane) - 1));
+      if (on && slot < kListMost) list[slot] = (u64)key[e] << 32 | (0xffffffffu - (unsigned)span_index(base, e));
+      count += __popcll(mask);
+    }
+  }
+  u64 sum = 0;
+  if (needs_whole(rule, c.vocab) && top != kNothing) {
+    Scale sc = scale_of(c, rule, logit_of(top));
+    sc.unit_log = kSpanUnit;
+    each(x, [&](float v) { sum += units(sc, weight_of(sc, v)); });
+#pragma unroll 1
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  }
+  if (lane == 0) *record = {top, count > kListMost ? 0xffffffffu : tau, min(count, kListMost), first, sum};
+}
+
+// Of lane ^ D, without LDS: rotations and mirrors within 16 lanes, exchanges of 16 and of 32.
+template <int D>
+__device__ __forceinline__ unsigned across(unsigned v) {
+  constexpr int kCtrl = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x128;
+  if constexpr (D == 16 || D == 32) {
+    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+    u32x2 o;
+    if constexpr (D == 16)
+      o = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(v, v, false, false));
+    else
+      o = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+    return threadIdx.x & D ? o[0] : o[1];
+  }
+  v = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, true);
+  if constexpr (D == 4) v = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x1B, 0xF, 0xF, true);  // (a mirror of 8, then of 4)
+  return v;
+}
+template <int D>
+__device__ __forceinline__ u64 across(u64 v) {
+  return (u64)across<D>((unsigned)(v >> 32)) << 32 | across<D>((unsigned)v);
+}
+// One step of a bitonic sort: the larger of a pair to the lower place where `down`.
+template <int D>
+__device__ __forceinline__ void step(u64& v, int i, bool down) {
+  const u64 o = across<D>(v);
+  const bool lower = (i & D) == 0;
+  v = (lower == down) == (v > o) ? v : o;
+}
+// a[0 .. n) descending, n a power of two from 64 to kSortMost.  A thread holds the entries t and t + kThreads; pairs of one
+// wavefront meet in registers, others in LDS.
+__device__ void sort_descending(u64* a, int n) {
+  __syncthreads();
+  const int t = threadIdx.x;
+  u64 v[2] = {t < n ? a[t] : 0, t + kThreads < n ? a[t + kThreads] : 0};
+  for (int k = 2; k <= n; k *= 2) {
+    for (int j = k / 2; j >= 64; j /= 2) {
+      if (j == kThreads) {
+        const u64 x = max(v[0], v[1]);
+        v[1] = min(v[0], v[1]);
+        v[0] = x;
+        continue;
+      }
+      __syncthreads();
+      if (t < n) a[t] = v[0];
+      if (t + kThreads < n) a[t + kThreads] = v[1];
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int i = t + e * kThreads;
+        if (i < n) {
+          const u64 o = a[i ^ j];
+          v[e] = (((i & j) == 0) == ((i & k) == 0)) == (v[e] > o) ? v[e] : o;
+        }
+      }
+    }
+    const int most = min(32, k / 2);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = t + e * kThreads;
+      if (i >= n) continue;  // (whole wavefronts)
+      const bool down = (i & k) == 0;
+      if (most >= 32) step<32>(v[e], i, down);
+      if (most >= 16) step<16>(v[e], i, down);
+      if (most >= 8) step<8>(v[e], i, down);
+      if (most >= 4) step<4>(v[e], i, down);
+      if (most >= 2) step<2>(v[e], i, down);
+      step<1>(v[e], i, down);
+    }
+  }
+  __syncthreads();
+  if (t < n) a[t] = v[0];
+  if (t + kThreads < n) a[t + kThreads] = v[1];
+  __syncthreads();
+}
+__device__ __forceinline__ int power_of_two(int n) { return n <= 64 ? 64 : 1 << (32 - __clz(n - 1)); }
+
+struct Lists {
+  u64 entry[kSortMost], weight[kSortMost];
+};
+union Work {
+  General general;
+  Lists lists;
+};
+struct Common {
+  Sums sums;
+  int n, pick, large;
+  double before;
+  u64 want;
+  u64 chunk[kThreads];
+};
+
+// A row of which all tokens stay: the span that the target falls into, then the token in it.
+__device__ void draw_span(Common& m, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc, int spans,
+                          const Record* records) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // a thread's spans lie together; weights in units of 2^-kSpanUnit of the row's largest
+  const int per = (spans - 1) / kThreads + 1, lo = min((long long)spans, (long long)per * threadIdx.x), hi = min(spans, lo + per);
+  auto span_weight = [&](int i) {
+    const Record q = records[i];
+    return q.top == kNothing ? 0.0 : (double)q.weight * weight_of(sc, logit_of(q.top));
+  };
+  double mine = 0.0;
+  for (int i = lo; i < hi; ++i) mine += span_weight(i);
+  double run = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const double o = __shfl_up(run, d);
+    if (lane >= d) run += o;
+  }
+  if (lane == 63) m.sums[0][wave] = __builtin_bit_cast(u64, run);
+  if (threadIdx.x == 0) {
+    m.pick = kThreads;
+    m.n = 0;
+  }
+  __syncthreads();
+  double whole = 0.0, before = 0.0;
+  for (int w = 0; w < kWaves; ++w) {
+    if (w == wave) before = whole;
+    whole += __builtin_bit_cast(double, m.sums[0][w]);
+  }
+  run += before;
+  const double target = draw_at(c, r, whole);
+  // the first thread whose spans end beyond the target; of a target at the end (sums in other orders may fall short of it), the
+  // last with any weight
+  if (mine > 0.0 && run > target) atomicMin(&m.pick, (int)threadIdx.x);
+  if (mine > 0.0) atomicMax(&m.n, (int)threadIdx.x);
+  __syncthreads();
+  const int chosen = m.pick < kThreads ? m.pick : m.n;
+  __syncthreads();
+  if ((int)threadIdx.x == chosen) {
+    double at = run - mine;
+    int i = lo, last = lo;
+    for (; i < hi; ++i) {
+      const double w = span_weight(i);
+      if (w > 0.0) last = i;
+      if (at + w > target) break;
+      at += w;
+    }
+    if (i == hi) {
+      i = last;
+      at -= span_weight(i);
+    }
+    m.n = i;
+    m.before = at;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  const Record q = records[m.n];
+  const double of = weight_of(sc, logit_of(q.top));
+  u64 left = min((u64)fmax((target - m.before) / of, 0.0), q.weight - 1);
+  Scale span = scale_of(c, rule, logit_of(q.top));
+  span.unit_log = kSpanUnit;
+  // eight tokens a lane, in index order
+  float x[8];
+  int i = m.n * kSpan + 8 * lane;
+  load_eight(c, c.logits + r * c.stride, i, x);
+  u64 sum = 0;
+  each(x, [&](float v) { sum += units(span, weight_of(span, v)); });
+  left -= wave_scan(sum, lane) - sum;
+  if (left >= sum) return;  // also where it has become less than 0
+  each(x, [&](float v) {
+    const u64 w = units(span, weight_of(span, v));
+    if (left < w) answer(c, r, i, (double)w * of / whole);
+    left = left < w ? ~0ull >> 1 : left - w;
+    ++i;
+  });
+}
+
+// A row's token from its records and lists (list of span i at lists + i * kListMost).  False if they do not tell; `top`: the
+// largest logit's key.
+__device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, int spans, const Record* records,
+                       const u64* lists, unsigned& top) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the largest logit and its lowest index; the bound from which the lists are whole
+  unsigned tau = 0;
+  u64 best = 0;
+  for (int i = threadIdx.x; i < spans; i += kThreads) {
+    const Record q = records[i];
+    best = max(best, (u64)q.top << 32 | (0xffffffffu - (unsigned)q.first));
+    tau = max(tau, q.tau);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    best = max(best, __shfl_xor(best, d));
+    tau = max(tau, (unsigned)__shfl_xor((int)tau, d));
+  }
+  if (lane == 0) {
+    m.sums[0][wave] = best;
+    m.sums[1][wave] = tau;
+  }
+  if (threadIdx.x == 0) m.n = 0;
+  __syncthreads();
+  for (int i = 0; i < kWaves; ++i) {
+    best = max(best, m.sums[0][i]);
+    tau = max(tau, (unsigned)m.sums[1][i]);
+  }
+  __syncthreads();
+  top = (unsigned)(best >> 32);
+  if (top == kNothing || one_token(rule)) {
+    if (threadIdx.x == 0) {
+      const bool any = top != kNothing;
+      answer(c, r, any ? (int)(0xffffffffu - (unsigned)best) : -1, any ? 1.0 : 0.0);
+    }
+    return true;
+  }
+  const Scale sc = scale_of(c, rule, logit_of(top));
+  const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
+  if (!count_cut && !weight_cut && sc.min_p == 0.0) {
+    draw_span(m, c, r, rule, sc, spans, records);
+    return true;
+  }
+  // the lists' tokens from tau on, 16 lanes a span
+  auto take = [&](u64 e, bool on) {
+    on = on && (unsigned)(e >> 32) >= tau;
+    const u64 mask = __ballot(on);
+    int slot = 0;
+    if (lane == 0 && mask) slot = atomicAdd(&m.n, __popcll(mask));
+    slot = __shfl(slot, 0) + __popcll(mask & ((1ull << lane) - 1));
+    if (on && slot < kSortMost) work.lists.entry[slot] = e;
+  };
+  constexpr int kFlight = 4, kAt = kThreads / 16;  // spans of a thread in flight, of all threads
+  for (int i0 = 0; i0 < spans; i0 += kFlight * kAt) {
+    int n[kFlight];
+    u64 e[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kAt + threadIdx.x / 16, at = min(i, spans - 1);
+      n[f] = i < spans ? records[at].count : 0;
+      e[f] = lists[(long long)at * kListMost + threadIdx.x % 16];
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = min(i0 + f * kAt + (int)threadIdx.x / 16, spans - 1);
+      take(e[f], (int)threadIdx.x % 16 < n[f]);
+      for (int j = threadIdx.x % 16 + 16; __any(j < n[f]); j += 16)
+        take(j < n[f] ? lists[(long long)i * kListMost + j] : 0, j < n[f]);
+    }
+  }
+  double whole = 0.0;  // the row's weight, in units
+  if (!count_cut && weight_cut) {
+    for (int i = threadIdx.x; i < spans; i += kThreads) {
+      const Record q = records[i];
+      if (q.top != kNothing) whole += (double)q.weight * weight_of(sc, logit_of(q.top));
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) whole += __shfl_xor(whole, d);
+    if (lane == 0) m.sums[0][wave] = __builtin_bit_cast(u64, whole);
+    __syncthreads();
+    whole = 0.0;
+    for (int i = 0; i < kWaves; ++i) whole += __builtin_bit_cast(double, m.sums[0][i]);
+    whole = ldexp(whole, c.unit_log - kSpanUnit);
+  }
+  __syncthreads();
+  const int n = m.n;
+  bool found = n > 0 && n <= kSortMost;
+  if (found) {
+    const int n2 = power_of_two(n);
+    for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
+    sort_descending(work.lists.entry, n2);
+    if (threadIdx.x == 0) m.large = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n2; i += kThreads) {
+      const double real = i < n ? weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))) : 0.0;
+      work.lists.weight[i] = units(sc, real);
+      const int large = __popcll(__ballot(i < n && real >= sc.min_p));
+      if (lane == 0) atomicAdd(&m.large, large);
+    }
+    __syncthreads();
+    const bool complete = tau <= kNothing + 1;  // all that is not -inf is on the lists
+    // min_p: weights descend, those that are large enough come first; beyond the lists there may be more if all on them are
+    int stay = sc.min_p > 0.0 ? m.large : n;
+    const bool short_of_min = sc.min_p > 0.0 && (complete || stay < n);
+    const int of = count_cut ? min(n, rule.top_k) : n;
+    found = short_of_min && !weight_cut && !count_cut;
+    if (count_cut) {
+      found = complete || n >= rule.top_k;
+      stay = min(stay, of);
+    }
+    if (weight_cut && (found || !count_cut)) {
+      // from here on thread t has the entries 2 t and 2 t + 1
+      const int i0 = 2 * threadIdx.x;
+      const u64 w0 = i0 < of ? work.lists.weight[i0] : 0, w1 = i0 + 1 < of ? work.lists.weight[i0 + 1] : 0;
+      u64 listed;
+      const u64 before = block_scan(m.sums, w0 + w1, listed);
+      const u64 target = part_units(rule, count_cut ? (double)listed : whole);
+      found = count_cut || complete || listed >= target || short_of_min;
+      if (threadIdx.x == 0) m.pick = stay;
+      __syncthreads();
+      // the first entry that reaches the target is the last to stay
+      if (before < target && before + w0 + w1 >= target) atomicMin(&m.pick, before + w0 >= target ? i0 + 1 : i0 + 2);
+      __syncthreads();
+      stay = m.pick;
+    }
+    if (found) {
+      // in index order
+      __syncthreads();
+      const int s2 = power_of_two(stay);
+      for (int i = threadIdx.x; i < s2; i += kThreads)
+        work.lists.entry[i] = i < stay ? work.lists.entry[i] << 32 | (unsigned)i : 0;
+      sort_descending(work.lists.entry, s2);
+      const int i0 = 2 * threadIdx.x;
+      const u64 e0 = i0 < stay ? work.lists.entry[i0] : 0, e1 = i0 + 1 < stay ? work.lists.entry[i0 + 1] : 0;
+      const u64 w0 = i0 < stay ? work.lists.weight[(unsigned)e0] : 0, w1 = i0 + 1 < stay ? work.lists.weight[(unsigned)e1] : 0;
+      u64 left;
+      const u64 before = block_scan(m.sums, w0 + w1, left), target = draw_units(c, r, left);
+      if (target >= before && target < before + w0 + w1) {
+        const bool second = target >= before + w0;
+        answer(c, r, (int)(0xffffffffu - (unsigned)((second ? e1 : e0) >> 32)), (double)(second ? w1 : w0) / (double)left);
+      }
+      return true;
+    }
+  }
+  __syncthreads();
+  return false;
+}
+
+// ---- rows of which thousands of tokens stay ----
+// Where only weights cut a row (top_p or min_p, no top_k), its weights are sorted into kBins bins of their logarithm, a chunk of kChunk
+// logits a workgroup; then one workgroup a row finds the bin that the cut falls into, collects and sorts that bin's tokens,
+// and draws: the bins hold each chunk's weight above the cut, so one chunk is read again.
+constexpr int kChunk = 8192, kChunksMost = kThreads;
+
+__device__ __forceinline__ bool binned(const SampleRule& rule, int vocab) {
+  return !by_count(rule, vocab) && !(by_weight(rule) && rule.min_p > 0.0f);
+}
+// Descending with x; a weight of 0 falls into the last.
+__device__ __forceinline__ int bin_of(const Scale& s, float x) {
+  const float d = s.m - x, g = (float)(s.per * (kBins / 50.0));
+  return x == s.m ? 0 : (int)fminf(d * g, (float)(kBins - 1));
+}
+
+// hist (LDS): the weights of a chunk's tokens, of those that min_p leaves.
+__device__ void bin_chunk(u64* hist, const SampleCall& c, const float* row, const Scale& sc, int chunk) {
+  for (int i = threadIdx.x; i < kBins; i += kThreads) hist[i] = 0;
+  float x[8];
+  load_eight(c, row, chunk * kChunk + 8 * threadIdx.x, x);
+  __syncthreads();
+  each(x, [&](float t) {
+    const double v = weight_of(sc, t);
+    const u64 w = v >= sc.min_p ? units(sc, v) : 0;
+    if (w) atomicAdd(&hist[bin_of(sc, t)], w);
+  });
+  __syncthreads();
+}
+
+// The row's token from its chunks' bins (chunk i's at hist + i * kBins).
+__device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc,
+                              const u64* hist) {
+  const float* row = c.logits + r * c.stride;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = (c.vocab - 1) / kChunk + 1;
+  if (chunks > kChunksMost) {
+    general_row(work.general, m.sums, c, r, rule, sc);
+    return;
+  }
+  int cut = kBins;   // the bin that the cut falls into: tokens of lower ones stay,
+  u64 last = ~0ull;  // and of its tokens those at or above this entry
+  int stay = 0;
+  if (by_weight(rule)) {
+    const int i0 = 2 * threadIdx.x;
+    u64 w0 = 0, w1 = 0;
+#pragma unroll 8
+    for (int i = 0; i < chunks; ++i) {
+      w0 += hist[(long long)i * kBins + i0];
+      w1 += hist[(long long)i * kBins + i0 + 1];
+    }
+    u64 whole;
+    u64 before = block_scan(m.sums, w0 + w1, whole);
+    const u64 target = min(whole, part_units(rule, (double)whole));
+    if (before < target && before + w0 + w1 >= target) {
+      const bool second = before + w0 < target;
+      m.pick = second ? i0 + 1 : i0;
+      m.want = target - before - (second ? w0 : 0);
+    }
+    if (threadIdx.x == 0) m.n = 0;
+    __syncthreads();
+    cut = m.pick;
+    const u64 want = m.want;
+    // four logits a thread at a time
+    float x[4], next[4];
+    load_four(c, row, 4 * threadIdx.x, x);
+#pragma unroll 1
+    for (int at = 4 * threadIdx.x; at < c.vocab; at += 4 * kThreads) {
+      if (at + 4 * kThreads < c.vocab) load_four(c, row, at + 4 * kThreads, next);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (bin_of(sc, x[e]) == cut && x[e] > -INFINITY) {
+          const int slot = atomicAdd(&m.n, 1);
+          if (slot < kSortMost) work.lists.entry[slot] = (u64)key_of(x[e]) << 32 | (0xffffffffu - (unsigned)(at + e));
+        }
+        x[e] = next[e];
+      }
+    }
+    __syncthreads();
+    const int n = m.n;
+    if (n > kSortMost) {
+      __syncthreads();
+      general_row(work.general, m.sums, c, r, rule, sc);
+      return;
+    }
+    const int n2 = power_of_two(n);
+    for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
+    sort_descending(work.lists.entry, n2);
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n2; i += kThreads)
+      work.lists.weight[i] = i < n ? units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32)))) : 0;
+    if (threadIdx.x == 0) m.pick = n;
+    __syncthreads();
+    w0 = i0 < n ? work.lists.weight[i0] : 0;
+    w1 = i0 + 1 < n ? work.lists.weight[i0 + 1] : 0;
+    u64 all;
+    before = block_scan(m.sums, w0 + w1, all);
+    if (before < want && before + w0 + w1 >= want) atomicMin(&m.pick, before + w0 >= want ? i0 + 1 : i0 + 2);
+    __syncthreads();
+    stay = m.pick;
+    last = stay > 0 ? work.lists.entry[stay - 1] : ~0ull;
+  }
+  // what stays of each chunk
+  __syncthreads();
+  for (int i = wave; i < chunks; i += kWaves) {
+    u64 sum = 0;
+#pragma unroll 8
+    for (int b = 0; b < kBins; b += 64) sum += b + lane < cut ? hist[(long long)i * kBins + b + lane] : 0;
+    for (int j = lane; j < stay; j += 64)
+      if ((int)((0xffffffffu - (unsigned)work.lists.entry[j]) / kChunk) == i) sum += work.lists.weight[j];
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) m.chunk[i] = sum;
+  }
+  __syncthreads();
+  const u64 mine = (int)threadIdx.x < chunks ? m.chunk[threadIdx.x] : 0;
+  u64 whole;
+  const u64 before = block_scan(m.sums, mine, whole), target = draw_units(c, r, whole);
+  if (target >= before && target < before + mine) {
+    m.pick = threadIdx.x;
+    m.want = target - before;
+  }
+  __syncthreads();
+  // of that chunk's tokens each thread has eight, in index order
+  int i = m.pick * kChunk + 8 * threadIdx.x;
+  u64 want = m.want, sum = 0;
+  float x[8];
+  load_eight(c, row, i, x);
+  const auto weight = [&](float t, int at) -> u64 {
+    const int b = bin_of(sc, t);
+    if (b > cut || (b == cut && ((u64)key_of(t) << 32 | (0xffffffffu - (unsigned)at)) < last)) return 0;
+    const double v = weight_of(sc, t);
+    return v >= sc.min_p ? units(sc, v) : 0;
+  };
+  int at = i;
+  each(x, [&](float t) { sum += weight(t, at++); });
+  u64 all;
+  const u64 start = block_scan(m.sums, sum, all);
+  if (want < start || want - start >= sum) return;
+  want -= start;
+  each(x, [&](float t) {
+    const u64 w = weight(t, i);
+    if (want < w) answer(c, r, i, (double)w / (double)whole);
+    want = want < w ? ~0ull >> 1 : want - w;
+    ++i;
+  });
+}
+
+// Spans of all rows, four a workgroup.
+__global__ __launch_bounds__(256) void sample_list_kernel(SampleCall c, int spans, int groups, Record* records, u64* lists) {
+  const long long r = blockIdx.x / groups;
+  const int at = (int)(blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
+  if (at >= spans) return;
+  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
+  list_span(c, c.logits + r * c.stride, rule, spans, at, records + r * spans + at,
+            lists + (r * spans + at) * kListMost);
+}
+// later: rows that the lists do not tell are left to the next two kernels where their rule allows; left[r]: the largest logit's key,
+// or 0 for a row that is done.
+__global__ __launch_bounds__(kThreads) void sample_choose_kernel(SampleCall c, int spans, const Record* records, const u64* lists,
+                                                                 bool later, unsigned* left) {
+  __shared__ Work work;
+  __shared__ Common common;
+  const long long r = blockIdx.x;
+  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
+  unsigned top;
+  const bool done = choose(work, common, c, r, rule, spans, records + r * spans, lists + r * spans * kListMost, top);
+  const bool leave = !done && later && binned(rule, c.vocab);
+  if (threadIdx.x == 0) left[r] = leave ? top : 0;
+  if (!done && !leave) general_row(work.general, common.sums, c, r, rule, scale_of(c, rule, logit_of(top)));
+}
+__global__ __launch_bounds__(kThreads) void sample_bin_kernel(SampleCall c, int chunks, const unsigned* left, u64* hists) {
+  __shared__ u64 hist[kBins];
+  const long long r = blockIdx.x / chunks;
+  const int chunk = blockIdx.x % chunks;
+  const unsigned top = left[r];
+  if (!top) return;
+  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
+  bin_chunk(hist, c, c.logits + r * c.stride, scale_of(c, rule, logit_of(top)), chunk);
+  u64* to = hists + (r * chunks + chunk) * kBins;
+  for (int i = threadIdx.x; i < kBins; i += kThreads) to[i] = hist[i];
+}
+__global__ __launch_bounds__(kThreads) void sample_binned_kernel(SampleCall c, int chunks, const unsigned* left, const u64* hists) {
+  __shared__ Work work;
+  __shared__ Common common;
+  const long long r = blockIdx.x;
+  const unsigned top = left[r];
+  if (!top) return;
+  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
+  choose_binned(work, common, c, r, rule, scale_of(c, rule, logit_of(top)), hists + r * chunks * kBins);
+}
+
+// All of it for a row of up to kWaves spans, or, where there is no room for records, for a row of any length by general_row.
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int spans) {
+  __shared__ Work work;
+  __shared__ Common common;
+  __shared__ Record records[kWaves];
+  __shared__ u64 lists[kWaves * kListMost];  // and then the bins
+  static_assert(kWaves * kListMost >= kBins && kWaves * kSpan <= kChunk, "bins of one chunk in the lists' place");
+  const long long r = blockIdx.x;
+  const float* row = c.logits + r * c.stride;
+  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  if (spans <= kWaves) {
+    if (wave < spans) list_span(c, row, rule, spans, wave, &records[wave], &lists[wave * kListMost]);
+    __syncthreads();
+    unsigned top;
+    if (choose(work, common, c, r, rule, spans, records, lists, top)) return;
+    const Scale sc = scale_of(c, rule, logit_of(top));
+    if (binned(rule, c.vocab)) {
+      bin_chunk(lists, c, row, sc, 0);
+      choose_binned(work, common, c, r, rule, sc, lists);
+    } else {
+      general_row(work.general, common.sums, c, r, rule, sc);
+    }
+    return;
+  }
+  // the largest logit, of equal ones the lowest index
+  u64 top = 0;
+  for (int i = threadIdx.x; i < c.vocab; i += kThreads)
+    top = max(top, (u64)key_of(clean(row[i])) << 32 | (0xffffffffu - (unsigned)i));
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = max(top, __shfl_xor(top, d));
+  if (lane == 0) common.sums[0][wave] = top;
+  __syncthreads();
+  for (int w = 0; w < kWaves; ++w) top = max(top, common.sums[0][w]);
+  __syncthreads();
+  const unsigned top_key = (unsigned)(top >> 32);
+  if (top_key == kNothing || one_token(rule)) {
+    const bool any = top_key != kNothing;
+    if (threadIdx.x == 0) answer(c, r, any ? (int)(0xffffffffu - (unsigned)top) : -1, any ? 1.0 : 0.0);
+    return;
+  }
+  general_row(work.general, common.sums, c, r, rule, scale_of(c, rule, logit_of(top_key)));
 }
 
 }  // namespace
@@ -313,20 +990,62 @@ int sample_unit_log(int vocab) {
   return std::min(51, 62 - bits);
 }
 
-size_t sample_workspace_bytes(const SampleCall&) { return 0; }
+// Of a row: lists, records, a word for what is left, and bins; none where a workgroup holds them.
+struct RowBytes {
+  size_t lists, records, bins, all;
+};
+static RowBytes row_bytes(const SampleCall& c) {
+  const size_t spans = (size_t)(c.vocab - 1) / kSpan + 1, chunks = (size_t)(c.vocab - 1) / kChunk + 1;
+  if (spans <= kWaves) return {0, 0, 0, 0};
+  RowBytes b{spans * kListMost * sizeof(u64), spans * sizeof(Record), chunks > kChunksMost ? 0 : chunks * kBins * sizeof(u64), 0};
+  b.all = b.lists + b.records + b.bins + 8;
+  return b;
+}
+constexpr size_t kMostBytes = (size_t)64 << 20;  // rows go through it in turn
+
+size_t sample_workspace_bytes(const SampleCall& call, int rows) {
+  const size_t each = row_bytes(call).all;
+  return std::min(each * (size_t)rows, std::max(kMostBytes, each));
+}
 
 hipError_t launch_sample(hipStream_t s, const SampleCall& call, int rows, void* ws, size_t ws_bytes) {
-  constexpr int kMost = 1 << 21;
-  for (int at = 0; at < rows; at += kMost) {
+  const int spans = (call.vocab - 1) / kSpan + 1, groups = (spans - 1) / 4 + 1, chunks = (call.vocab - 1) / kChunk + 1;
+  const RowBytes each = row_bytes(call);
+  const bool listed = each.all > 0 && ws_bytes >= each.all;
+  // the two kernels for rows that the lists do not tell: not if the host knows that a count cuts every row, or nothing does
+  const SampleRule& rule = call.rule;
+  const bool later = each.bins > 0 && (call.rules || ((rule.top_k == 0 || rule.top_k >= call.vocab) && rule.temperature > 0.0f &&
+                                                      (rule.top_p < 1.0f) != (rule.min_p > 0.0f)));
+  long long most = 1 << 21;
+  if (listed)
+    most = std::min({most, (long long)(std::min(ws_bytes, std::max(kMostBytes, each.all)) / each.all), (1LL << 21) / groups + 1});
+  for (long long at = 0; at < rows; at += most) {
+    const int n = (int)std::min(most, rows - at);
     SampleCall c = call;
     c.logits += at * call.stride;
     if (c.rules) c.rules += at;
     c.u += at;
     c.tokens += at;
     if (c.probs) c.probs += at;
-    hipLaunchKernelGGL(sample_row_kernel, dim3((unsigned)std::min(kMost, rows - at)), dim3(kThreads), 0, s, c);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+    hipError_t e;
+    if (listed) {
+      u64* lists = static_cast<u64*>(ws);
+      u64* hists = lists + n * each.lists / sizeof(u64);
+      Record* records = reinterpret_cast<Record*>(hists + n * each.bins / sizeof(u64));
+      unsigned* left = reinterpret_cast<unsigned*>(records + (size_t)n * spans);
+      hipLaunchKernelGGL(sample_list_kernel, dim3((unsigned)(n * (long long)groups)), dim3(256), 0, s, c, spans, groups, records, lists);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      hipLaunchKernelGGL(sample_choose_kernel, dim3(n), dim3(kThreads), 0, s, c, spans, records, lists, later, left);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      if (later) {
+        hipLaunchKernelGGL(sample_bin_kernel, dim3((unsigned)(n * (long long)chunks)), dim3(kThreads), 0, s, c, chunks, left, hists);
+        if ((e = hipGetLastError()) != hipSuccess) return e;
+        hipLaunchKernelGGL(sample_binned_kernel, dim3(n), dim3(kThreads), 0, s, c, chunks, left, hists);
+      }
+    } else {
+      hipLaunchKernelGGL(sample_row_kernel, dim3(n), dim3(kThreads), 0, s, c, spans);
+    }
+    if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   return hipSuccess;
 }
