@@ -597,6 +597,67 @@ __device__ void draw_span(Common& m, const SampleCall& c, long long r, const Sam
   });
 }
 
+// The choice from all of a few tokens, without a sort: four threads a token compare it with the others.  Its place and the weight
+// before it decide whether it stays, and the weight of the tokens with lower indexes whether it is drawn.  `whole`: the row's
+// weight where only a weight cuts; complete: nothing else is in the row.  False if the tokens do not tell.
+constexpr int kFew = kThreads / 4;
+template <typename T>
+__device__ __forceinline__ T of_four(T v) {
+  v += across<1>(v);
+  return v + across<2>(v);
+}
+__device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const SampleCall& c, long long r, const SampleRule& rule,
+                                           const Scale& sc, int n, double whole, bool complete) {
+  const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
+  const int i = threadIdx.x / 4, part = threadIdx.x % 4;
+  if ((int)threadIdx.x < n) {
+    const double real = weight_of(sc, logit_of((unsigned)(lists.entry[threadIdx.x] >> 32)));
+    lists.weight[threadIdx.x] = units(sc, real);
+    const int large = __popcll(__ballot(real >= sc.min_p));
+    if ((threadIdx.x & 63) == 0) atomicAdd(&m.large, large);
+  }
+  __syncthreads();
+  const int of = count_cut ? min(n, rule.top_k) : n;
+  const u64 own = i < n ? lists.entry[i] : 0, weight = i < n ? lists.weight[i] : 0;
+  unsigned place = 0;
+  u64 before = 0;
+  if (i < n) {
+#pragma unroll 4
+    for (int j = part; j < n; j += 4) {
+      const bool above = lists.entry[j] > own;
+      place += above;
+      before += above ? lists.weight[j] : 0;
+    }
+    place = of_four(place);
+    before = of_four(before);
+    if (part == 0 && (int)place == of - 1) m.want = before + weight;
+  }
+  __syncthreads();
+  const u64 listed = m.want, target = part_units(rule, count_cut ? (double)listed : whole);
+  const int large = sc.min_p > 0.0 ? m.large : n;
+  const bool short_of_min = sc.min_p > 0.0 && (complete || large < n);
+  if (count_cut ? !(complete || n >= rule.top_k) : !(short_of_min || (weight_cut && (complete || listed >= target)))) return false;
+  const bool stays = i < n && (int)place < min(of, large) && (!weight_cut || before < target);
+  if (part == 0 && i < n) lists.weight[i] = stays ? weight : 0;
+  __syncthreads();
+  u64 left = 0;
+  before = 0;
+  if (i < n) {
+#pragma unroll 4
+    for (int j = part; j < n; j += 4) {
+      const u64 w = lists.weight[j];
+      left += w;
+      before += (unsigned)lists.entry[j] > (unsigned)own ? w : 0;
+    }
+    left = of_four(left);
+    before = of_four(before);
+    const u64 at = draw_units(c, r, left);
+    if (part == 0 && stays && at >= before && at < before + weight)
+      answer(c, r, (int)(0xffffffffu - (unsigned)own), (double)weight / (double)left);
+  }
+  return true;
+}
+
 // A row's token from its records and lists (list of span i at lists + i * kListMost).  False if they do not tell; `top`: the
 // largest logit's key.
 __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, int spans, const Record* records,
@@ -619,8 +680,9 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     m.sums[0][wave] = best;
     m.sums[1][wave] = tau;
   }
-  if (threadIdx.x == 0) m.n = 0;
+  if (threadIdx.x == 0) m.n = m.large = 0;
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < kWaves; ++i) {
     best = max(best, m.sums[0][i]);
     tau = max(tau, (unsigned)m.sums[1][i]);
@@ -683,13 +745,23 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
   }
   __syncthreads();
   const int n = m.n;
+  const bool complete = tau <= kNothing + 1;  // all that is not -inf is on the lists
   bool found = n > 0 && n <= kSortMost;
+  if (found && n <= kFew) {
+    if (choose_few(work.lists, m, c, r, rule, sc, n, whole, complete)) return true;
+    found = false;
+  }
+  if (found && weight_cut && !count_cut && !complete && !(sc.min_p > 0.0)) {  // do the lists reach what top_p asks for?
+    u64 mine = 0, listed;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += kThreads) mine += units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))));
+    block_scan(m.sums, mine, listed);
+    found = listed >= part_units(rule, whole);
+  }
   if (found) {
     const int n2 = power_of_two(n);
     for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
     sort_descending(work.lists.entry, n2);
-    if (threadIdx.x == 0) m.large = 0;
-    __syncthreads();
 #pragma unroll 1
     for (int i = threadIdx.x; i < n2; i += kThreads) {
       const double real = i < n ? weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))) : 0.0;
@@ -698,7 +770,6 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
       if (lane == 0) atomicAdd(&m.large, large);
     }
     __syncthreads();
-    const bool complete = tau <= kNothing + 1;  // all that is not -inf is on the lists
     // min_p: weights descend, those that are large enough come first; beyond the lists there may be more if all on them are
     int stay = sc.min_p > 0.0 ? m.large : n;
     const bool short_of_min = sc.min_p > 0.0 && (complete || stay < n);
@@ -807,20 +878,21 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     __syncthreads();
     cut = m.pick;
     const u64 want = m.want;
-    // four logits a thread at a time
-    float x[4], next[4];
-    load_four(c, row, 4 * threadIdx.x, x);
+    // 16 logits a thread at a time
 #pragma unroll 1
-    for (int at = 4 * threadIdx.x; at < c.vocab; at += 4 * kThreads) {
-      if (at + 4 * kThreads < c.vocab) load_four(c, row, at + 4 * kThreads, next);
+    for (int at = 4 * threadIdx.x; at < c.vocab; at += 16 * kThreads) {
+      float x[4][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (bin_of(sc, x[e]) == cut && x[e] > -INFINITY) {
-          const int slot = atomicAdd(&m.n, 1);
-          if (slot < kSortMost) work.lists.entry[slot] = (u64)key_of(x[e]) << 32 | (0xffffffffu - (unsigned)(at + e));
-        }
-        x[e] = next[e];
-      }
+      for (int f = 0; f < 4; ++f) load_four(c, row, at + 4 * kThreads * f, x[f]);
+#pragma unroll
+      for (int f = 0; f < 4; ++f)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (bin_of(sc, x[f][e]) == cut && x[f][e] > -INFINITY) {
+            const int slot = atomicAdd(&m.n, 1);
+            if (slot < kSortMost)
+              work.lists.entry[slot] = (u64)key_of(x[f][e]) << 32 | (0xffffffffu - (unsigned)(at + 4 * kThreads * f + e));
+          }
     }
     __syncthreads();
     const int n = m.n;
@@ -829,22 +901,38 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
       general_row(work.general, m.sums, c, r, rule, sc);
       return;
     }
-    const int n2 = power_of_two(n);
-    for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
-    sort_descending(work.lists.entry, n2);
+    if (threadIdx.x == 0) m.want = 0;
+    if (n <= kFew) {
+      if ((int)threadIdx.x < n)
+        work.lists.weight[threadIdx.x] = units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[threadIdx.x] >> 32))));
+      __syncthreads();
+      const int i = threadIdx.x / 4, part = threadIdx.x % 4;
+      if (i < n) {
+        const u64 own = work.lists.entry[i];
+        u64 above = 0;
+#pragma unroll 4
+        for (int j = part; j < n; j += 4) above += work.lists.entry[j] > own ? work.lists.weight[j] : 0;
+        above = of_four(above);
+        // the first entry that reaches the target is the last to stay
+        if (part == 0 && above < want && above + work.lists.weight[i] >= want) m.want = own;
+      }
+    } else {
+      const int n2 = power_of_two(n);
+      for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
+      sort_descending(work.lists.entry, n2);
 #pragma unroll 1
-    for (int i = threadIdx.x; i < n2; i += kThreads)
-      work.lists.weight[i] = i < n ? units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32)))) : 0;
-    if (threadIdx.x == 0) m.pick = n;
+      for (int i = threadIdx.x; i < n2; i += kThreads)
+        work.lists.weight[i] = i < n ? units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32)))) : 0;
+      __syncthreads();
+      w0 = i0 < n ? work.lists.weight[i0] : 0;
+      w1 = i0 + 1 < n ? work.lists.weight[i0 + 1] : 0;
+      u64 all;
+      before = block_scan(m.sums, w0 + w1, all);
+      if (before < want && before + w0 + w1 >= want) m.want = work.lists.entry[before + w0 >= want ? i0 : i0 + 1];
+    }
     __syncthreads();
-    w0 = i0 < n ? work.lists.weight[i0] : 0;
-    w1 = i0 + 1 < n ? work.lists.weight[i0 + 1] : 0;
-    u64 all;
-    before = block_scan(m.sums, w0 + w1, all);
-    if (before < want && before + w0 + w1 >= want) atomicMin(&m.pick, before + w0 >= want ? i0 + 1 : i0 + 2);
-    __syncthreads();
-    stay = m.pick;
-    last = stay > 0 ? work.lists.entry[stay - 1] : ~0ull;
+    last = m.want;
+    stay = n;
   }
   // what stays of each chunk
   __syncthreads();
@@ -853,7 +941,8 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
 #pragma unroll 8
     for (int b = 0; b < kBins; b += 64) sum += b + lane < cut ? hist[(long long)i * kBins + b + lane] : 0;
     for (int j = lane; j < stay; j += 64)
-      if ((int)((0xffffffffu - (unsigned)work.lists.entry[j]) / kChunk) == i) sum += work.lists.weight[j];
+      if (work.lists.entry[j] >= last && (int)((0xffffffffu - (unsigned)work.lists.entry[j]) / kChunk) == i)
+        sum += work.lists.weight[j];
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
     if (lane == 0) m.chunk[i] = sum;
