@@ -232,10 +232,11 @@ __global__ __launch_bounds__(kThreads, 2) void w4_skinny_kernel(W4 w, int m, int
       for (int q = 0; q < 3; ++q) a[j % kSteps][mb][q] = px[mb][q * part + at];
   };
   if (b0 + wave < b1) {
+    fetch_codes(0, b0 + wave);
 #pragma unroll
     for (int j = 0; j < kSteps - 1; ++j) fetch_x(b0 + wave, j);
 #pragma unroll
-    for (int n = 0; n < kAhead; ++n) fetch_codes(n, b0 + wave + n * kWaves);
+    for (int n = 1; n < kAhead; ++n) fetch_codes(n, b0 + wave + n * kWaves);
   }
   for (int base = b0 + wave; base < b1; base += kAhead * kWaves) {
 #pragma unroll

@@ -38,7 +38,7 @@ class Sampling:
         if not (self.temperature >= 0 and self.top_k >= 0 and 0 <= self.top_p <= 1 and 0 <= self.min_p <= 1):
             raise InvalidInput(f"Sampling: temperature ({self.temperature}) and top_k ({self.top_k}) must not be negative, "
                                f"top_p ({self.top_p}) and min_p ({self.min_p}) from 0 to 1")
-        if self.top_k != int(self.top_k):
+        if not np.isfinite(self.top_k) or self.top_k != int(self.top_k):
             raise InvalidInput(f"Sampling: top_k ({self.top_k}) must be a whole number")
 
     def _native(self) -> N.Sampling:

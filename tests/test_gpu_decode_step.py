@@ -208,3 +208,35 @@ def test_captured_token(dev, rows, dim, h, hkv, d, vocab):
                 assert near <= near_border(want[4][i], 0.9) or want[5].view(np.int32)[i] == token
         hip.hipGraphExecDestroy(ex)
         hip.hipGraphDestroy(graph)
+
+
+def test_two_contexts_at_once(dev):
+    """Calls of two contexts, one behind the other without a wait: each has its own stream and scratch, and gives what it gives alone."""
+    rng = np.random.default_rng(77)
+    rows, k, n = 20, 1024, 30011
+    w = Weights4.quantize(rng.standard_normal((n, k), dtype=np.float32), 64, device=dev)
+    xs = [_t(rng.standard_normal((rows, k), dtype=np.float32), dev) for _ in range(2)]
+    us = [_t(rng.random(rows, dtype=np.float32), dev) for _ in range(2)]
+    out = [(Tensor.empty([rows, n], dev), Tensor.empty([rows], dev), Tensor.empty([rows], dev)) for _ in range(2)]
+    rules = [N.Sampling(1.0, 0, 0.9, 0.0), N.Sampling(0.7, 30, 0.95, 0.0)]
+    dev.sync()
+    with _FreshCtx(dev) as f, _FreshCtx(dev) as g:
+        def call(c, i):
+            y, tokens, probs = out[i]
+            assert c.lib.bch_w4_linear(c.ctx, rows, w._w, _p(xs[i]), k, None, N.BCH_ACT_NONE, _p(y), n) == 0
+            assert c.lib.bch_sample(c.ctx, rows, n, _p(y), n, rules[i], None, _p(us[i]), _p(tokens), _p(probs)) == 0
+
+        def results():
+            assert f.lib.bch_sync(f.ctx) == 0 and g.lib.bch_sync(g.ctx) == 0
+            return [t.to_numpy().view(np.int32).copy() for o in out for t in o]
+
+        call(f, 0)
+        alone = results()[:3]
+        call(g, 1)
+        alone += results()[3:]
+        for _ in range(3):
+            for _ in range(10):
+                call(f, 0)
+                call(g, 1)
+            for a, b in zip(results(), alone):
+                assert np.array_equal(a, b)

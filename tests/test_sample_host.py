@@ -28,7 +28,7 @@ def test_model():
     assert choose(np.array([-np.inf, np.nan, 0.0], np.float32), 0.0, 1.0, 0, 1.0, 0.0)[0] == 2
 
 
-@pytest.mark.parametrize("kwargs", [{"temperature": -1.0}, {"temperature": math.nan}, {"top_k": -1}, {"top_k": 1.5}, {"top_p": 1.1},
+@pytest.mark.parametrize("kwargs", [{"temperature": -1.0}, {"temperature": math.nan}, {"top_k": -1}, {"top_k": 1.5}, {"top_k": math.inf}, {"top_p": 1.1},
                                     {"top_p": -0.1}, {"top_p": math.nan}, {"min_p": 1.5}, {"min_p": -1.0}, {"min_p": math.nan}])
 def test_rules_refuse(kwargs):
     with pytest.raises(InvalidInput):
