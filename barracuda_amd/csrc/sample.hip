@@ -597,19 +597,23 @@ __device__ void draw_span(Common& m, const SampleCall& c, long long r, const Sam
   });
 }
 
-// The choice from all of a few tokens, without a sort: four threads a token compare it with the others.  Its place and the weight
+// The choice from all of a few tokens, without a sort: 4 to 16 threads a token compare it with the others.  Its place and the weight
 // before it decide whether it stays, and the weight of the tokens with lower indexes whether it is drawn.  `whole`: the row's
 // weight where only a weight cuts; complete: nothing else is in the row.  False if the tokens do not tell.
 constexpr int kFew = kThreads / 4;
+__device__ __forceinline__ int few_log(int n) { return n <= kThreads / 16 ? 4 : n <= kThreads / 8 ? 3 : n <= kThreads / 4 ? 2 : 1; }
 template <typename T>
-__device__ __forceinline__ T of_four(T v) {
+__device__ __forceinline__ T over_parts(T v, int log) {
   v += across<1>(v);
-  return v + across<2>(v);
+  if (log > 1) v += across<2>(v);
+  if (log > 2) v += across<4>(v);
+  if (log > 3) v += across<8>(v);
+  return v;
 }
 __device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const SampleCall& c, long long r, const SampleRule& rule,
                                            const Scale& sc, int n, double whole, bool complete) {
   const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
-  const int i = threadIdx.x / 4, part = threadIdx.x % 4;
+  const int log = few_log(n), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
   if ((int)threadIdx.x < n) {
     const double real = weight_of(sc, logit_of((unsigned)(lists.entry[threadIdx.x] >> 32)));
     lists.weight[threadIdx.x] = units(sc, real);
@@ -622,14 +626,15 @@ __device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const Sample
   unsigned place = 0;
   u64 before = 0;
   if (i < n) {
-#pragma unroll 4
-    for (int j = part; j < n; j += 4) {
+#pragma unroll 1
+    for (int j = part; j < n; j += parts) {
+      const u64 w = lists.weight[j];
       const bool above = lists.entry[j] > own;
       place += above;
-      before += above ? lists.weight[j] : 0;
+      before += above ? w : 0;
     }
-    place = of_four(place);
-    before = of_four(before);
+    place = over_parts(place, log);
+    before = over_parts(before, log);
     if (part == 0 && (int)place == of - 1) m.want = before + weight;
   }
   __syncthreads();
@@ -643,14 +648,15 @@ __device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const Sample
   u64 left = 0;
   before = 0;
   if (i < n) {
-#pragma unroll 4
-    for (int j = part; j < n; j += 4) {
+#pragma unroll 1
+    for (int j = part; j < n; j += parts) {
       const u64 w = lists.weight[j];
+      const unsigned low = (unsigned)lists.entry[j];
       left += w;
-      before += (unsigned)lists.entry[j] > (unsigned)own ? w : 0;
+      before += low > (unsigned)own ? w : 0;
     }
-    left = of_four(left);
-    before = of_four(before);
+    left = over_parts(left, log);
+    before = over_parts(before, log);
     const u64 at = draw_units(c, r, left);
     if (part == 0 && stays && at >= before && at < before + weight)
       answer(c, r, (int)(0xffffffffu - (unsigned)own), (double)weight / (double)left);
@@ -658,11 +664,57 @@ __device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const Sample
   return true;
 }
 
+// Of n entries those with fewer than k larger logits above them; how many that are.  Comparing keys alone, two operations a pair, it
+// spares choose_few most of its pairs (191 entries, k = 40: a call of one row 17.8 -> 14.5 us).
+constexpr int kKeysMost = kThreads / 2;
+__device__ __forceinline__ int largest_of(Lists& lists, Common& m, int n, int k) {
+  unsigned* keys = reinterpret_cast<unsigned*>(lists.weight);
+  const int log = few_log(n), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
+  keys[threadIdx.x] = (int)threadIdx.x < n ? (unsigned)(lists.entry[threadIdx.x] >> 32) : 0;
+  if (threadIdx.x == 0) m.pick = 0;
+  __syncthreads();
+  bool on = false;
+  u64 own = 0;
+  if (i < n) {
+    own = lists.entry[i];
+    const unsigned key = (unsigned)(own >> 32);
+    int above = 0;
+#pragma unroll 2
+    for (int j = part; 4 * j < n; j += parts) {
+      const uint4 q = reinterpret_cast<const uint4*>(keys)[j];
+      above += (q.x > key) + (q.y > key) + (q.z > key) + (q.w > key);
+    }
+    on = over_parts((unsigned)above, log) < (unsigned)k && part == 0;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  const u64 mask = __ballot(on);
+  int slot = 0;
+  if (lane == 0 && mask) slot = atomicAdd(&m.pick, __popcll(mask));
+  slot = __shfl(slot, 0) + __popcll(mask & ((1ull << lane) - 1));
+  if (on) lists.entry[slot] = own;
+  __syncthreads();
+  return m.pick;
+}
+
 // A row's token from its records and lists (list of span i at lists + i * kListMost).  False if they do not tell; `top`: the
 // largest logit's key.
 __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, int spans, const Record* records,
                        const u64* lists, unsigned& top) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // the beginnings of the lists, 16 lanes a span
+  constexpr int kFlight = 4, kAt = kThreads / 16;  // spans of a thread in flight, of all threads
+  int count[kFlight];
+  u64 e[kFlight];
+  auto fetch = [&](int i0) {
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int i = i0 + f * kAt + threadIdx.x / 16, at = min(i, spans - 1);
+      count[f] = i < spans ? records[at].count : 0;
+      e[f] = lists[(long long)at * kListMost + threadIdx.x % 16];
+    }
+  };
+  fetch(0);
   // the largest logit and its lowest index; the bound from which the lists are whole
   unsigned tau = 0;
   u64 best = 0;
@@ -702,7 +754,7 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     draw_span(m, c, r, rule, sc, spans, records);
     return true;
   }
-  // the lists' tokens from tau on, 16 lanes a span
+  // the lists' tokens from tau on
   auto take = [&](u64 e, bool on) {
     on = on && (unsigned)(e >> 32) >= tau;
     const u64 mask = __ballot(on);
@@ -711,22 +763,14 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     slot = __shfl(slot, 0) + __popcll(mask & ((1ull << lane) - 1));
     if (on && slot < kSortMost) work.lists.entry[slot] = e;
   };
-  constexpr int kFlight = 4, kAt = kThreads / 16;  // spans of a thread in flight, of all threads
   for (int i0 = 0; i0 < spans; i0 += kFlight * kAt) {
-    int n[kFlight];
-    u64 e[kFlight];
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const int i = i0 + f * kAt + threadIdx.x / 16, at = min(i, spans - 1);
-      n[f] = i < spans ? records[at].count : 0;
-      e[f] = lists[(long long)at * kListMost + threadIdx.x % 16];
-    }
+    if (i0 > 0) fetch(i0);
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
       const int i = min(i0 + f * kAt + (int)threadIdx.x / 16, spans - 1);
-      take(e[f], (int)threadIdx.x % 16 < n[f]);
-      for (int j = threadIdx.x % 16 + 16; __any(j < n[f]); j += 16)
-        take(j < n[f] ? lists[(long long)i * kListMost + j] : 0, j < n[f]);
+      take(e[f], (int)threadIdx.x % 16 < count[f]);
+      for (int j = threadIdx.x % 16 + 16; __any(j < count[f]); j += 16)
+        take(j < count[f] ? lists[(long long)i * kListMost + j] : 0, j < count[f]);
     }
   }
   double whole = 0.0;  // the row's weight, in units
@@ -744,9 +788,10 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     whole = ldexp(whole, c.unit_log - kSpanUnit);
   }
   __syncthreads();
-  const int n = m.n;
+  int n = m.n;
   const bool complete = tau <= kNothing + 1;  // all that is not -inf is on the lists
   bool found = n > 0 && n <= kSortMost;
+  if (count_cut && n > 64 && n > rule.top_k && n <= kKeysMost) n = largest_of(work.lists, m, n, rule.top_k);
   if (found && n <= kFew) {
     if (choose_few(work.lists, m, c, r, rule, sc, n, whole, complete)) return true;
     found = false;
@@ -827,9 +872,9 @@ __device__ __forceinline__ bool binned(const SampleRule& rule, int vocab) {
   return !by_count(rule, vocab) && !(by_weight(rule) && rule.min_p > 0.0f);
 }
 // Descending with x; a weight of 0 falls into the last.
+__device__ __forceinline__ float bins_per(const Scale& s) { return (float)(s.per * (kBins / 50.0)); }
 __device__ __forceinline__ int bin_of(const Scale& s, float x) {
-  const float d = s.m - x, g = (float)(s.per * (kBins / 50.0));
-  return x == s.m ? 0 : (int)fminf(d * g, (float)(kBins - 1));
+  return x == s.m ? 0 : (int)fminf((s.m - x) * bins_per(s), (float)(kBins - 1));
 }
 
 // hist (LDS): the weights of a chunk's tokens, of those that min_p leaves.
@@ -878,21 +923,31 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     __syncthreads();
     cut = m.pick;
     const u64 want = m.want;
-    // 16 logits a thread at a time
+    // eight logits a thread at a time, by bin_of's comparison without its rounding; few of them are in the bin
+    const float from = (float)cut, to = cut == kBins - 1 ? INFINITY : from + 1.0f, g = bins_per(sc), same = cut == 0 ? sc.m : NAN;
+    float x[8], next[8];
+    load_eight(c, row, 8 * threadIdx.x, x);
 #pragma unroll 1
-    for (int at = 4 * threadIdx.x; at < c.vocab; at += 16 * kThreads) {
-      float x[4][4];
+    for (int at = 8 * threadIdx.x; at < c.vocab; at += 8 * kThreads) {
+      if (at + 8 * kThreads < c.vocab) load_eight(c, row, at + 8 * kThreads, next);
+      bool any = false;
 #pragma unroll
-      for (int f = 0; f < 4; ++f) load_four(c, row, at + 4 * kThreads * f, x[f]);
-#pragma unroll
-      for (int f = 0; f < 4; ++f)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (bin_of(sc, x[f][e]) == cut && x[f][e] > -INFINITY) {
+      for (int e = 0; e < 8; ++e) {
+        const float v = (sc.m - x[e]) * g;
+        any |= (v >= from && v < to) || x[e] == same;
+      }
+      if (any) {
+        int i = at;
+        each(x, [&](float t) {
+          if (t > -INFINITY && bin_of(sc, t) == cut) {
             const int slot = atomicAdd(&m.n, 1);
-            if (slot < kSortMost)
-              work.lists.entry[slot] = (u64)key_of(x[f][e]) << 32 | (0xffffffffu - (unsigned)(at + 4 * kThreads * f + e));
+            if (slot < kSortMost) work.lists.entry[slot] = (u64)key_of(t) << 32 | (0xffffffffu - (unsigned)i);
           }
+          ++i;
+        });
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = next[e];
     }
     __syncthreads();
     const int n = m.n;
@@ -906,13 +961,16 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
       if ((int)threadIdx.x < n)
         work.lists.weight[threadIdx.x] = units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[threadIdx.x] >> 32))));
       __syncthreads();
-      const int i = threadIdx.x / 4, part = threadIdx.x % 4;
+      const int log = few_log(n), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
       if (i < n) {
         const u64 own = work.lists.entry[i];
         u64 above = 0;
-#pragma unroll 4
-        for (int j = part; j < n; j += 4) above += work.lists.entry[j] > own ? work.lists.weight[j] : 0;
-        above = of_four(above);
+#pragma unroll 1
+        for (int j = part; j < n; j += parts) {
+          const u64 w = work.lists.weight[j];
+          above += work.lists.entry[j] > own ? w : 0;
+        }
+        above = over_parts(above, log);
         // the first entry that reaches the target is the last to stay
         if (part == 0 && above < want && above + work.lists.weight[i] >= want) m.want = own;
       }
