@@ -60,6 +60,12 @@ __device__ __forceinline__ double weight_of(const Scale& s, float x) {
   p = fma(r, p, 1.0);
   return ldexp(p, -(int)n);
 }
+// A key below which no token reaches min_p of the largest's weight (v_log_f32 is right to 2^-20 here; what it may be off by is taken off
+// many times over), or 0.
+__device__ __forceinline__ unsigned least_key(const SampleRule& rule, const Scale& s) {
+  const double t = -(double)__builtin_amdgcn_logf(rule.min_p), x = (double)s.m - (t + 1e-4 * (t + 1.0)) / s.per;
+  return fabs(x) < 3e38 ? key_of((float)x - 1e-6f * fabsf((float)x)) - 1 : 0;
+}
 // In units: 2^52 is added, which leaves the whole number in the low bits (U <= 51).
 __device__ __forceinline__ u64 units(const Scale& s, double w) {
   return __builtin_bit_cast(u64, ldexp(w, s.unit_log) + 0x1p52) - 0x4330000000000000ull;
@@ -68,7 +74,7 @@ __device__ __forceinline__ u64 units(const Scale& s, double w) {
 // ---- sums over a workgroup ----
 // A workgroup goes through most of its code once, and much of its time is the fetching of that code.  So what a thread has several
 // of goes through loops in turn, with one copy of weight_of in each (16 rows of 50021 logits, 4900 of them finite, top_p 0.98: the
-// last step takes 25 us, and 48 with the loops unrolled and eight weights a thread in scratch memory).
+// last step takes 24 us, and 48 with the loops unrolled and eight weights a thread in scratch memory).
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
 
 __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {  // inclusive
@@ -313,7 +319,7 @@ __device__ void general_row(General& s, Sums& sums, const SampleCall& c, long lo
 // row's tokens from the largest such bound of any wavefront on (`tau`) then are on lists, and where the rule's cuts are found
 // among them, they alone decide.  Where they are not (flat rows with a top_p near 1, thousands of equal logits),
 // general_row does.
-constexpr int kSpan = 512, kListMost = 128, kSortMost = 2048;
+constexpr int kSpan = 512, kListMost = 128, kListedMost = 2048;
 constexpr int kSpanUnit = 51;  // 512 weights in units of 2^-51 stay below 2^61
 
 struct Record {
@@ -322,10 +328,17 @@ struct Record {
   u64 weight;
 };
 
-// How many of a wavefront's lanes are to hold a token from tau on: the largest of the wavefronts' bounds then leaves a good deal more
-// than top_k tokens of the row, or some hundreds.
+// Does the top_k-th largest of the spans' largest logits bound the row's top_k largest?
+constexpr int kTopsMost = 512;
+__device__ __forceinline__ bool tops_tell(const SampleRule& rule, int vocab, int spans) {
+  return by_count(rule, vocab) && rule.top_k < spans && spans <= kTopsMost;
+}
+// How many of a wavefront's lanes are to hold a token from tau on: top_k where the spans' largest bound what is taken of them (so
+// up to 32 of the row's top_k may lie in one span); else the largest of the wavefronts' bounds leaves a good deal more than top_k
+// tokens of the row, or some hundreds.
 __device__ __forceinline__ int list_rank(const SampleRule& rule, int vocab, int spans) {
   if (one_token(rule)) return 1;
+  if (tops_tell(rule, vocab, spans)) return min(32, max(8, rule.top_k));
   if (by_count(rule, vocab)) return (int)min(48LL, 5 + (4LL * rule.top_k + spans - 1) / spans);
   return min(32, max(8, 1024 / spans));
 }
@@ -429,19 +442,10 @@ __device__ __forceinline__ void list_span(const SampleCall& c, const float* row,
   if (lane == 0) *record = {top, count > kListMost ? 0xffffffffu : tau, min(count, kListMost), first, sum};
 }
 
-// Of lane ^ D, without LDS: rotations and mirrors within 16 lanes, exchanges of 16 and of 32.
+// Of lane ^ D, without LDS: exchanges, mirrors and a rotation within 16 lanes.
 template <int D>
 __device__ __forceinline__ unsigned across(unsigned v) {
   constexpr int kCtrl = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x128;
-  if constexpr (D == 16 || D == 32) {
-    typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
-    u32x2 o;
-    if constexpr (D == 16)
-      o = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane16_swap(v, v, false, false));
-    else
-      o = __builtin_bit_cast(u32x2, __builtin_amdgcn_permlane32_swap(v, v, false, false));
-    return threadIdx.x & D ? o[0] : o[1];
-  }
   v = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, 0xF, 0xF, true);
   if constexpr (D == 4) v = (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x1B, 0xF, 0xF, true);  // (a mirror of 8, then of 4)
   return v;
@@ -450,63 +454,12 @@ template <int D>
 __device__ __forceinline__ u64 across(u64 v) {
   return (u64)across<D>((unsigned)(v >> 32)) << 32 | across<D>((unsigned)v);
 }
-// One step of a bitonic sort: the larger of a pair to the lower place where `down`.
-template <int D>
-__device__ __forceinline__ void step(u64& v, int i, bool down) {
-  const u64 o = across<D>(v);
-  const bool lower = (i & D) == 0;
-  v = (lower == down) == (v > o) ? v : o;
-}
-// a[0 .. n) descending, n a power of two from 64 to kSortMost.  A thread holds the entries t and t + kThreads; pairs of one
-// wavefront meet in registers, others in LDS.
-__device__ void sort_descending(u64* a, int n) {
-  __syncthreads();
-  const int t = threadIdx.x;
-  u64 v[2] = {t < n ? a[t] : 0, t + kThreads < n ? a[t + kThreads] : 0};
-  for (int k = 2; k <= n; k *= 2) {
-    for (int j = k / 2; j >= 64; j /= 2) {
-      if (j == kThreads) {
-        const u64 x = max(v[0], v[1]);
-        v[1] = min(v[0], v[1]);
-        v[0] = x;
-        continue;
-      }
-      __syncthreads();
-      if (t < n) a[t] = v[0];
-      if (t + kThreads < n) a[t + kThreads] = v[1];
-      __syncthreads();
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int i = t + e * kThreads;
-        if (i < n) {
-          const u64 o = a[i ^ j];
-          v[e] = (((i & j) == 0) == ((i & k) == 0)) == (v[e] > o) ? v[e] : o;
-        }
-      }
-    }
-    const int most = min(32, k / 2);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int i = t + e * kThreads;
-      if (i >= n) continue;  // (whole wavefronts)
-      const bool down = (i & k) == 0;
-      if (most >= 32) step<32>(v[e], i, down);
-      if (most >= 16) step<16>(v[e], i, down);
-      if (most >= 8) step<8>(v[e], i, down);
-      if (most >= 4) step<4>(v[e], i, down);
-      if (most >= 2) step<2>(v[e], i, down);
-      step<1>(v[e], i, down);
-    }
-  }
-  __syncthreads();
-  if (t < n) a[t] = v[0];
-  if (t + kThreads < n) a[t + kThreads] = v[1];
-  __syncthreads();
-}
-__device__ __forceinline__ int power_of_two(int n) { return n <= 64 ? 64 : 1 << (32 - __clz(n - 1)); }
 
+constexpr int kFew = kThreads / 4, kSlots = kThreads;
 struct Lists {
-  u64 entry[kSortMost], weight[kSortMost];
+  u64 entry[kListedMost], weight[kListedMost];
+  u64 slot[kSlots];
+  u64 few[kFew], few_value[kFew];
 };
 union Work {
   General general;
@@ -515,6 +468,7 @@ union Work {
 struct Common {
   Sums sums;
   int n, pick, large;
+  unsigned least;
   double before;
   u64 want;
   u64 chunk[kThreads];
@@ -600,7 +554,6 @@ __device__ void draw_span(Common& m, const SampleCall& c, long long r, const Sam
 // The choice from all of a few tokens, without a sort: 4 to 16 threads a token compare it with the others.  Its place and the weight
 // before it decide whether it stays, and the weight of the tokens with lower indexes whether it is drawn.  `whole`: the row's
 // weight where only a weight cuts; complete: nothing else is in the row.  False if the tokens do not tell.
-constexpr int kFew = kThreads / 4;
 __device__ __forceinline__ int few_log(int n) { return n <= kThreads / 16 ? 4 : n <= kThreads / 8 ? 3 : n <= kThreads / 4 ? 2 : 1; }
 template <typename T>
 __device__ __forceinline__ T over_parts(T v, int log) {
@@ -665,7 +618,7 @@ __device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const Sample
 }
 
 // Of n entries those with fewer than k larger logits above them; how many that are.  Comparing keys alone, two operations a pair, it
-// spares choose_few most of its pairs (191 entries, k = 40: a call of one row 17.8 -> 14.5 us).
+// spares choose_few most of its pairs (191 entries, k = 40: a call of one row 16.1 -> 12.8 us).
 constexpr int kKeysMost = kThreads / 2;
 __device__ __forceinline__ int largest_of(Lists& lists, Common& m, int n, int k) {
   unsigned* keys = reinterpret_cast<unsigned*>(lists.weight);
@@ -697,21 +650,188 @@ __device__ __forceinline__ int largest_of(Lists& lists, Common& m, int n, int k)
   return m.pick;
 }
 
+// Entries in kSlots bins of their logits, evenly from the largest down; never descending with the logit, whatever the numbers.
+struct Bins {
+  float m, per, from;
+};
+__device__ __forceinline__ int slot_of(const Bins& b, u64 entry) {
+  const float x = logit_of((unsigned)(entry >> 32));
+  return x == b.m ? 0 : (int)fminf(fmaxf((b.m - x) * b.per - b.from, 0.0f), (float)(kSlots - 1));
+}
+// Of n entries with their weights those that are at least `floor`, in descending order: the one with which their weights (or, counts:
+// their number) reach `target`, 0 if they do not.  The bins tell between which it lies, one bin's are compared with
+// each other.  False if those are too many.
+__device__ bool list_cut(Lists& lists, Common& m, const Bins& bins, int n, u64 floor, bool counts, u64 target, u64& last) {
+  __syncthreads();
+  lists.slot[threadIdx.x] = 0;
+  if (threadIdx.x == 0) {
+    m.pick = n <= kFew ? 0 : -1;  // few entries are one bin
+    m.large = 0;
+    m.want = target;
+  }
+  __syncthreads();
+  if (n > kFew) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const u64 e = lists.entry[i], w = counts ? 1 : lists.weight[i];
+      if (e >= floor) atomicAdd(&lists.slot[slot_of(bins, e)], w);
+    }
+    __syncthreads();
+    const u64 own = lists.slot[threadIdx.x];
+    u64 all;
+    const u64 before = block_scan(m.sums, own, all);
+    if (before < target && before + own >= target) {
+      m.pick = threadIdx.x;
+      m.want = target - before;
+    }
+    __syncthreads();
+  }
+  const int at = m.pick;
+  const u64 want = m.want;
+  last = 0;
+  if (at < 0) return true;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const u64 e = lists.entry[i];
+    if (e >= floor && (n <= kFew || slot_of(bins, e) == at)) {
+      const int to = atomicAdd(&m.large, 1);
+      if (to < kFew) {
+        lists.few[to] = e;
+        lists.few_value[to] = counts ? 1 : lists.weight[i];
+      }
+    }
+  }
+  __syncthreads();
+  const int few = m.large;
+  if (few > kFew) return false;
+  if (threadIdx.x == 0) m.want = 0;
+  __syncthreads();
+  const int log = few_log(few), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
+  if (i < few) {
+    const u64 mine = lists.few[i];
+    u64 above = 0;
+#pragma unroll 1
+    for (int j = part; j < few; j += parts) {
+      const u64 w = lists.few_value[j];
+      above += lists.few[j] > mine ? w : 0;
+    }
+    above = over_parts(above, log);
+    if (part == 0 && above < want && above + lists.few_value[i] >= want) m.want = mine;
+  }
+  __syncthreads();
+  last = m.want;
+  return true;
+}
+// The draw from the entries that are at least `last`: bins of their indexes tell between which it falls.
+__device__ bool list_draw(Lists& lists, Common& m, const SampleCall& c, long long r, int n, u64 last) {
+  const int shift = max(0, 22 - __clz(c.vocab - 1 | 1));  // kSlots parts of the row
+  __syncthreads();
+  lists.slot[threadIdx.x] = 0;
+  if (threadIdx.x == 0) m.large = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const u64 e = lists.entry[i];
+    if (e >= last) atomicAdd(&lists.slot[(0xffffffffu - (unsigned)e) >> shift], lists.weight[i]);
+  }
+  __syncthreads();
+  const u64 own = lists.slot[threadIdx.x];
+  u64 all;
+  const u64 before = block_scan(m.sums, own, all), target = draw_units(c, r, all);
+  if (target >= before && target < before + own) {
+    m.pick = threadIdx.x;
+    m.want = target - before;
+  }
+  __syncthreads();
+  const unsigned at = (unsigned)m.pick;
+  const u64 want = m.want;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const u64 e = lists.entry[i];
+    if (e >= last && (0xffffffffu - (unsigned)e) >> shift == at) {
+      const int to = atomicAdd(&m.large, 1);
+      if (to < kFew) {
+        lists.few[to] = e;
+        lists.few_value[to] = lists.weight[i];
+      }
+    }
+  }
+  __syncthreads();
+  const int few = m.large, log = few_log(few), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
+  if (few > kFew) return false;
+  if (i < few) {
+    const u64 mine = lists.few[i], weight = lists.few_value[i];
+    u64 below = 0;
+#pragma unroll 1
+    for (int j = part; j < few; j += parts) {
+      const u64 w = lists.few_value[j];
+      below += (unsigned)lists.few[j] > (unsigned)mine ? w : 0;
+    }
+    below = over_parts(below, log);
+    if (part == 0 && want >= below && want < below + weight)
+      answer(c, r, (int)(0xffffffffu - (unsigned)mine), (double)weight / (double)all);
+  }
+  return true;
+}
+// choose_few for up to kListedMost tokens, none below key `tau`.
+__device__ __forceinline__ bool choose_many(Lists& lists, Common& m, const SampleCall& c, long long r, const SampleRule& rule,
+                                            const Scale& sc, int n, unsigned tau, double whole, bool complete) {
+  const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
+  if (count_cut && !complete && n < rule.top_k) return false;
+  if (threadIdx.x == 0) m.least = 0xffffffffu;
+  __syncthreads();
+  u64 mine = 0, listed;
+#pragma unroll 1
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const unsigned key = (unsigned)(lists.entry[i] >> 32);
+    const double real = weight_of(sc, logit_of(key));
+    mine += lists.weight[i] = units(sc, real);
+    if (sc.min_p > 0.0) {
+      if (real >= sc.min_p)
+        atomicMin(&m.least, key);
+      else
+        m.large = 1;
+    }
+  }
+  block_scan(m.sums, mine, listed);
+  const unsigned least = m.least;
+  const bool short_of_min = sc.min_p > 0.0 && (complete || m.large > 0);
+  if (!count_cut && !short_of_min && !(weight_cut && (complete || listed >= part_units(rule, whole)))) return false;
+  const Bins bins{sc.m, (float)kSlots / (sc.m - logit_of(tau)), 0.0f};
+  u64 last = 0, more = 0;
+  if (count_cut && n > rule.top_k) {
+    if (!list_cut(lists, m, bins, n, 0, true, rule.top_k, last)) return false;
+    if (weight_cut) {
+      mine = 0;
+      for (int i = threadIdx.x; i < n; i += kThreads) mine += lists.entry[i] >= last ? lists.weight[i] : 0;
+      block_scan(m.sums, mine, listed);
+    }
+  }
+  if (weight_cut) {
+    if (!list_cut(lists, m, bins, n, last, false, part_units(rule, count_cut ? (double)listed : whole), more)) return false;
+    last = max(last, more);
+  }
+  if (sc.min_p > 0.0) last = max(last, (u64)least << 32);
+  return list_draw(lists, m, c, r, n, last);
+}
+
 // A row's token from its records and lists (list of span i at lists + i * kListMost).  False if they do not tell; `top`: the
 // largest logit's key.
 __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, int spans, const Record* records,
                        const u64* lists, unsigned& top) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  // the beginnings of the lists, 16 lanes a span
-  constexpr int kFlight = 4, kAt = kThreads / 16;  // spans of a thread in flight, of all threads
+  // the beginnings of the lists, 16 lanes a span: of up to four spans a thread, or more of fewer
+  constexpr int kFlight = 4, kAt = kThreads / 16;
+  const int glog = spans <= kAt ? 0 : spans <= 2 * kAt ? 1 : 2, j0 = threadIdx.x % 16, rounds = kFlight >> glog;
   int count[kFlight];
   u64 e[kFlight];
+  auto span_at = [&](int i0, int f) { return i0 + (f & ((1 << glog) - 1)) * kAt + (int)threadIdx.x / 16; };
   auto fetch = [&](int i0) {
 #pragma unroll
     for (int f = 0; f < kFlight; ++f) {
-      const int i = i0 + f * kAt + threadIdx.x / 16, at = min(i, spans - 1);
+      const int i = span_at(i0, f), at = min(i, spans - 1);
       count[f] = i < spans ? records[at].count : 0;
-      e[f] = lists[(long long)at * kListMost + threadIdx.x % 16];
+      e[f] = lists[(long long)at * kListMost + j0 + 16 * (f >> glog)];
     }
   };
   fetch(0);
@@ -723,6 +843,7 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     best = max(best, (u64)q.top << 32 | (0xffffffffu - (unsigned)q.first));
     tau = max(tau, q.tau);
   }
+  const unsigned mine = (unsigned)(best >> 32);
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
     best = max(best, __shfl_xor(best, d));
@@ -732,6 +853,9 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     m.sums[0][wave] = best;
     m.sums[1][wave] = tau;
   }
+  unsigned* tops = reinterpret_cast<unsigned*>(work.lists.slot);
+  const bool by_tops = tops_tell(rule, c.vocab, spans);
+  if (by_tops && (int)threadIdx.x < kTopsMost) tops[threadIdx.x] = (int)threadIdx.x < spans ? mine : 0;
   if (threadIdx.x == 0) m.n = m.large = 0;
   __syncthreads();
 #pragma unroll
@@ -739,8 +863,30 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     best = max(best, m.sums[0][i]);
     tau = max(tau, (unsigned)m.sums[1][i]);
   }
-  __syncthreads();
   top = (unsigned)(best >> 32);
+  // as few tokens as hold all that can stay: from the top_k-th largest of the spans' largest on (its upper half), or from min_p on
+  if (by_tops) {
+    if (wave == 0) {
+      unsigned v[kTopsMost / 64], from = 0;
+#pragma unroll
+      for (int f = 0; f < kTopsMost / 64; ++f) v[f] = tops[64 * f + lane];
+      const int differ = 31 - __clz((int)((tau ^ top) | 1u));  // above it any bound from tau on is as top
+      from = differ < 31 ? top >> (differ + 1) << (differ + 1) : 0;
+#pragma unroll 1
+      for (int bit = differ; bit >= 16; --bit) {
+        const unsigned next = from | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int f = 0; f < kTopsMost / 64; ++f)
+          if (64 * f < spans) n += __popcll(__ballot(v[f] >= next));
+        if (n >= rule.top_k) from = next;
+      }
+      if (lane == 0) m.least = from;
+    }
+    __syncthreads();
+    tau = max(tau, m.least);
+  }
+  __syncthreads();
   if (top == kNothing || one_token(rule)) {
     if (threadIdx.x == 0) {
       const bool any = top != kNothing;
@@ -754,6 +900,12 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     draw_span(m, c, r, rule, sc, spans, records);
     return true;
   }
+  bool covers_min = false;
+  if (sc.min_p > 0.0 && !count_cut) {
+    const unsigned from = least_key(rule, sc);
+    covers_min = from >= tau;
+    tau = max(tau, from);
+  }
   // the lists' tokens from tau on
   auto take = [&](u64 e, bool on) {
     on = on && (unsigned)(e >> 32) >= tau;
@@ -761,16 +913,27 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
     int slot = 0;
     if (lane == 0 && mask) slot = atomicAdd(&m.n, __popcll(mask));
     slot = __shfl(slot, 0) + __popcll(mask & ((1ull << lane) - 1));
-    if (on && slot < kSortMost) work.lists.entry[slot] = e;
+    if (on && slot < kListedMost) work.lists.entry[slot] = e;
   };
-  for (int i0 = 0; i0 < spans; i0 += kFlight * kAt) {
+#pragma unroll 1
+  for (int i0 = 0; i0 < spans; i0 += kAt << glog) {
     if (i0 > 0) fetch(i0);
+    for (int j = j0;; j += 16 * rounds) {
+      u64 now[kFlight];
+      bool on[kFlight], more = false;
 #pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const int i = min(i0 + f * kAt + (int)threadIdx.x / 16, spans - 1);
-      take(e[f], (int)threadIdx.x % 16 < count[f]);
-      for (int j = threadIdx.x % 16 + 16; __any(j < count[f]); j += 16)
-        take(j < count[f] ? lists[(long long)i * kListMost + j] : 0, j < count[f]);
+      for (int f = 0; f < kFlight; ++f) {
+        const int k = j + 16 * (f >> glog), then = k + 16 * rounds;
+        now[f] = e[f];
+        on[f] = k < count[f];
+        if (then < count[f]) {
+          more = true;
+          e[f] = lists[(long long)span_at(i0, f) * kListMost + then];
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < kFlight; ++f) take(now[f], on[f]);
+      if (!__any(more)) break;
     }
   }
   double whole = 0.0;  // the row's weight, in units
@@ -789,75 +952,12 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
   }
   __syncthreads();
   int n = m.n;
-  const bool complete = tau <= kNothing + 1;  // all that is not -inf is on the lists
-  bool found = n > 0 && n <= kSortMost;
+  const bool complete = tau <= kNothing + 1 || covers_min;  // all that can stay is on the lists
+  const bool found = n > 0 && n <= kListedMost;
   if (count_cut && n > 64 && n > rule.top_k && n <= kKeysMost) n = largest_of(work.lists, m, n, rule.top_k);
-  if (found && n <= kFew) {
-    if (choose_few(work.lists, m, c, r, rule, sc, n, whole, complete)) return true;
-    found = false;
-  }
-  if (found && weight_cut && !count_cut && !complete && !(sc.min_p > 0.0)) {  // do the lists reach what top_p asks for?
-    u64 mine = 0, listed;
-#pragma unroll 1
-    for (int i = threadIdx.x; i < n; i += kThreads) mine += units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))));
-    block_scan(m.sums, mine, listed);
-    found = listed >= part_units(rule, whole);
-  }
-  if (found) {
-    const int n2 = power_of_two(n);
-    for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
-    sort_descending(work.lists.entry, n2);
-#pragma unroll 1
-    for (int i = threadIdx.x; i < n2; i += kThreads) {
-      const double real = i < n ? weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))) : 0.0;
-      work.lists.weight[i] = units(sc, real);
-      const int large = __popcll(__ballot(i < n && real >= sc.min_p));
-      if (lane == 0) atomicAdd(&m.large, large);
-    }
-    __syncthreads();
-    // min_p: weights descend, those that are large enough come first; beyond the lists there may be more if all on them are
-    int stay = sc.min_p > 0.0 ? m.large : n;
-    const bool short_of_min = sc.min_p > 0.0 && (complete || stay < n);
-    const int of = count_cut ? min(n, rule.top_k) : n;
-    found = short_of_min && !weight_cut && !count_cut;
-    if (count_cut) {
-      found = complete || n >= rule.top_k;
-      stay = min(stay, of);
-    }
-    if (weight_cut && (found || !count_cut)) {
-      // from here on thread t has the entries 2 t and 2 t + 1
-      const int i0 = 2 * threadIdx.x;
-      const u64 w0 = i0 < of ? work.lists.weight[i0] : 0, w1 = i0 + 1 < of ? work.lists.weight[i0 + 1] : 0;
-      u64 listed;
-      const u64 before = block_scan(m.sums, w0 + w1, listed);
-      const u64 target = part_units(rule, count_cut ? (double)listed : whole);
-      found = count_cut || complete || listed >= target || short_of_min;
-      if (threadIdx.x == 0) m.pick = stay;
-      __syncthreads();
-      // the first entry that reaches the target is the last to stay
-      if (before < target && before + w0 + w1 >= target) atomicMin(&m.pick, before + w0 >= target ? i0 + 1 : i0 + 2);
-      __syncthreads();
-      stay = m.pick;
-    }
-    if (found) {
-      // in index order
-      __syncthreads();
-      const int s2 = power_of_two(stay);
-      for (int i = threadIdx.x; i < s2; i += kThreads)
-        work.lists.entry[i] = i < stay ? work.lists.entry[i] << 32 | (unsigned)i : 0;
-      sort_descending(work.lists.entry, s2);
-      const int i0 = 2 * threadIdx.x;
-      const u64 e0 = i0 < stay ? work.lists.entry[i0] : 0, e1 = i0 + 1 < stay ? work.lists.entry[i0 + 1] : 0;
-      const u64 w0 = i0 < stay ? work.lists.weight[(unsigned)e0] : 0, w1 = i0 + 1 < stay ? work.lists.weight[(unsigned)e1] : 0;
-      u64 left;
-      const u64 before = block_scan(m.sums, w0 + w1, left), target = draw_units(c, r, left);
-      if (target >= before && target < before + w0 + w1) {
-        const bool second = target >= before + w0;
-        answer(c, r, (int)(0xffffffffu - (unsigned)((second ? e1 : e0) >> 32)), (double)(second ? w1 : w0) / (double)left);
-      }
-      return true;
-    }
-  }
+  if (found && n <= kFew ? choose_few(work.lists, m, c, r, rule, sc, n, whole, complete)
+                         : found && choose_many(work.lists, m, c, r, rule, sc, n, tau, whole, complete))
+    return true;
   __syncthreads();
   return false;
 }
@@ -941,7 +1041,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
         each(x, [&](float t) {
           if (t > -INFINITY && bin_of(sc, t) == cut) {
             const int slot = atomicAdd(&m.n, 1);
-            if (slot < kSortMost) work.lists.entry[slot] = (u64)key_of(t) << 32 | (0xffffffffu - (unsigned)i);
+            if (slot < kListedMost) work.lists.entry[slot] = (u64)key_of(t) << 32 | (0xffffffffu - (unsigned)i);
           }
           ++i;
         });
@@ -951,45 +1051,20 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     }
     __syncthreads();
     const int n = m.n;
-    if (n > kSortMost) {
+    if (n > kListedMost) {
       __syncthreads();
       general_row(work.general, m.sums, c, r, rule, sc);
       return;
     }
-    if (threadIdx.x == 0) m.want = 0;
-    if (n <= kFew) {
-      if ((int)threadIdx.x < n)
-        work.lists.weight[threadIdx.x] = units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[threadIdx.x] >> 32))));
-      __syncthreads();
-      const int log = few_log(n), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
-      if (i < n) {
-        const u64 own = work.lists.entry[i];
-        u64 above = 0;
 #pragma unroll 1
-        for (int j = part; j < n; j += parts) {
-          const u64 w = work.lists.weight[j];
-          above += work.lists.entry[j] > own ? w : 0;
-        }
-        above = over_parts(above, log);
-        // the first entry that reaches the target is the last to stay
-        if (part == 0 && above < want && above + work.lists.weight[i] >= want) m.want = own;
-      }
-    } else {
-      const int n2 = power_of_two(n);
-      for (int i = n + threadIdx.x; i < n2; i += kThreads) work.lists.entry[i] = 0;
-      sort_descending(work.lists.entry, n2);
-#pragma unroll 1
-      for (int i = threadIdx.x; i < n2; i += kThreads)
-        work.lists.weight[i] = i < n ? units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32)))) : 0;
+    for (int i = threadIdx.x; i < n; i += kThreads)
+      work.lists.weight[i] = units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))));
+    // (the bin's own kSlots parts)
+    if (!list_cut(work.lists, m, Bins{sc.m, g * (float)kSlots, from * (float)kSlots}, n, 0, false, want, last)) {
       __syncthreads();
-      w0 = i0 < n ? work.lists.weight[i0] : 0;
-      w1 = i0 + 1 < n ? work.lists.weight[i0 + 1] : 0;
-      u64 all;
-      before = block_scan(m.sums, w0 + w1, all);
-      if (before < want && before + w0 + w1 >= want) m.want = work.lists.entry[before + w0 >= want ? i0 : i0 + 1];
+      general_row(work.general, m.sums, c, r, rule, sc);
+      return;
     }
-    __syncthreads();
-    last = m.want;
     stay = n;
   }
   // what stays of each chunk

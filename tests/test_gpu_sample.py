@@ -75,6 +75,35 @@ def test_batches(dev, rows, vocab, rule):
     assert check(x, u, [rule] * rows, out.tokens(), out.probs.to_numpy()) == 0
 
 
+MANY = [Sampling(1.0, k) for k in (2, 20, 50, 200, 255, 256, 257, 700, 2000, 5000)] + [
+    Sampling(0.7, 200, 0.9, 0.01), Sampling(1.0, 600, 0.99), Sampling(1.3, 1500, 0.98, 0.05), Sampling(0.7, 0, 0.9), Sampling(1.0, 0, 0.6),
+    Sampling(0.5, 0, 0.99, 0.001), Sampling(1.0, 0, 1.0, 0.02), Sampling(2.0, 0, 1.0, 1e-4), Sampling(1.0, 0, 0.9, 1e-6)]
+
+
+@pytest.mark.parametrize("kind", ["together", "descending", "ascending", "spread", "few"])
+@pytest.mark.parametrize("vocab", [9000, 33333, 131072, 300001])
+def test_where_the_largest_lie(dev, vocab, kind):
+    """The largest logits in one place, in order, or a few hundred among nothing."""
+    rng = np.random.default_rng(vocab)
+    rows = len(MANY)
+    x = rng.standard_normal((rows, vocab), dtype=np.float32)
+    if kind == "together":
+        x[:, 700:1200] += np.float32(6)
+    if kind in ("descending", "ascending"):
+        x = np.sort(x, axis=1)[:, ::-1 if kind == "descending" else 1].copy()
+    if kind == "spread":
+        x *= np.float32(3)
+    if kind == "few":
+        x[rng.random((rows, vocab)) > 400 / vocab] = -np.inf
+    u = rng.random(rows, dtype=np.float32)
+    out = _t(x, dev).sample(u, MANY)
+    # tokens at a top_p of 0.9 weigh 1e-6 of the whole, those at a min_p of 0.001 lie 5e-8 apart, and slack() is 4e-9 to 2e-8: a row in
+    # some hundred lies within it.  Of these it is (by the model alone) one of 131072 tokens in order, top_p 0.9, 2.9e-9 from
+    # its border, and one of 300001 spread, min_p 1e-4, 5.3e-9 from its.
+    on_border = (vocab == 131072 and kind in ("descending", "ascending")) or (vocab == 300001 and kind == "spread")
+    assert check(x, u, MANY, out.tokens(), out.probs.to_numpy()) == on_border
+
+
 def test_equal_logits_go_by_index(dev):
     """All alike: top_k and top_p take the lowest indexes, and the borders are exact."""
     for vocab in (8, 1000, 30000):
