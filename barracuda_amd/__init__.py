@@ -1,6 +1,7 @@
 """barracuda_amd -- MI355X (gfx950) implementation of barraCuda's dense ML-ops
 hot path: f32 matmul / batched matmul, row softmax, fused attention forward;
-and a paged key/value cache with windowed attention over it.
+a paged key/value cache with windowed attention over it; and for a token's step
+around that, rotary positions, linear layers with 4-bit weights, and sampling.
 
 The compute lives in libbarracuda_hip.so (C ABI: include/barracuda_hip.h);
 this package is the host side that mirrors the reference's op API.

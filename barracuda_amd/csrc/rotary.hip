@@ -24,7 +24,7 @@ using bch::RotaryPlan;
 using bch::SdpaLayout;
 
 constexpr int kThreads = 256;
-constexpr int kHeads = 4;  // heads of a thread in flight
+constexpr int kHeads = 2;  // heads of a thread in flight (4: 8.8 instead of 6.9 us for 16 trees, 1 and 2 alike, 8 10.4)
 
 // cos and sin of t, times scale.  n quarter turns are taken out of t in 64 bits (pi/2 in two parts: t up to 2^31 keeps
 // 2^-50), what remains lies within pi/4 and goes through Taylor's series to x^9 and x^10: off by 2^-28 there, below the
@@ -272,9 +272,11 @@ void plan(Call& c, int vec, long long tokens_each, int heads) {
   const int hn = kThreads >> (c.width_log + c.tn_log);
   c.chunks = (heads + hn - 1) / hn;  // at most; fewer where there are workgroups enough
 }
-// Workgroups enough: eight a CU.  Fewer would leave loads unhidden, more would compute the sines of a token again.
-void share_heads(Call& c, long long blocks) {
-  const long long want = 8LL * bch::device_cu_count();
+// Workgroups enough.  Fewer leave loads unhidden, more compute the sines of a token again: 48 a CU for streams (4 x 32 heads x 2048 rows
+// of 128: 47 us, 54 with 8; a prompt's 10031 tokens of 32 + 2 x 8 heads 91, 95 with 8, 97 with 64), three for small
+// calls (3069 rows of 12 heads of 80 7.7 us, 8.8 with 1, 8.4 with 16).
+void share_heads(Call& c, long long blocks, bool stream) {
+  const long long want = (stream ? 48LL : 3LL) * bch::device_cu_count();
   c.chunks = (int)std::max(1LL, std::min({(long long)c.chunks, (want + blocks - 1) / std::max(1LL, blocks), 65535LL}));
 }
 
@@ -302,7 +304,7 @@ hipError_t launch_rotary(hipStream_t s, int B, int H, int S, int D, const Rotary
   const bool nt = 8.0 * B * S * H * D >= kNtBytes;
   plan(c, vec ? 4 : 1, c.tokens, H);
   const long long blocks = ((c.tokens - 1) >> c.tn_log) + 1;
-  share_heads(c, blocks);
+  share_heads(c, blocks, nt);
   const dim3 grid((unsigned)std::min(blocks, 1LL << 20), c.chunks), block(kThreads);
 #define BCH_ROTARY(V, IL) (nt ? rotary_dense_kernel<V, IL, true> : rotary_dense_kernel<V, IL, false>)
   auto kern = r.interleaved ? (vec ? BCH_ROTARY(4, true) : BCH_ROTARY(1, true))
@@ -344,7 +346,7 @@ hipError_t launch_kv_append_rotary(hipStream_t s, const KvPages& kv, float* k, f
   const bool find = !fits_grid((long long)c.tiles * B, kThreads);
   const long long blocks = find ? ((seqs.total - 1LL) >> c.tn_log) + 1 : (long long)c.tiles * B;
   // of many sequences with room for long chunks most workgroups are empty: the rows that there are count
-  share_heads(c, std::min(blocks, ((seqs.total - 1LL) >> c.tn_log) + 1 + B));
+  share_heads(c, std::min(blocks, ((seqs.total - 1LL) >> c.tn_log) + 1 + B), nt);
 #define BCH_ROTARY(V, IL)                                                                         \
   (find ? (nt ? rotary_append_kernel<V, IL, true, true> : rotary_append_kernel<V, IL, false, true>) \
         : (nt ? rotary_append_kernel<V, IL, true, false> : rotary_append_kernel<V, IL, false, false>))
