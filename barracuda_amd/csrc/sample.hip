@@ -622,6 +622,7 @@ __device__ __forceinline__ bool choose_few(Lists& lists, Common& m, const Sample
 // Of n entries those with fewer than k larger logits above them; how many that are.  Comparing keys alone, two operations a pair, it
 // spares choose_few most of its pairs (191 entries, k = 40: a call of one row 16.1 -> 12.8 us).
 constexpr int kKeysMost = kThreads / 2;
+constexpr int kFewMost = 208;  // about where choose_few, whose time grows with the square, takes the 7 us of choose_many
 __device__ __forceinline__ int largest_of(Lists& lists, Common& m, int n, int k) {
   unsigned* keys = reinterpret_cast<unsigned*>(lists.weight);
   const int log = few_log(n), parts = 1 << log, i = threadIdx.x >> log, part = threadIdx.x & (parts - 1);
@@ -956,8 +957,8 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
   int n = m.n;
   const bool complete = tau <= kNothing + 1 || covers_min;  // all that can stay is on the lists
   const bool found = n > 0 && n <= kListedMost;
-  if (count_cut && n > 64 && n > rule.top_k && n <= kKeysMost) n = largest_of(work.lists, m, n, rule.top_k);
-  if (found && n <= kFew ? choose_few(work.lists, m, c, r, rule, sc, n, whole, complete)
+  if (count_cut && n > 64 && n > rule.top_k && rule.top_k <= 128 && n <= kKeysMost) n = largest_of(work.lists, m, n, rule.top_k);
+  if (found && n <= kFewMost ? choose_few(work.lists, m, c, r, rule, sc, n, whole, complete)
                          : found && choose_many(work.lists, m, c, r, rule, sc, n, tau, whole, complete))
     return true;
   __syncthreads();
