@@ -74,7 +74,7 @@ __device__ __forceinline__ u64 units(const Scale& s, double w) {
 // ---- sums over a workgroup ----
 // A workgroup goes through most of its code once, and much of its time is the fetching of that code.  So what a thread has several
 // of goes through loops in turn, with one copy of weight_of in each (16 rows of 50021 logits, 4900 of them finite, top_p 0.98: the
-// last step takes 24 us, and 48 with the loops unrolled and eight weights a thread in scratch memory).
+// last step took 25 us, and 48 with the loops unrolled and eight weights a thread in scratch memory).
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048;
 
 __device__ __forceinline__ u64 wave_scan(u64 v, int lane) {  // inclusive
@@ -319,8 +319,8 @@ __device__ void general_row(General& s, Sums& sums, const SampleCall& c, long lo
 // row's tokens from the largest such bound of any wavefront on (`tau`) then are on lists, and where the rule's cuts are found
 // among them, they alone decide.  Where they are not, the rows of the next section go on there and others (thousands of equal
 // logits, more than 32 of a top_k's tokens in one span) to general_row.
-// What bounds it (64 rows of 131072): the lists 16.5 us, 500 vector operations a 512 logits, where the stream takes 6; the choice 8 us
-// a row for tens of entries, 14 for some hundreds, exchanges between wavefronts and trips to memory one behind the other.
+// What bounds it (64 rows of 131072): the lists 15.5 us, some 350 vector operations a 512 logits, 80% of the
+// cycles, where the stream takes 6; the choice 8 us a row for tens of entries, 12 to 20 for some hundreds, exchanges between wavefronts and trips to memory one behind the other.
 constexpr int kSpan = 512, kListMost = 128, kListedMost = 2048;
 constexpr int kSpanUnit = 51;  // 512 weights in units of 2^-51 stay below 2^61
 
@@ -342,7 +342,7 @@ __device__ __forceinline__ int list_rank(const SampleRule& rule, int vocab, int 
   if (one_token(rule)) return 1;
   if (tops_tell(rule, vocab, spans)) return min(32, max(8, rule.top_k));
   if (by_count(rule, vocab)) return (int)min(48LL, 5 + (4LL * rule.top_k + spans - 1) / spans);
-  return min(32, max(8, 1024 / spans));
+  return min(32, max(12, 1024 / spans));
 }
 __device__ __forceinline__ bool needs_whole(const SampleRule& rule, int vocab) {
   return !one_token(rule) && !by_count(rule, vocab) && (by_weight(rule) || !(rule.min_p > 0.0f));
@@ -392,6 +392,8 @@ __device__ __forceinline__ int span_index(int base, int e) {
 }
 
 // Span `at` of a row, by one wavefront: its record, and its list (keys in the upper half, 2^32 - 1 - index in the lower).
+// MANY: a launch of many wavefronts, whose code is fetched once for all of them: its weights without a loop.
+template <bool MANY>
 __device__ __forceinline__ void list_span(const SampleCall& c, const float* row, const SampleRule& rule, int spans, int at,
                                           Record* record, u64* list) {
   const int lane = threadIdx.x & 63, base = at * kSpan;
@@ -437,7 +439,12 @@ __device__ __forceinline__ void list_span(const SampleCall& c, const float* row,
   if (needs_whole(rule, c.vocab) && top != kNothing) {
     Scale sc = scale_of(c, rule, logit_of(top));
     sc.unit_log = kSpanUnit;
-    each(x, [&](float v) { sum += units(sc, weight_of(sc, v)); });
+    if constexpr (MANY) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sum += units(sc, weight_of(sc, x[e]));
+    } else {
+      each(x, [&](float v) { sum += units(sc, weight_of(sc, v)); });
+    }
 #pragma unroll 1
     for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   }
@@ -544,13 +551,14 @@ __device__ void draw_span(Common& m, const SampleCall& c, long long r, const Sam
   u64 sum = 0;
   each(x, [&](float v) { sum += units(span, weight_of(span, v)); });
   left -= wave_scan(sum, lane) - sum;
-  if (left >= sum) return;  // also where it has become less than 0
-  each(x, [&](float v) {
-    const u64 w = units(span, weight_of(span, v));
-    if (left < w) answer(c, r, i, (double)w * of / whole);
-    left = left < w ? ~0ull >> 1 : left - w;
-    ++i;
-  });
+  const u64 here = __ballot(left < sum);  // (what has become less than 0 is large)
+  if (!here) return;
+  // and of that lane's eight a lane one
+  const int owner = __ffsll((long long)here) - 1;
+  left = __shfl(left, owner);
+  i = __shfl(i, owner) + lane;
+  const u64 w = lane < 8 && i < c.vocab ? units(span, weight_of(span, clean(c.logits[r * c.stride + i]))) : 0, end = wave_scan(w, lane);
+  if (left < end && left >= end - w) answer(c, r, i, (double)w * of / whole);
 }
 
 // The choice from all of a few tokens, without a sort: 4 to 16 threads a token compare it with the others.  Its place and the weight
@@ -968,8 +976,9 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
 // ---- rows of which thousands of tokens stay ----
 // Where only weights cut a row (top_p or min_p, no top_k), its weights are sorted into kBins bins of their logarithm, a chunk of kChunk
 // logits a workgroup; then one workgroup a row finds the bin that the cut falls into, collects that bin's tokens and cuts among them,
-// and draws: the bins hold each chunk's weight above the cut, so one chunk is read again.  What bounds it: of 24 us for rows of
-// 50021 the collecting takes 6.5 (a CU's share of the memory, whatever the code), the weights of the one chunk 8.
+// and draws: the bins hold each chunk's weight above the cut, so one chunk is read again.  What bounds it: of 20 us for 16 rows of
+// 50021 (23 for one of 131072) the bins' sums take 3, the collecting 4 (7; 17 with eight logits a thread in flight instead of 32), the
+// chunks' sums 2, the weights of the one chunk 5.
 constexpr int kChunk = 8192, kChunksMost = kThreads;
 
 __device__ __forceinline__ bool binned(const SampleRule& rule, int vocab) {
@@ -1000,7 +1009,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
                               const u64* hist) {
   const float* row = c.logits + r * c.stride;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = (c.vocab - 1) / kChunk + 1;
-  if (chunks > kChunksMost) {
+  if (chunks > kChunksMost || c.vocab < 4) {
     general_row(work.general, m.sums, c, r, rule, sc);
     return;
   }
@@ -1023,39 +1032,51 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
       m.pick = second ? i0 + 1 : i0;
       m.want = target - before - (second ? w0 : 0);
     }
-    if (threadIdx.x == 0) m.n = 0;
+    if (threadIdx.x == 0) m.n = m.large = 0;
     __syncthreads();
     cut = m.pick;
     const u64 want = m.want;
-    // eight logits a thread at a time, by bin_of's comparison without its rounding; few of them are in the bin
-    const float from = (float)cut, to = cut == kBins - 1 ? INFINITY : from + 1.0f, g = bins_per(sc), same = cut == 0 ? sc.m : NAN;
-    float x[8], next[8];
-    load_eight(c, row, 8 * threadIdx.x, x);
+    // 32 logits a thread in flight (a CU has its share of the memory only so); fours that hold one near the bin are noted (its ends as
+    // logits, with room for what bin_of rounds), and then looked at
+    const float g = bins_per(sc), from = (float)cut / g, to = cut == kBins - 1 ? INFINITY : ((float)cut + 1.0f) / g;
+    float low = sc.m - to - 2e-6f * (fabsf(sc.m) + to), high = sc.m - from + 2e-6f * (fabsf(sc.m) + from);
+    low = low == low ? low : -INFINITY;
+    high = high == high ? high : INFINITY;
+    int* near = reinterpret_cast<int*>(work.lists.slot);
+    constexpr int kFours = 8, kNearMost = 2 * kSlots;
+    typedef float f32x4_any __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll 1
-    for (int at = 8 * threadIdx.x; at < c.vocab; at += 8 * kThreads) {
-      if (at + 8 * kThreads < c.vocab) load_eight(c, row, at + 8 * kThreads, next);
-      bool any = false;
+    for (int at = 4 * threadIdx.x; at < c.vocab; at += 4 * kThreads * kFours) {
+      f32x4_any x[kFours];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float v = (sc.m - x[e]) * g;
-        any |= (v >= from && v < to) || x[e] == same;
-      }
-      if (any) {
-        int i = at;
-        each(x, [&](float t) {
-          if (t > -INFINITY && bin_of(sc, t) == cut) {
-            const int slot = atomicAdd(&m.n, 1);
-            if (slot < kListedMost) work.lists.entry[slot] = (u64)key_of(t) << 32 | (0xffffffffu - (unsigned)i);
-          }
-          ++i;
-        });
-      }
+      for (int f = 0; f < kFours; ++f)  // (a four that would end behind the row: the row's last, and with them all that it has)
+        x[f] = *reinterpret_cast<const f32x4_any*>(row + min(at + 4 * kThreads * f, c.vocab - 4));
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = next[e];
+      for (int f = 0; f < kFours; ++f) {
+        bool any = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) any |= x[f][e] >= low && x[f][e] <= high;
+        if (any) {
+          const int to = atomicAdd(&m.large, 1);
+          if (to < kNearMost) near[to] = at + 4 * kThreads * f;
+        }
+      }
+    }
+    __syncthreads();
+    const int fours = m.large;
+#pragma unroll 1
+    for (int j = threadIdx.x; j < 4 * min(fours, kNearMost); j += kThreads) {
+      const int i = near[j / 4] + j % 4;
+      if (i >= c.vocab) continue;
+      const float t = clean(row[i]);
+      if (t > -INFINITY && bin_of(sc, t) == cut) {
+        const int to = atomicAdd(&m.n, 1);
+        if (to < kListedMost) work.lists.entry[to] = (u64)key_of(t) << 32 | (0xffffffffu - (unsigned)i);
+      }
     }
     __syncthreads();
     const int n = m.n;
-    if (n > kListedMost) {
+    if (n > kListedMost || fours > kNearMost) {
       __syncthreads();
       general_row(work.general, m.sums, c, r, rule, sc);
       return;
@@ -1064,7 +1085,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     for (int i = threadIdx.x; i < n; i += kThreads)
       work.lists.weight[i] = units(sc, weight_of(sc, logit_of((unsigned)(work.lists.entry[i] >> 32))));
     // (the bin's own kSlots parts)
-    if (!list_cut(work.lists, m, Bins{sc.m, g * (float)kSlots, from * (float)kSlots}, n, 0, false, want, last)) {
+    if (!list_cut(work.lists, m, Bins{sc.m, g * (float)kSlots, (float)cut * (float)kSlots}, n, 0, false, want, last)) {
       __syncthreads();
       general_row(work.general, m.sums, c, r, rule, sc);
       return;
@@ -1108,14 +1129,17 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
   each(x, [&](float t) { sum += weight(t, at++); });
   u64 all;
   const u64 start = block_scan(m.sums, sum, all);
-  if (want < start || want - start >= sum) return;
-  want -= start;
-  each(x, [&](float t) {
-    const u64 w = weight(t, i);
-    if (want < w) answer(c, r, i, (double)w / (double)whole);
-    want = want < w ? ~0ull >> 1 : want - w;
-    ++i;
-  });
+  if (want >= start && want - start < sum) {
+    m.pick = i;
+    m.want = want - start;
+  }
+  __syncthreads();
+  if (wave > 0) return;
+  // and of those eight a lane one
+  i = m.pick + lane;
+  const u64 w = lane < 8 ? weight(i < c.vocab ? clean(row[i]) : -INFINITY, i) : 0, end = wave_scan(w, lane);
+  want = m.want;
+  if (want < end && want >= end - w) answer(c, r, i, (double)w / (double)whole);
 }
 
 // Spans of all rows, four a workgroup.
@@ -1124,7 +1148,7 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleCall c, int span
   const int at = (int)(blockIdx.x % groups) * 4 + (threadIdx.x >> 6);
   if (at >= spans) return;
   const SampleRule rule = c.rules ? c.rules[r] : c.rule;
-  list_span(c, c.logits + r * c.stride, rule, spans, at, records + r * spans + at,
+  list_span<true>(c, c.logits + r * c.stride, rule, spans, at, records + r * spans + at,
             lists + (r * spans + at) * kListMost);
 }
 // later: rows that the lists do not tell are left to the next two kernels where their rule allows; left[r]: the largest logit's key,
@@ -1174,7 +1198,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int 
   const SampleRule rule = c.rules ? c.rules[r] : c.rule;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   if (spans <= kWaves) {
-    if (wave < spans) list_span(c, row, rule, spans, wave, &records[wave], &lists[wave * kListMost]);
+    if (wave < spans) list_span<false>(c, row, rule, spans, wave, &records[wave], &lists[wave * kListMost]);
     __syncthreads();
     unsigned top;
     if (choose(work, common, c, r, rule, spans, records, lists, top)) return;
