@@ -337,12 +337,13 @@ __device__ __forceinline__ bool tops_tell(const SampleRule& rule, int vocab, int
 }
 // How many of a wavefront's lanes are to hold a token from tau on: top_k where the spans' largest bound what is taken of them (so
 // up to 32 of the row's top_k may lie in one span); else the largest of the wavefronts' bounds leaves a good deal more than top_k
-// tokens of the row, or some hundreds.
+// tokens of the row, or, where there is no top_k, 1000 to 1500 of any number of spans (of independent logits; more than kListedMost
+// would be of no use).
 __device__ __forceinline__ int list_rank(const SampleRule& rule, int vocab, int spans) {
   if (one_token(rule)) return 1;
   if (tops_tell(rule, vocab, spans)) return min(32, max(8, rule.top_k));
   if (by_count(rule, vocab)) return (int)min(48LL, 5 + (4LL * rule.top_k + spans - 1) / spans);
-  return min(32, max(12, 1024 / spans));
+  return min(32, max(4, (int)(192.0f * __builtin_amdgcn_rsqf((float)spans))));
 }
 __device__ __forceinline__ bool needs_whole(const SampleRule& rule, int vocab) {
   return !one_token(rule) && !by_count(rule, vocab) && (by_weight(rule) || !(rule.min_p > 0.0f));
