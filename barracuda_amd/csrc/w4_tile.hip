@@ -17,37 +17,41 @@ using bch::W4;
 
 // ---- x into parts ----
 // Part p, inputs 8 o .. 8 o + 7 of row r: 16 bytes at ((p octets + o) rows + r): neighbouring rows lie together, as the matrix
-// cores take them.  A workgroup has 8 rows; a thread every 64th octet of one.
-constexpr int kSplitThreads = 512, kSplitRows = 8, kSplitHeld = 8;
+// cores take them.  A workgroup has ROWS rows, and a row THREADS / ROWS threads in turn: eight rows store whole lines of 128 bytes
+// (2048 rows of 4096: 15 us), four have four times the threads where few rows leave CUs idle (65 rows, 11008 -> 4096: a
+// call 66 us, 80 by eights).
+constexpr int kSplitRows = 8, kSplitHeld = 8;
 
-__global__ __launch_bounds__(kSplitThreads) void w4_split_kernel(int m, int k, int octets, int rows, const float* __restrict__ x,
-                                                                 long long ldx, bool vec, u32x4* parts, int* exponent) {
-  __shared__ unsigned tops[8][8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rr = threadIdx.x & 7, o0 = threadIdx.x >> 3;
-  const int r = blockIdx.x * kSplitRows + rr;
+template <int ROWS, int THREADS>
+__global__ __launch_bounds__(THREADS) void w4_split_kernel(int m, int k, int octets, int rows, const float* __restrict__ x,
+                                                           long long ldx, bool vec, u32x4* parts, int* exponent) {
+  constexpr int kStep = THREADS / ROWS;
+  __shared__ unsigned tops[THREADS / 64][ROWS];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rr = threadIdx.x % ROWS, o0 = threadIdx.x / ROWS;
+  const int r = blockIdx.x * ROWS + rr;
   const float* row = x + min(r, m - 1) * ldx;
   float held[kSplitHeld][8];
   unsigned top = 0;
 #pragma unroll
   for (int h = 0; h < kSplitHeld; ++h) {
-    if (o0 + 64 * h < octets) {
-      bch::w4_load8(held[h], row, 8 * (o0 + 64 * h), k, vec);
+    if (o0 + kStep * h < octets) {
+      bch::w4_load8(held[h], row, 8 * (o0 + kStep * h), k, vec);
       top = bch::w4_top(held[h], top);
     }
   }
-  for (int o = o0 + 64 * kSplitHeld; o < octets; o += 64) {
+  for (int o = o0 + kStep * kSplitHeld; o < octets; o += kStep) {
     float v[8];
     bch::w4_load8(v, row, 8 * o, k, vec);
     top = bch::w4_top(v, top);
   }
 #pragma unroll
-  for (int d = 8; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
-  if (lane < 8) tops[wave][lane] = top;
+  for (int d = ROWS; d < 64; d *= 2) top = max(top, (unsigned)__shfl_xor((int)top, d));
+  if (lane < ROWS) tops[wave][lane] = top;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < 8; ++w) top = max(top, tops[w][rr]);
+  for (int w = 0; w < THREADS / 64; ++w) top = max(top, tops[w][rr]);
   const int e = bch::w4_exponent(top);
-  if (threadIdx.x < 8 && r < m) exponent[r] = bch::kW4Unit - e;
+  if ((int)threadIdx.x < ROWS && r < m) exponent[r] = bch::kW4Unit - e;
   auto put = [&](const float (&v)[8], int o) {
     u32x4 p[3];
     bch::w4_split(v, e, p);
@@ -56,8 +60,8 @@ __global__ __launch_bounds__(kSplitThreads) void w4_split_kernel(int m, int k, i
   };
 #pragma unroll
   for (int h = 0; h < kSplitHeld; ++h)
-    if (o0 + 64 * h < octets) put(held[h], o0 + 64 * h);
-  for (int o = o0 + 64 * kSplitHeld; o < octets; o += 64) {
+    if (o0 + kStep * h < octets) put(held[h], o0 + kStep * h);
+  for (int o = o0 + kStep * kSplitHeld; o < octets; o += kStep) {
     float v[8];
     bch::w4_load8(v, row, 8 * o, k, vec);
     put(v, o);
@@ -69,7 +73,8 @@ __global__ __launch_bounds__(kSplitThreads) void w4_split_kernel(int m, int k, i
 // buffered, [part][octet][row], free of bank conflicts), the codes straight from memory into the wavefront that takes
 // them apart, 128 inputs ahead.
 constexpr int kRows = 128, kCols = 256, kThreads = 512;
-constexpr int kPassBytes = 3 * 4 * kRows * 16;
+constexpr int kPassBytes = 3 * 4 * kRows * 16, kTileBytes = 4 * kRows * kCols;
+static_assert(kTileBytes >= 2 * kPassBytes, "two passes, then the results");
 
 // FL: passes of one group in every 128 inputs (4: the group is a multiple of 128, 2: of 64, 1: of 32).
 template <int FL>
@@ -175,27 +180,42 @@ __global__ __launch_bounds__(kThreads, 2) void w4_tile_kernel(W4 w, int m, int r
 #pragma unroll
       for (int h = 0; h < 2; ++h) codes[b][h] = next[b][h];
   }
+  // out through LDS (the last pass has left it): whole rows of 256, and a loop of few instructions, not 64 times an activation's
+  float* tile = reinterpret_cast<float*>(lds);
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const int o = c0 + 32 * b + l32;
-    if (o >= w.n) continue;
-    const float add = bias ? bias[o] : 0.0f;
-    float* p = partial ? partial + (long long)slice * m * w.n + o : nullptr;
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = r0 + 64 * wm + 32 * i + 8 * (e / 4) + 4 * kh + e % 4;
-        if (r < m) {
-          float v = ldexpf(acc[i][b][e], exponent[r]);
-          if (p) {
-            p[(long long)r * w.n] = v;
-          } else {
-            if (bias) v += add;
-            y[r * ldy + o] = bch::activate(v, act);
-          }
-        }
+      for (int e = 0; e < 16; ++e)
+        tile[(64 * wm + 32 * i + 8 * (e / 4) + 4 * kh + e % 4) * kCols + 64 * wn + 32 * b + l32] = acc[i][b][e];
+  __syncthreads();
+  float* out = partial ? partial + (long long)slice * m * w.n : y;
+  const long long ld = partial ? w.n : ldy;
+  const bool wide = ld % 4 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+#pragma unroll 1
+  for (int j = threadIdx.x; j < kRows * kCols / 4; j += kThreads) {
+    const int r = r0 + j / (kCols / 4), o = c0 - 64 * wn + j % (kCols / 4) * 4;
+    if (r >= m) break;
+    if (o >= w.n) continue;
+    const int up = exponent[r];
+    bch::f32x4 v = *reinterpret_cast<const bch::f32x4*>(tile + 4 * j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = ldexpf(v[e], up);
+      if (!partial) {
+        if (bias && o + e < w.n) v[e] += bias[o + e];
+        v[e] = bch::activate(v[e], act);
       }
+    }
+    float* to = out + r * ld + o;
+    if (wide && o + 3 < w.n) {
+      *reinterpret_cast<bch::f32x4*>(to) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (o + e < w.n) to[e] = v[e];
+    }
   }
 }
 
@@ -207,6 +227,7 @@ __global__ __launch_bounds__(256) void w4_reduce_kernel(int m, int n, int slices
     const long long r = at / n;
     const int o = (int)(at - r * n);
     float v = partial[at];
+#pragma unroll 8
     for (int s = 1; s < slices; ++s) v += partial[s * total + at];
     if (bias) v += bias[o];
     y[r * ldy + o] = bch::activate(v, act);
@@ -228,8 +249,10 @@ hipError_t launch_w4_split(hipStream_t s, int m, const W4& w, const float* x, lo
   const int rows = up(m, kSplitRows), octets = 16 * w.blocks;
   u32x4* p = static_cast<u32x4*>(ws);
   int* e = reinterpret_cast<int*>(p + 3LL * octets * rows);
-  hipLaunchKernelGGL(w4_split_kernel, dim3(rows / kSplitRows), dim3(kSplitThreads), 0, s, m, w.k, octets, rows, x, ldx,
-                     w4_vec(w, x, ldx), p, e);
+  if (rows / kSplitRows < device_cu_count())
+    hipLaunchKernelGGL((w4_split_kernel<4, 1024>), dim3(rows / 4), dim3(1024), 0, s, m, w.k, octets, rows, x, ldx, w4_vec(w, x, ldx), p, e);
+  else
+    hipLaunchKernelGGL((w4_split_kernel<8, 512>), dim3(rows / 8), dim3(512), 0, s, m, w.k, octets, rows, x, ldx, w4_vec(w, x, ldx), p, e);
   *parts = p;
   *exponent = e;
   return hipGetLastError();
@@ -244,18 +267,18 @@ hipError_t launch_w4_reduce(hipStream_t s, int m, int n, int slices, const float
 }
 
 // The slices of inputs: 4.9 us for a round of workgroups and 128 inputs (2048 rows, or 128, 4096 -> 11008), 5 for the sums over
-// the slices and their bytes, written and read, at 4 TB/s.
+// the slices and their bytes, written and read, at 4 TB/s.  Up to 32 of them (65 rows, 11008 -> 4096: 17 slices 50 us, 8 66).
 W4Plan w4_tile_plan(int m, const W4& w, int cus, bool may_split) {
   W4Plan best{0, 1, 0.0};
   const long long tiles = (long long)((m - 1) / kRows + 1) * ((w.n - 1) / kCols + 1);
-  for (int s = 1; s <= (may_split ? 8 : 1) && s <= w.blocks; ++s) {
+  for (int s = 1; s <= (may_split ? 32 : 1) && s <= w.blocks; ++s) {
     const int per = (w.blocks - 1) / s + 1, slices = (w.blocks - 1) / per + 1;
     if (s > 1 && 4.0 * slices * m * w.n > 256e6) break;
     const double c = (double)((tiles * slices - 1) / cus + 1) * per * 4.9 +
                      (slices > 1 ? 5.0 + 2e-6 * slices * m * w.n : 0.0);
     if (best.cost == 0.0 || c < best.cost) best = {0, s, c};
   }
-  best.cost += 8.0 + 1e-6 * 3.5 * m * w.k / 2;
+  best.cost += 3.0 + 1e-6 * 3.5 * m * w.k / 2;
   return best;
 }
 size_t w4_tile_bytes(int m, const W4& w, const W4Plan& p) {
@@ -272,7 +295,9 @@ hipError_t launch_w4_tile(hipStream_t s, int m, const W4& w, const float* x, lon
   const int per = (w.blocks - 1) / p.slices + 1, slices = (w.blocks - 1) / per + 1;
   float* partial = slices > 1 ? reinterpret_cast<float*>(static_cast<char*>(ws) + w4_parts_bytes(m, w)) : nullptr;
   auto kern = w.group % 128 == 0 ? w4_tile_kernel<4> : w.group % 64 == 0 ? w4_tile_kernel<2> : w4_tile_kernel<1>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)mt * nt * slices), dim3(kThreads), 2 * kPassBytes, s, w, m, rows, 16 * w.blocks, parts, exponent,
+  e = ensure_dynamic_lds(reinterpret_cast<const void*>(kern), kTileBytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(kern, dim3((unsigned)mt * nt * slices), dim3(kThreads), kTileBytes, s, w, m, rows, 16 * w.blocks, parts, exponent,
                      bias, act, y, ldy, mt, nt, per, partial);
   e = hipGetLastError();
   if (e != hipSuccess || slices == 1) return e;
