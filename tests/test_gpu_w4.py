@@ -215,6 +215,15 @@ def test_quantized_layer(dev):
         assert np.all(np.abs(got - x.astype(np.float64) @ back.astype(np.float64).T) <= slack(x, back) * (1 + 2.0**-20))
 
 
+@pytest.mark.parametrize("m,n,k,group,zeros,act", [(2050, 20, 5000, 64, True, None), (2056, 36, 4609, 32, False, Activation.ReLU),
+                                                   (70, 24, 20001, 32, True, None), (65, 259, 16392, 128, False, Activation.GELU),
+                                                   (129, 16, 9000, 96, True, None), (300, 1000, 1000, 32, True, Activation.GELU),
+                                                   (65, 64, 40000, 256, False, None), (191, 1030, 2000, 64, False, Activation.ReLU)])
+def test_many_rows(dev, m, n, k, group, zeros, act):
+    """Rows in fours and in eights with more inputs than a workgroup holds, many slices, and columns that do not fill a tile."""
+    check(dev, np.random.default_rng(m + k), m, n, k, group, zeros, bias=True, act=act)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (32, 1024, 8192), (64, 300, 3000), (130, 700, 1024)])
 def test_repeats_bit_for_bit_and_under_capture(dev, m, n, k):
     """The same call gives the same bits; captured on a fresh context (no workspace) it gives them to rounding, at every replay."""
