@@ -1154,8 +1154,8 @@ bch_status bch_kv_keep(bch_ctx* ctx, const bch_kv_pages* kv, int layers, long lo
 
 namespace {
 
-// Outputs of which a grid can have a workgroup of 512 threads for every 16 (fewer than 2^32 threads), and inputs whose blocks' first numbers fit 32 bits.
-constexpr int kW4MaxN = (1 << 27) - 16, kW4MaxK = 0x7fffff00;
+// Outputs of which a grid can have a workgroup of 1024 threads for every 16 (fewer than 2^32 threads), and inputs whose blocks' first numbers fit 32 bits.
+constexpr int kW4MaxN = (1 << 26) - 16, kW4MaxK = 0x7fffff00;
 
 bch_status check_w4(bch_ctx* ctx, const char* op, int n, int k, int group) {
   if (n < 1 || k < 1 || group < 1)

@@ -19,7 +19,10 @@ __device__ __forceinline__ f32x4_t mm16(u32x4 a, u32x4 b, f32x4_t c) {
 }
 
 // ---- one or two rows: f32 multiplications ----
-// A workgroup has 16 outputs, its wavefronts every eighth block of inputs, four of them in flight; x lies in LDS.
+// A workgroup has 16 outputs, its 16 wavefronts every 16th block of inputs, two of them in flight; x lies in LDS.  What bounds it: the
+// launch, the first trip to memory, the codes' stream.  4096 -> 11008, one row and two: 9.1 and 11.2 us, back 9.2 and 10.9; eight
+// wavefronts with four in flight 9.8 and 11.8, back 10.4; 16 with four 12.6 and 14.8 (one workgroup a CU fewer), back 9.5.
+constexpr int kLineThreads = 1024, kLineWaves = 16;
 constexpr int kLineBlocks = 64;  // blocks of x in LDS at a time
 
 // Code e of a word is nibble e / 2 + 4 (e % 2): its byte of the masked word, as a float.
@@ -36,16 +39,16 @@ __device__ __forceinline__ void codes_of(unsigned c, float zero, float (&v)[8]) 
 }
 
 template <int MT, int FL>
-__global__ __launch_bounds__(kThreads) void w4_line_kernel(W4 w, const float* __restrict__ x, long long ldx, bool vec,
+__global__ __launch_bounds__(kLineThreads) void w4_line_kernel(W4 w, const float* __restrict__ x, long long ldx, bool vec,
                                                            const float* __restrict__ bias, int act, float* y, long long ldy) {
   __shared__ float4 xs[MT][kLineBlocks * 32];
-  __shared__ float part[kWaves][MT][16];
+  __shared__ float part[kLineWaves][MT][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, kb = lane >> 4;
   const int tile = blockIdx.x;
   const u32x4* codes = w.codes + (long long)tile * w.blocks * 64 + lane;
   const float* scales = w.scale + (long long)tile * w.groups * 16 + r;
   const unsigned char* zeros = w.zero + (long long)tile * w.groups * 16 + r;
-  constexpr int kFlight = 4, kPer = 4 / FL;  // blocks in flight, groups of one
+  constexpr int kFlight = 2, kPer = 4 / FL;  // blocks in flight, groups of one
   float acc[MT] = {};
   for (int base = 0; base < w.blocks; base += kLineBlocks) {
     const int end = min(w.blocks, base + kLineBlocks);
@@ -54,7 +57,7 @@ __global__ __launch_bounds__(kThreads) void w4_line_kernel(W4 w, const float* __
     auto fetch = [&](int b0) {
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        const int b = min(b0 + kWaves * f, end - 1);
+        const int b = min(b0 + kLineWaves * f, end - 1);
         c[f] = __builtin_nontemporal_load(codes + (long long)b * 64);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -68,14 +71,14 @@ __global__ __launch_bounds__(kThreads) void w4_line_kernel(W4 w, const float* __
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < MT; ++u)
-      for (int i = threadIdx.x; i < (end - base) * 16; i += kThreads) {
+      for (int i = threadIdx.x; i < (end - base) * 16; i += kLineThreads) {
         float v[8];
         bch::w4_load8(v, x + u * ldx, 128 * base + 8 * i, w.k, vec);
         xs[u][2 * i] = make_float4(v[0], v[1], v[2], v[3]);
         xs[u][2 * i + 1] = make_float4(v[4], v[5], v[6], v[7]);
       }
     __syncthreads();
-    for (int b0 = base + wave; b0 < end; b0 += kWaves * kFlight) {
+    for (int b0 = base + wave; b0 < end; b0 += kLineWaves * kFlight) {
       u32x4 cc[kFlight];
       float ss[kFlight][kPer], zz[kFlight][kPer];
 #pragma unroll
@@ -87,10 +90,10 @@ __global__ __launch_bounds__(kThreads) void w4_line_kernel(W4 w, const float* __
           zz[f][i] = z[f][i];
         }
       }
-      if (b0 + kWaves * kFlight < end) fetch(b0 + kWaves * kFlight);
+      if (b0 + kLineWaves * kFlight < end) fetch(b0 + kLineWaves * kFlight);
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        const int b = b0 + kWaves * f;
+        const int b = b0 + kLineWaves * f;
         if (b >= end) break;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -132,7 +135,7 @@ __global__ __launch_bounds__(kThreads) void w4_line_kernel(W4 w, const float* __
     if (o < w.n) {
       float sum = 0.0f;
 #pragma unroll
-      for (int v = 0; v < kWaves; ++v) sum += part[v][u][r];
+      for (int v = 0; v < kLineWaves; ++v) sum += part[v][u][r];
       if (bias) sum += bias[o];
       y[u * ldy + o] = bch::activate(sum, act);
     }
@@ -365,7 +368,7 @@ hipError_t launch_w4_line(hipStream_t s, int m, const W4& w, const float* x, lon
 #define BCH_LINE(M) (w.group % 128 == 0 ? w4_line_kernel<M, 4> : w.group % 64 == 0 ? w4_line_kernel<M, 2> : w4_line_kernel<M, 1>)
   auto kern = m == 1 ? BCH_LINE(1) : BCH_LINE(2);
 #undef BCH_LINE
-  hipLaunchKernelGGL(kern, dim3(w.tiles), dim3(kThreads), 0, s, w, x, ldx, w4_vec(w, x, ldx), bias, act, y, ldy);
+  hipLaunchKernelGGL(kern, dim3(w.tiles), dim3(kLineThreads), 0, s, w, x, ldx, w4_vec(w, x, ldx), bias, act, y, ldy);
   return hipGetLastError();
 }
 

@@ -217,7 +217,7 @@ bch_status bch_w4_bytes(int n, int k, int group, size_t *bytes);
 /* Weights laid out once for bch_w4_linear, all in device memory: codes [n][ld
  * bytes], two inputs a byte, the even one in the low half; scale and zero (a
  * byte each; NULL: 8 everywhere) [n][ceil(k / group)]; out bch_w4_bytes, 16-byte aligned.
- * n <= 2^27 - 16. */
+ * n <= 2^26 - 16. */
 bch_status bch_w4_pack(bch_ctx *ctx, int n, int k, int group,
                        const unsigned char *codes, int ld, const float *scale,
                        const unsigned char *zero, void *out);

@@ -88,10 +88,10 @@ def test_c_refusals():
     size, x, odd = C.c_size_t(), C.c_void_p(64), C.c_void_p(72)
     assert lib.bch_w4_bytes(17, 129, 128, C.byref(size)) == 0 and size.value == 2 * 2 * 1024 + 80 * 2 * 2
     assert lib.bch_w4_bytes(16, 128, 2**31 - 32, C.byref(size)) == 0 and size.value == 1024 + 80
-    assert lib.bch_w4_bytes(2**27 - 16, 4096, 128, C.byref(size)) == 0 and size.value == (2**23 - 1) * 32 * (1024 + 80)
+    assert lib.bch_w4_bytes(2**26 - 16, 4096, 128, C.byref(size)) == 0 and size.value == (2**22 - 1) * 32 * (1024 + 80)
     assert lib.bch_w4_bytes(17, 129, 128, None) == E
     for n, k, g, st in ((0, 1, 32, S), (1, 0, 32, S), (1, 1, 0, S), (-1, 1, 32, S), (1, 1, 33, E), (1, 1, 16, E),
-                        (2**27 - 15, 1, 32, U), (1, 2**31 - 1, 32, U)):
+                        (2**26 - 15, 1, 32, U), (1, 2**31 - 1, 32, U)):
         assert lib.bch_w4_bytes(n, k, g, C.byref(size)) == st, (n, k, g)
         assert lib.bch_w4_pack(None, n, k, g, x, 2**31 - 1, x, None, x) == st, (n, k, g)
         assert lib.bch_w4_linear(None, 1, N.W4(n, k, g, 64), x, 2**31 - 1, None, 0, x, 2**31 - 1) == st, (n, k, g)
