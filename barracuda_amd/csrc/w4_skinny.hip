@@ -19,10 +19,10 @@ __device__ __forceinline__ f32x4_t mm16(u32x4 a, u32x4 b, f32x4_t c) {
 }
 
 // ---- one or two rows: f32 multiplications ----
-// A workgroup has 16 outputs, its 16 wavefronts every 16th block of inputs, two of them in flight; x lies in LDS.  What bounds it: the
-// launch, the first trip to memory, the codes' stream.  4096 -> 11008, one row and two: 9.1 and 11.2 us, back 9.2 and 10.9; eight
-// wavefronts with four in flight 9.8 and 11.8, back 10.4; 16 with four 12.6 and 14.8 (one workgroup a CU fewer), back 9.5.
-constexpr int kLineThreads = 1024, kLineWaves = 16;
+// A workgroup has 16 outputs, its wavefronts every 16th or eighth block of inputs, two of them in flight each; x lies in LDS.  What
+// bounds it: the launch, the first trip to memory, the codes' stream.  One row, 4096 -> 11008 / 50000 and back, us: 16 wavefronts
+// 9.2 / 31 / 9.2, eight 8.9 / 26 / 10.9; two rows 11.2 / 36 / 10.9 and 12.1 / 38 / 12.  So eight where one row has more workgroups than two
+// a CU, else 16.  Four blocks in flight: eight wavefronts 9.8 / 33 / 10.4, 16 12.6 and 9.5.
 constexpr int kLineBlocks = 64;  // blocks of x in LDS at a time
 
 // Code e of a word is nibble e / 2 + 4 (e % 2): its byte of the masked word, as a float.
@@ -38,11 +38,12 @@ __device__ __forceinline__ void codes_of(unsigned c, float zero, float (&v)[8]) 
   }
 }
 
-template <int MT, int FL>
-__global__ __launch_bounds__(kLineThreads) void w4_line_kernel(W4 w, const float* __restrict__ x, long long ldx, bool vec,
+template <int MT, int FL, int THREADS>
+__global__ __launch_bounds__(THREADS) void w4_line_kernel(W4 w, const float* __restrict__ x, long long ldx, bool vec,
                                                            const float* __restrict__ bias, int act, float* y, long long ldy) {
+  constexpr int kOf = THREADS / 64;
   __shared__ float4 xs[MT][kLineBlocks * 32];
-  __shared__ float part[kLineWaves][MT][16];
+  __shared__ float part[kOf][MT][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, kb = lane >> 4;
   const int tile = blockIdx.x;
   const u32x4* codes = w.codes + (long long)tile * w.blocks * 64 + lane;
@@ -57,7 +58,7 @@ __global__ __launch_bounds__(kLineThreads) void w4_line_kernel(W4 w, const float
     auto fetch = [&](int b0) {
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        const int b = min(b0 + kLineWaves * f, end - 1);
+        const int b = min(b0 + kOf * f, end - 1);
         c[f] = __builtin_nontemporal_load(codes + (long long)b * 64);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -71,14 +72,14 @@ __global__ __launch_bounds__(kLineThreads) void w4_line_kernel(W4 w, const float
     __syncthreads();
 #pragma unroll
     for (int u = 0; u < MT; ++u)
-      for (int i = threadIdx.x; i < (end - base) * 16; i += kLineThreads) {
+      for (int i = threadIdx.x; i < (end - base) * 16; i += THREADS) {
         float v[8];
         bch::w4_load8(v, x + u * ldx, 128 * base + 8 * i, w.k, vec);
         xs[u][2 * i] = make_float4(v[0], v[1], v[2], v[3]);
         xs[u][2 * i + 1] = make_float4(v[4], v[5], v[6], v[7]);
       }
     __syncthreads();
-    for (int b0 = base + wave; b0 < end; b0 += kLineWaves * kFlight) {
+    for (int b0 = base + wave; b0 < end; b0 += kOf * kFlight) {
       u32x4 cc[kFlight];
       float ss[kFlight][kPer], zz[kFlight][kPer];
 #pragma unroll
@@ -90,10 +91,10 @@ __global__ __launch_bounds__(kLineThreads) void w4_line_kernel(W4 w, const float
           zz[f][i] = z[f][i];
         }
       }
-      if (b0 + kLineWaves * kFlight < end) fetch(b0 + kLineWaves * kFlight);
+      if (b0 + kOf * kFlight < end) fetch(b0 + kOf * kFlight);
 #pragma unroll
       for (int f = 0; f < kFlight; ++f) {
-        const int b = b0 + kLineWaves * f;
+        const int b = b0 + kOf * f;
         if (b >= end) break;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
@@ -135,7 +136,7 @@ __global__ __launch_bounds__(kLineThreads) void w4_line_kernel(W4 w, const float
     if (o < w.n) {
       float sum = 0.0f;
 #pragma unroll
-      for (int v = 0; v < kLineWaves; ++v) sum += part[v][u][r];
+      for (int v = 0; v < kOf; ++v) sum += part[v][u][r];
       if (bias) sum += bias[o];
       y[u * ldy + o] = bch::activate(sum, act);
     }
@@ -365,10 +366,12 @@ namespace bch {
 
 hipError_t launch_w4_line(hipStream_t s, int m, const W4& w, const float* x, long long ldx, const float* bias, int act,
                           float* y, long long ldy) {
-#define BCH_LINE(M) (w.group % 128 == 0 ? w4_line_kernel<M, 4> : w.group % 64 == 0 ? w4_line_kernel<M, 2> : w4_line_kernel<M, 1>)
-  auto kern = m == 1 ? BCH_LINE(1) : BCH_LINE(2);
+#define BCH_LINE(M, N) \
+  (w.group % 128 == 0 ? w4_line_kernel<M, 4, N> : w.group % 64 == 0 ? w4_line_kernel<M, 2, N> : w4_line_kernel<M, 1, N>)
+  const bool wide = m == 1 && w.tiles > 2 * device_cu_count();
+  auto kern = m == 2 ? BCH_LINE(2, 1024) : wide ? BCH_LINE(1, 512) : BCH_LINE(1, 1024);
 #undef BCH_LINE
-  hipLaunchKernelGGL(kern, dim3(w.tiles), dim3(kLineThreads), 0, s, w, x, ldx, w4_vec(w, x, ldx), bias, act, y, ldy);
+  hipLaunchKernelGGL(kern, dim3(w.tiles), dim3(wide ? 512 : 1024), 0, s, w, x, ldx, w4_vec(w, x, ldx), bias, act, y, ldy);
   return hipGetLastError();
 }
 

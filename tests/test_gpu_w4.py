@@ -215,6 +215,13 @@ def test_quantized_layer(dev):
         assert np.all(np.abs(got - x.astype(np.float64) @ back.astype(np.float64).T) <= slack(x, back) * (1 + 2.0**-20))
 
 
+@pytest.mark.parametrize("m", [1, 2])
+@pytest.mark.parametrize("n,k,group", [(9001, 200, 64), (8201, 300, 32), (8209, 9000, 160), (16400, 130, 128), (20001, 1, 32)])
+def test_one_row_many_outputs(dev, m, n, k, group):
+    """More workgroups than the card holds at a time."""
+    check(dev, np.random.default_rng(n), m, n, k, group, True, bias=True, act=Activation.ReLU)
+
+
 @pytest.mark.parametrize("m,n,k,group,zeros,act", [(2050, 20, 5000, 64, True, None), (2056, 36, 4609, 32, False, Activation.ReLU),
                                                    (70, 24, 20001, 32, True, None), (65, 259, 16392, 128, False, Activation.GELU),
                                                    (129, 16, 9000, 96, True, None), (300, 1000, 1000, 32, True, Activation.GELU),
