@@ -29,6 +29,7 @@ per step and serves every layer.  A cache is for one thread at a time.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 from typing import Iterable, Sequence
 
@@ -79,8 +80,18 @@ class KvStep:
         for i, s in enumerate(sequences):
             table[i, :len(cache._seqs[s].pages)] = cache._seqs[s].pages
         flat = [] if parents is None else [p for tree in parents for p in tree]
-        self._dev = _I32(cache.device, self.start, lens, table, flat)
-        start, length, tab, par = self._dev.ptrs
+        # where the new tokens stand, unless it is where their keys lie (with keys that were closed up before them it is not)
+        self._positions, self._far = None, False
+        where = []
+        ahead = [cache._seqs[s].ahead(length - n) for s, n, length in zip(sequences, counts, lens)]
+        if any(x and n for x, n in zip(ahead, counts)):
+            where = np.concatenate([x + length - n + np.array(_depths(parents[i]) if parents is not None else range(n), dtype=np.int64)
+                                    for i, (x, n, length) in enumerate(zip(ahead, counts, lens))])
+            self._far = bool(where.max() > _I32_MAX)
+        self._dev = _I32(cache.device, self.start, lens, table, flat, where if not self._far else [])
+        start, length, tab, par, pos = self._dev.ptrs
+        if len(where):
+            self._positions = C.c_void_p(pos)
         self._batch = N.KvBatch(len(lens), self.total, max([0] + self.counts), max([0] + lens), start, length)
         self._table, self._width = tab, width
         self._parents = C.c_void_p(par) if parents is not None else None
@@ -95,12 +106,35 @@ class KvStep:
 
 
 class _Sequence:
-    __slots__ = ("pages", "length", "evicted")
+    __slots__ = ("pages", "length", "evicted", "shifts")
 
     def __init__(self):
         self.pages: list[int] = []  # -1: given back by evict
         self.length = 0
         self.evicted = False  # whether there may be such pages
+        # (key, positions that it and those behind it stand ahead of their places), ascending; none before the first
+        self.shifts: list[tuple[int, int]] = []
+
+    def ahead(self, key: int) -> int:
+        """How far ahead of its place a token stands that becomes this key: one behind the key before it."""
+        at = bisect.bisect_left(self.shifts, (key,))
+        return self.shifts[at - 1][1] if at else 0
+
+    def place(self, key: int, aheads: Sequence[int]) -> None:
+        """The keys from this one on stand so far ahead of their places."""
+        last = self.ahead(key)
+        del self.shifts[bisect.bisect_left(self.shifts, (key,)):]
+        x = np.asarray(aheads, dtype=np.int64)
+        for i in np.flatnonzero(np.diff(x, prepend=last)).tolist():
+            self.shifts.append((key + i, int(x[i])))
+
+
+def _depths(tree: Sequence[int]) -> list[int]:
+    """The number of each draft's ancestors."""
+    out: list[int] = []
+    for p in tree:
+        out.append(out[p] + 1 if p >= 0 else 0)
+    return out
 
 
 class KvCache:
@@ -137,6 +171,7 @@ class KvCache:
         writes into them."""
         s, f = self._seq(sequence), self.new_sequence()
         self._seqs[f].pages, self._seqs[f].length, self._seqs[f].evicted = list(s.pages), s.length, s.evicted
+        self._seqs[f].shifts = list(s.shifts)
         for p in s.pages:
             if p >= 0:
                 self._refs[p] += 1
@@ -194,11 +229,14 @@ class KvCache:
             while len(s.pages) * ps < s.length:
                 s.pages.append(self._take())
         try:
-            return KvStep(self, [s for s, _ in items], [n for _, n in items], parents)
+            step = KvStep(self, [s for s, _ in items], [n for _, n in items], parents)
         except BaseException:
             for s, length in zip(seqs, old):
                 self._cut(s, length)
             raise
+        for s, length, tree in zip(seqs, old, parents or []):
+            s.place(length, s.ahead(length) + np.array(_depths(tree), dtype=np.int64) - np.arange(len(tree)))
+        return step
 
     def append(self, step: KvStep, layer: int, k: Tensor, v: Tensor) -> None:
         """The step's keys and values, [total, kv_heads, head_dim], into their pages."""
@@ -219,9 +257,11 @@ class KvCache:
     def append_rotary(self, step: KvStep, layer: int, rotary, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
         """append with the keys turned by their positions (a Rotary of head_dim),
         and q [total, heads, head_dim] turned by the same: the result is for
-        attention.  A draft stands behind its parent.  Keys stay turned as they
-        were appended: after retain has closed them up, distances over the gap
-        are as before."""
+        attention.  A sequence's new tokens stand behind the last key that it
+        held, a draft behind its parent.  Keys stay turned as they were appended:
+        where keep or retain close up keys with others between them, these, and
+        the tokens that follow, stand where they stood.  (A step with tokens
+        behind such keys takes three launches instead of one.)"""
         self._check_step("KvCache.append_rotary", step, layer)
         shape = [step.total, self.kv_heads, self.head_dim]
         for t in (k, v):
@@ -235,6 +275,8 @@ class KvCache:
         self._own(q, k, v)
         if rotary.device is not self.device:
             raise DeviceError("tensors live on different devices")
+        if step._far:
+            raise InvalidOperation("KvCache.append_rotary", "a position beyond 32 bits")
         out = Tensor.empty(qs, self.device)
         if step.total == 0:
             return out
@@ -242,6 +284,14 @@ class KvCache:
         row = N.AttnLayout(0, self.head_dim, self.kv_heads * self.head_dim)
         q_row = N.AttnLayout(0, self.head_dim, max(1, heads) * self.head_dim)
         dev = self.device
+        if step._positions is not None:
+            turned = Tensor.empty(shape, dev)
+            with dev._lock:
+                for src, dst, h, lay in ((q, out, heads, q_row), (k, turned, self.kv_heads, row)):
+                    dev.check(dev._lib.bch_rotary(dev.ctx, 1, h, step.total, self.head_dim, rotary._plan, 0, 0, step._positions,
+                                                  C.c_void_p(src.ptr), lay, C.c_void_p(dst.ptr), lay), "rotary")
+            self.append(step, layer, turned, v)
+            return out
         with dev._lock:
             dev.check(dev._lib.bch_kv_append_rotary(dev.ctx, self._pages(step, layer), step._batch, step._parents,
                                                     rotary._plan, heads, C.c_void_p(q.ptr), q_row, C.c_void_p(out.ptr), q_row,
@@ -385,6 +435,7 @@ class KvCache:
         for p in s.pages[keep:]:
             self._drop(p)
         del s.pages[keep:]
+        del s.shifts[bisect.bisect_left(s.shifts, (length,)):]
         s.length = length
 
     def _own(self, *ts: Tensor) -> None:
@@ -484,4 +535,10 @@ class KvCache:
                                                        C.c_void_p(keep), C.c_void_p(tos + 4 * b0)), "kv_keep")
         self._generation += 1
         for seq, to, positions in moves:
-            self._cut(self._seqs[seq], to + len(positions))
+            s = self._seqs[seq]
+            if s.shifts or (positions and positions[-1] >= to + len(positions)):
+                x = np.asarray(positions, dtype=np.int64)
+                # a kept key stands where it stood
+                ahead = np.array([0] + [a for _, a in s.shifts])[np.searchsorted([k for k, _ in s.shifts], x, side="right")]
+                s.place(to, ahead + x - to - np.arange(len(x)))
+            self._cut(s, to + len(positions))

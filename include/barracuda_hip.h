@@ -537,7 +537,10 @@ bch_status bch_rotary(bch_ctx *ctx, int B, int H, int S, int D,
  * Its key's place in the pages is that of the len[b]-n+i'th, as for
  * bch_kv_append; keys of pages that are not held, and keys before the
  * sequence's beginning, are not written (q is turned all the same).  H of 0: q and o
- * are not looked at.  A tree has at most 128 drafts a sequence. */
+ * are not looked at.  A tree has at most 128 drafts a sequence.  A sequence whose keys
+ * have been closed up (bch_kv_keep, with others between them given up) stands further
+ * on than its length: its new tokens take bch_rotary with their positions, and
+ * bch_kv_append. */
 bch_status bch_kv_append_rotary(bch_ctx *ctx, const bch_kv_pages *kv,
                                 const bch_kv_batch *batch, const int *parent,
                                 const bch_rotary_plan *plan, int H,
