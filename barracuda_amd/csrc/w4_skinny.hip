@@ -38,6 +38,31 @@ __device__ __forceinline__ void codes_of(unsigned c, float zero, float (&v)[8]) 
   }
 }
 
+// A group's inputs times its whole numbers are added up before the scale: up to 2^11 times an input, and what a small scale would bring
+// back into f32's range may have left it.  Such rows are computed again times 2^-kDown: this lane's part of an output's sum of
+// blocks b0, b0 + step, ..  (codes, scales and zeros are the lane's.)
+constexpr int kDown = 12;
+__device__ __forceinline__ float line_again(const W4& w, const u32x4* codes, const float* scales, const unsigned char* zeros,
+                                            const float* row, bool vec, int b0, int b1, int step) {
+  const int kb = (threadIdx.x & 63) >> 4;
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int b = b0; b < b1; b += step) {
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j) {
+      const long long g = bch::w4_group(w, 4 * b + j);
+      float v[8], q[8], one = 0.0f;
+      codes_of(reinterpret_cast<const unsigned*>(codes + (long long)b * 64)[j], (float)zeros[16 * g], v);
+      bch::w4_load8(q, row, 128 * b + 32 * j + 8 * kb, w.k, vec);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one = fmaf(v[e], ldexpf(q[e], -kDown), one);
+      sum = fmaf(scales[16 * g], one, sum);
+    }
+  }
+  sum += __shfl_xor(sum, 16);
+  return sum + __shfl_xor(sum, 32);
+}
+
 template <int MT, int FL, int THREADS>
 __global__ __launch_bounds__(THREADS) void w4_line_kernel(W4 w, const float* __restrict__ x, long long ldx, bool vec,
                                                            const float* __restrict__ bias, int act, float* y, long long ldy) {
@@ -131,15 +156,27 @@ __global__ __launch_bounds__(THREADS) void w4_line_kernel(W4 w, const float* __r
     if (kb == 0) part[wave][u][r] = acc[u];
   }
   __syncthreads();
-  if (threadIdx.x < 16 * MT) {
-    const int u = threadIdx.x >> 4, o = 16 * tile + r;
-    if (o < w.n) {
-      float sum = 0.0f;
+  if (wave > 0) return;
+  const int o = 16 * tile + r;
+  const bool on = kb < MT && o < w.n;
+  float sum = 0.0f;
+  if (on) {
 #pragma unroll
-      for (int v = 0; v < kOf; ++v) sum += part[v][u][r];
-      if (bias) sum += bias[o];
-      y[u * ldy + o] = bch::activate(sum, act);
+    for (int v = 0; v < kOf; ++v) sum += part[v][kb][r];
+  }
+  if (__any(!(fabsf(sum) < INFINITY))) {  // of a row of finite inputs: lost before the scale
+#pragma unroll
+    for (int u = 0; u < MT; ++u) {
+      bool finite = true;
+      for (int i = lane; i < w.k; i += 64) finite = finite && fabsf(x[u * ldx + i]) < INFINITY;
+      if (!__all(finite)) continue;
+      const float again = ldexpf(line_again(w, codes, scales, zeros, x + u * ldx, vec, 0, w.blocks, 1), kDown);
+      if (kb == u && !(fabsf(sum) < INFINITY)) sum = again;
     }
+  }
+  if (on) {
+    if (bias) sum += bias[o];
+    y[kb * ldy + o] = bch::activate(sum, act);
   }
 }
 
@@ -326,7 +363,7 @@ __global__ __launch_bounds__(kThreads, 2) void w4_skinny_kernel(W4 w, int m, int
           codes_of(cc[j], (float)zeros[t][16 * g], v);
           bch::w4_load8(q, x + r * ldx, 128 * b + 32 * j + 8 * kb, w.k, vec);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) one = fmaf(v[e], q[e], one);
+          for (int e = 0; e < 8; ++e) one = fmaf(v[e], ldexpf(q[e], -kDown), one);
           sum = fmaf(scales[t][16 * g], one, sum);
         }
       }
@@ -341,6 +378,7 @@ __global__ __launch_bounds__(kThreads, 2) void w4_skinny_kernel(W4 w, int m, int
       float v = 0.0f;
 #pragma unroll
       for (int u = 0; u < kWaves; ++u) v += f[u * T * 16 + i];
+      v = ldexpf(v, kDown);
       if (p) {
         p[(long long)r * w.n + o] = v;
       } else {
