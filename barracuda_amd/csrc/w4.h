@@ -124,11 +124,11 @@ __device__ __forceinline__ unsigned w4_top(const float (&v)[8], unsigned top) {
   }
   return top;
 }
-// The e that puts values whose largest has these bits below 2^kW4Top: far above bf16's smallest (a part
-// below it belongs to a value that is less than 2^-200 of the largest), and the sums of 2^20 products and
-// those times any scale from 2^-100 to 2^100 within f32.
-constexpr int kW4Top = 90;
-__device__ __forceinline__ int w4_exponent(unsigned top) { return kW4Top + 126 - (int)(top >> 23); }
+// The e of a row whose largest value has these bits: all below 2^kW4Top, as high as bf16 reaches, so that values far below the largest
+// keep their bits (all of them from 2^-160 of it on: a product's last lies 114 below its value, f32's at 2^-149).  Not beyond
+// kW4Unit: sums then never exceed what they stand for, and f32 holds them wherever it holds that.
+constexpr int kW4Top = 127;
+__device__ __forceinline__ int w4_exponent(unsigned top) { return min(kW4Unit, kW4Top + 126 - (int)(top >> 23)); }
 inline bool w4_vec(const W4& w, const float* x, long long ldx) {
   return w.k % 4 == 0 && ldx % 4 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 }
