@@ -181,11 +181,11 @@ __global__ __launch_bounds__(THREADS) void w4_line_kernel(W4 w, const float* __r
 }
 
 // ---- up to 64 rows ----
-// x's parts are of 2^kUp x here, whatever the row (subnormal numbers keep all their bits): no row has to be read whole before the
-// first part is written.  A value from 2^24 on would leave bf16's range; its row and chunk are noted, and the product
-// computes such rows again in f32.
-constexpr int kUp = 100;
-constexpr float kMost = 0x1p24f;
+// x's parts are of 2^kUp x here, whatever the row: no row has to be read whole before the first part is written.  2^kUp takes back
+// kW4Unit: sums are what they stand for, finite wherever f32 is, and subnormal numbers keep their bits.  A value
+// from 2^36 on would leave bf16's range; its row and chunk are noted, and the product computes such rows again in f32.
+constexpr int kUp = bch::kW4Unit;
+constexpr float kMost = 0x1p36f;
 constexpr int kSplitThreads = 256, kSplitRows = 8, kSplitOctets = kSplitThreads / kSplitRows;
 
 __global__ __launch_bounds__(kSplitThreads) void w4_split_few_kernel(int m, int k, int octets, int rows, const float* __restrict__ x,
@@ -336,7 +336,7 @@ __global__ __launch_bounds__(kThreads, 2) void w4_skinny_kernel(W4 w, int m, int
     for (int e = 0; e < 4; ++e) {
       const int r = r0 + e;
       if (r >= m) continue;
-      float v = ldexpf(sum[e], bch::kW4Unit - kUp);
+      float v = sum[e];
       if (p) {
         p[(long long)r * w.n + o] = v;
       } else {

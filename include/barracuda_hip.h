@@ -234,7 +234,7 @@ typedef struct bch_w4 {
  * its zero point contributes nothing (0 * infinity: NaN, as in f32).  One or two rows
  * run on f32 multiplications, more on the bf16 matrix cores, where a weight's whole number is
  * exact and x takes three parts: three part products a weight, to f32 accuracy (beside
- * an input of 2^24 or more, those below 2^-130 of it may lose bits).  From three rows on
+ * an input of 2^36 or more, those below 2^-130 of it may lose bits).  From three rows on
  * scratch in the context's workspace holds the parts (at most 256 MiB); where that may not grow (under
  * capture, or out of memory) the call runs with what there is, two rows at a time if need be. */
 bch_status bch_w4_linear(bch_ctx *ctx, int m, const bch_w4 *w, const float *x,

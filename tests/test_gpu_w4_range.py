@@ -57,7 +57,7 @@ def test_ordinary_inputs_beside_one_whose_weights_are_zero(dev, m, group, large)
 
 @pytest.mark.parametrize("m", MS)
 @pytest.mark.parametrize("k,group", [(96, 32), (700, 128)])
-@pytest.mark.parametrize("x_log,scale_log", [(-20, 125), (-60, 120), (-100, 127), (-140, 100), (-140, 127), (20, -130),
+@pytest.mark.parametrize("x_log,scale_log", [(5, 113), (-20, 125), (-60, 120), (-100, 127), (-140, 100), (-140, 127), (20, -130),
                                              (100, -140), (120, -149), (-30, -100), (-70, -70)])
 def test_scales_of_any_magnitude(dev, m, k, group, x_log, scale_log):
     """What inputs and scales of opposite magnitudes give is what f32 gives; results of 2^-149 steps are off by half of one a sum."""
