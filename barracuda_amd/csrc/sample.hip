@@ -10,7 +10,8 @@
 // them are exact, so neither the order in which threads add nor how a row is cut up changes a choice, and the
 // roundings move a border by 2^-45 of the largest weight a token.  What is below half of 2^-U is never drawn.  (The whole
 // weight of a row of which nothing but top_p, or nothing at all, leaves some is added up from spans of 512 logits, whole
-// numbers of 2^-51 of each span's largest: the same spans and order for every row of that length.)
+// numbers of 2^-51 of each span's largest, and rows that nothing cuts are drawn from these: the same spans and order for every
+// row of that length, whichever kernels take it.)
 #include "sample.h"
 
 #include <algorithm>
@@ -44,9 +45,10 @@ struct Scale {
 // 2^-t for t = (m - x) per: the whole part of t is an exponent, the rest, within 1/2, goes through the series of exp to the
 // eleventh power (off by 2^-47).  A token of an infinite distance weighs nothing.
 __device__ __forceinline__ double weight_of(const Scale& s, float x) {
+#pragma clang fp contract(off)  // (the same bits wherever it is inlined)
   const double d = x == s.m ? 0.0 : (double)s.m - (double)x, t = d * s.per;
   if (!(t < 64.0)) return 0.0;
-  const double n = rint(t), r = (n - t) * 0.69314718055994530942;
+  const double n = rint(t), r = fma(-d, s.per, n) * 0.69314718055994530942;
   double p = fma(r, 2.50521083854417187751e-08, 2.75573192239858906526e-07);
   p = fma(r, p, 2.75573192239858906526e-06);
   p = fma(r, p, 2.48015873015873015873e-05);
@@ -208,8 +210,9 @@ __device__ u64 find_cut(General& s, Sums& sums, const float* row, int vocab, con
   return above_weight + cut.ties * tie_weight;
 }
 
-// For a rule that leaves more than one token.
-__device__ void general_row(General& s, Sums& sums, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc) {
+// For a rule that leaves more than one token, and not all.  whole_row: the row's weight in units, where only a weight cuts.
+__device__ void general_row(General& s, Sums& sums, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc,
+                            double whole_row) {
   const float* row = c.logits + r * c.stride;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   Cut cut{0, 0};
@@ -219,8 +222,7 @@ __device__ void general_row(General& s, Sums& sums, const SampleCall& c, long lo
   if (by_weight(rule))
     find_cut<false>(s, sums, row, c.vocab, sc,
                     [&](u64 all) {
-                      const u64 of = count_cut ? left : all;
-                      return min(of, part_units(rule, (double)of));
+                      return min(count_cut ? left : all, part_units(rule, count_cut ? (double)left : whole_row));
                     },
                     cut);
   // the draw: the part of the row that the target falls into, sixteen times smaller each time
@@ -392,6 +394,40 @@ __device__ __forceinline__ int span_index(int base, int e) {
   return base + 256 * (e / 4) + 4 * (int)(threadIdx.x & 63) + e % 4;
 }
 
+// What the logits of a wavefront's span, the largest of them `top`, weigh against that one, in units of 2^-kSpanUnit.
+template <bool MANY>
+__device__ __forceinline__ u64 weigh(const SampleCall& c, const SampleRule& rule, const float (&x)[8], unsigned top) {
+  Scale sc = scale_of(c, rule, logit_of(top));
+  sc.unit_log = kSpanUnit;
+  u64 sum = 0;
+  if constexpr (MANY) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sum += units(sc, weight_of(sc, x[e]));
+  } else {
+    each(x, [&](float v) { sum += units(sc, weight_of(sc, v)); });
+  }
+#pragma unroll 1
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
+  return sum;
+}
+// The largest logit and the weight of span `at`, by one wavefront, where no record holds them.
+__device__ __forceinline__ Record weigh_span(const SampleCall& c, const float* row, const SampleRule& rule, int at) {
+  float x[8];
+  load_span(c, row, at * kSpan, x);
+  unsigned mine = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) mine = max(mine, key_of(x[e]));
+  Record q{};
+  q.top = key_of(bch::wave_allreduce(logit_of(mine), bch::OpMax()));
+  if (q.top != kNothing) q.weight = weigh<false>(c, rule, x, q.top);
+  return q;
+}
+// A span's weight against the row's largest logit, in units of 2^-kSpanUnit.
+__device__ __forceinline__ double span_weight(const Scale& s, const Record& q) {
+#pragma clang fp contract(off)
+  return q.top == kNothing ? 0.0 : (double)q.weight * weight_of(s, logit_of(q.top));
+}
+
 // Span `at` of a row, by one wavefront: its record, and its list (keys in the upper half, 2^32 - 1 - index in the lower).
 // MANY: a launch of many wavefronts, whose code is fetched once for all of them: its weights without a loop.
 template <bool MANY>
@@ -437,18 +473,7 @@ __device__ __forceinline__ void list_span(const SampleCall& c, const float* row,
     }
   }
   u64 sum = 0;
-  if (needs_whole(rule, c.vocab) && top != kNothing) {
-    Scale sc = scale_of(c, rule, logit_of(top));
-    sc.unit_log = kSpanUnit;
-    if constexpr (MANY) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum += units(sc, weight_of(sc, x[e]));
-    } else {
-      each(x, [&](float v) { sum += units(sc, weight_of(sc, v)); });
-    }
-#pragma unroll 1
-    for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
-  }
+  if (needs_whole(rule, c.vocab) && top != kNothing) sum = weigh<MANY>(c, rule, x, top);
   if (lane == 0) *record = {top, count > kListMost ? 0xffffffffu : tau, min(count, kListMost), first, sum};
 }
 
@@ -484,18 +509,57 @@ struct Common {
   u64 chunk[kThreads];
 };
 
+// The threads' sums of their spans' weights.  HELD: of records; else each thread's spans are weighed by a wavefront, in the same
+// order.  spans_of(thread, i): that thread's i-th span, or -1.
+template <bool HELD, typename Of>
+__device__ __forceinline__ double thread_weight(Common& m, const SampleCall& c, const float* row, const SampleRule& rule, const Scale& sc,
+                                                const Record* records, Of spans_of) {
+#pragma clang fp contract(off)
+  if constexpr (HELD) {
+    double sum = 0.0;
+    for (int i = 0, at; (at = spans_of((int)threadIdx.x, i)) >= 0; ++i) sum += span_weight(sc, records[at]);
+    return sum;
+  } else {
+    for (int t = threadIdx.x >> 6; t < kThreads; t += kWaves) {
+      double sum = 0.0;
+      for (int i = 0, at; (at = spans_of(t, i)) >= 0; ++i) sum += span_weight(sc, weigh_span(c, row, rule, at));
+      if ((threadIdx.x & 63) == 0) m.chunk[t] = __builtin_bit_cast(u64, sum);
+    }
+    __syncthreads();
+    return __builtin_bit_cast(double, m.chunk[threadIdx.x]);
+  }
+}
+// A row's weight in units.  (Behind a barrier since sums were read.)
+template <bool HELD>
+__device__ __forceinline__ double row_weight(Common& m, const SampleCall& c, const float* row, const SampleRule& rule, const Scale& sc,
+                                             int spans, const Record* records) {
+#pragma clang fp contract(off)
+  double whole = thread_weight<HELD>(m, c, row, rule, sc, records, [&](int t, int i) {
+    const long long at = t + (long long)kThreads * i;
+    return at < spans ? (int)at : -1;
+  });
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) whole += __shfl_xor(whole, d);
+  if ((threadIdx.x & 63) == 0) m.sums[0][threadIdx.x >> 6] = __builtin_bit_cast(u64, whole);
+  __syncthreads();
+  whole = 0.0;
+  for (int i = 0; i < kWaves; ++i) whole += __builtin_bit_cast(double, m.sums[0][i]);
+  return ldexp(whole, c.unit_log - kSpanUnit);
+}
+
 // A row of which all tokens stay: the span that the target falls into, then the token in it.
+template <bool HELD>
 __device__ void draw_span(Common& m, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc, int spans,
                           const Record* records) {
+#pragma clang fp contract(off)
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const float* row = c.logits + r * c.stride;
   // a thread's spans lie together; weights in units of 2^-kSpanUnit of the row's largest
-  const int per = (spans - 1) / kThreads + 1, lo = min((long long)spans, (long long)per * threadIdx.x), hi = min(spans, lo + per);
-  auto span_weight = [&](int i) {
-    const Record q = records[i];
-    return q.top == kNothing ? 0.0 : (double)q.weight * weight_of(sc, logit_of(q.top));
-  };
-  double mine = 0.0;
-  for (int i = lo; i < hi; ++i) mine += span_weight(i);
+  const int per = (spans - 1) / kThreads + 1;
+  const double mine = thread_weight<HELD>(m, c, row, rule, sc, records, [&](int t, int i) {
+    const long long at = (long long)per * t + i;
+    return i < per && at < spans ? (int)at : -1;
+  });
   double run = mine;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -521,36 +585,39 @@ __device__ void draw_span(Common& m, const SampleCall& c, long long r, const Sam
   if (mine > 0.0) atomicMax(&m.n, (int)threadIdx.x);
   __syncthreads();
   const int chosen = m.pick < kThreads ? m.pick : m.n;
-  __syncthreads();
-  if ((int)threadIdx.x == chosen) {
-    double at = run - mine;
-    int i = lo, last = lo;
-    for (; i < hi; ++i) {
-      const double w = span_weight(i);
-      if (w > 0.0) last = i;
-      if (at + w > target) break;
-      at += w;
-    }
-    if (i == hi) {
-      i = last;
-      at -= span_weight(i);
-    }
-    m.n = i;
-    m.before = at;
-  }
+  if ((int)threadIdx.x == chosen) m.before = run - mine;
   __syncthreads();
   if (wave > 0) return;
-  const Record q = records[m.n];
+  auto span = [&](int i) {
+    if constexpr (HELD)
+      return records[i];
+    else
+      return weigh_span(c, row, rule, i);
+  };
+  const int lo = per * chosen, hi = (int)min((long long)spans, (long long)lo + per);
+  double at = m.before;
+  int i = lo, last = lo;
+  for (; i < hi; ++i) {
+    const double w = span_weight(sc, span(i));
+    if (w > 0.0) last = i;
+    if (at + w > target) break;
+    at += w;
+  }
+  if (i == hi) {
+    i = last;
+    at -= span_weight(sc, span(i));
+  }
+  const Record q = span(i);
   const double of = weight_of(sc, logit_of(q.top));
-  u64 left = min((u64)fmax((target - m.before) / of, 0.0), q.weight - 1);
-  Scale span = scale_of(c, rule, logit_of(q.top));
-  span.unit_log = kSpanUnit;
+  u64 left = min((u64)fmax((target - at) / of, 0.0), q.weight - 1);
+  Scale own = scale_of(c, rule, logit_of(q.top));
+  own.unit_log = kSpanUnit;
   // eight tokens a lane, in index order
   float x[8];
-  int i = m.n * kSpan + 8 * lane;
-  load_eight(c, c.logits + r * c.stride, i, x);
+  i = i * kSpan + 8 * lane;
+  load_eight(c, row, i, x);
   u64 sum = 0;
-  each(x, [&](float v) { sum += units(span, weight_of(span, v)); });
+  each(x, [&](float v) { sum += units(own, weight_of(own, v)); });
   left -= wave_scan(sum, lane) - sum;
   const u64 here = __ballot(left < sum);  // (what has become less than 0 is large)
   if (!here) return;
@@ -558,7 +625,7 @@ __device__ void draw_span(Common& m, const SampleCall& c, long long r, const Sam
   const int owner = __ffsll((long long)here) - 1;
   left = __shfl(left, owner);
   i = __shfl(i, owner) + lane;
-  const u64 w = lane < 8 && i < c.vocab ? units(span, weight_of(span, clean(c.logits[r * c.stride + i]))) : 0, end = wave_scan(w, lane);
+  const u64 w = lane < 8 && i < c.vocab ? units(own, weight_of(own, clean(row[i]))) : 0, end = wave_scan(w, lane);
   if (left < end && left >= end - w) answer(c, r, i, (double)w * of / whole);
 }
 
@@ -828,9 +895,10 @@ __device__ __forceinline__ bool choose_many(Lists& lists, Common& m, const Sampl
 }
 
 // A row's token from its records and lists (list of span i at lists + i * kListMost).  False if they do not tell; `top`: the
-// largest logit's key.
+// largest logit's key, `whole`: the row's weight in units, where only a weight cuts.
 __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, int spans, const Record* records,
-                       const u64* lists, unsigned& top) {
+                       const u64* lists, unsigned& top, double& whole) {
+  whole = 0.0;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // the beginnings of the lists, 16 lanes a span: of up to four spans a thread, or more of fewer
   constexpr int kFlight = 4, kAt = kThreads / 16;
@@ -909,7 +977,7 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
   const Scale sc = scale_of(c, rule, logit_of(top));
   const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
   if (!count_cut && !weight_cut && sc.min_p == 0.0) {
-    draw_span(m, c, r, rule, sc, spans, records);
+    draw_span<true>(m, c, r, rule, sc, spans, records);
     return true;
   }
   bool covers_min = false;
@@ -948,20 +1016,7 @@ __device__ bool choose(Work& work, Common& m, const SampleCall& c, long long r, 
       if (!__any(more)) break;
     }
   }
-  double whole = 0.0;  // the row's weight, in units
-  if (!count_cut && weight_cut) {
-    for (int i = threadIdx.x; i < spans; i += kThreads) {
-      const Record q = records[i];
-      if (q.top != kNothing) whole += (double)q.weight * weight_of(sc, logit_of(q.top));
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) whole += __shfl_xor(whole, d);
-    if (lane == 0) m.sums[0][wave] = __builtin_bit_cast(u64, whole);
-    __syncthreads();
-    whole = 0.0;
-    for (int i = 0; i < kWaves; ++i) whole += __builtin_bit_cast(double, m.sums[0][i]);
-    whole = ldexp(whole, c.unit_log - kSpanUnit);
-  }
+  if (!count_cut && weight_cut) whole = row_weight<true>(m, c, c.logits + r * c.stride, rule, sc, spans, records);
   __syncthreads();
   int n = m.n;
   const bool complete = tau <= kNothing + 1 || covers_min;  // all that can stay is on the lists
@@ -1005,13 +1060,13 @@ __device__ void bin_chunk(u64* hist, const SampleCall& c, const float* row, cons
   __syncthreads();
 }
 
-// The row's token from its chunks' bins (chunk i's at hist + i * kBins).
+// The row's token from its chunks' bins (chunk i's at hist + i * kBins); whole_row as general_row's.
 __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long long r, const SampleRule& rule, const Scale& sc,
-                              const u64* hist) {
+                              const u64* hist, double whole_row) {
   const float* row = c.logits + r * c.stride;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunks = (c.vocab - 1) / kChunk + 1;
   if (chunks > kChunksMost || c.vocab < 4) {
-    general_row(work.general, m.sums, c, r, rule, sc);
+    general_row(work.general, m.sums, c, r, rule, sc, whole_row);
     return;
   }
   int cut = kBins;   // the bin that the cut falls into: tokens of lower ones stay,
@@ -1027,7 +1082,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     }
     u64 whole;
     u64 before = block_scan(m.sums, w0 + w1, whole);
-    const u64 target = min(whole, part_units(rule, (double)whole));
+    const u64 target = min(whole, part_units(rule, whole_row));
     if (before < target && before + w0 + w1 >= target) {
       const bool second = before + w0 < target;
       m.pick = second ? i0 + 1 : i0;
@@ -1079,7 +1134,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     const int n = m.n;
     if (n > kListedMost || fours > kNearMost) {
       __syncthreads();
-      general_row(work.general, m.sums, c, r, rule, sc);
+      general_row(work.general, m.sums, c, r, rule, sc, whole_row);
       return;
     }
 #pragma unroll 1
@@ -1088,7 +1143,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
     // (the bin's own kSlots parts)
     if (!list_cut(work.lists, m, Bins{sc.m, g * (float)kSlots, (float)cut * (float)kSlots}, n, 0, false, want, last)) {
       __syncthreads();
-      general_row(work.general, m.sums, c, r, rule, sc);
+      general_row(work.general, m.sums, c, r, rule, sc, whole_row);
       return;
     }
     stay = n;
@@ -1152,39 +1207,45 @@ __global__ __launch_bounds__(256) void sample_list_kernel(SampleCall c, int span
   list_span<true>(c, c.logits + r * c.stride, rule, spans, at, records + r * spans + at,
             lists + (r * spans + at) * kListMost);
 }
-// later: rows that the lists do not tell are left to the next two kernels where their rule allows; left[r]: the largest logit's key,
-// or 0 for a row that is done.
+// A row that the lists do not tell: its weight as choose gives it, and its largest logit's key, or 0 for a row that is done.
+struct Left {
+  double whole;
+  unsigned top;
+};
+// later: such rows are left to the next two kernels where their rule allows.
 __global__ __launch_bounds__(kThreads) void sample_choose_kernel(SampleCall c, int spans, const Record* records, const u64* lists,
-                                                                 bool later, unsigned* left) {
+                                                                 bool later, Left* left) {
   __shared__ Work work;
   __shared__ Common common;
   const long long r = blockIdx.x;
   const SampleRule rule = c.rules ? c.rules[r] : c.rule;
   unsigned top;
-  const bool done = choose(work, common, c, r, rule, spans, records + r * spans, lists + r * spans * kListMost, top);
+  double whole;
+  const bool done = choose(work, common, c, r, rule, spans, records + r * spans, lists + r * spans * kListMost, top, whole);
   const bool leave = !done && later && binned(rule, c.vocab);
-  if (threadIdx.x == 0) left[r] = leave ? top : 0;
-  if (!done && !leave) general_row(work.general, common.sums, c, r, rule, scale_of(c, rule, logit_of(top)));
+  if (threadIdx.x == 0) left[r] = {whole, leave ? top : 0};
+  if (!done && !leave) general_row(work.general, common.sums, c, r, rule, scale_of(c, rule, logit_of(top)), whole);
 }
-__global__ __launch_bounds__(kThreads) void sample_bin_kernel(SampleCall c, int chunks, const unsigned* left, u64* hists) {
+__global__ __launch_bounds__(kThreads) void sample_bin_kernel(SampleCall c, int chunks, const Left* left, u64* hists) {
   __shared__ u64 hist[kBins];
   const long long r = blockIdx.x / chunks;
   const int chunk = blockIdx.x % chunks;
-  const unsigned top = left[r];
+  const unsigned top = left[r].top;
   if (!top) return;
   const SampleRule rule = c.rules ? c.rules[r] : c.rule;
   bin_chunk(hist, c, c.logits + r * c.stride, scale_of(c, rule, logit_of(top)), chunk);
   u64* to = hists + (r * chunks + chunk) * kBins;
   for (int i = threadIdx.x; i < kBins; i += kThreads) to[i] = hist[i];
 }
-__global__ __launch_bounds__(kThreads) void sample_binned_kernel(SampleCall c, int chunks, const unsigned* left, const u64* hists) {
+__global__ __launch_bounds__(kThreads) void sample_binned_kernel(SampleCall c, int chunks, const Left* left, const u64* hists) {
   __shared__ Work work;
   __shared__ Common common;
   const long long r = blockIdx.x;
-  const unsigned top = left[r];
+  const unsigned top = left[r].top;
   if (!top) return;
   const SampleRule rule = c.rules ? c.rules[r] : c.rule;
-  choose_binned(work, common, c, r, rule, scale_of(c, rule, logit_of(top)), hists + r * chunks * kBins);
+  choose_binned(work, common, c, r, rule, scale_of(c, rule, logit_of(top)), hists + r * chunks * kBins,
+                left[r].whole);
 }
 
 // All of it for a row of up to kWaves spans, or, where there is no room for records, for a row of any length by general_row.
@@ -1202,13 +1263,14 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int 
     if (wave < spans) list_span<false>(c, row, rule, spans, wave, &records[wave], &lists[wave * kListMost]);
     __syncthreads();
     unsigned top;
-    if (choose(work, common, c, r, rule, spans, records, lists, top)) return;
+    double whole;
+    if (choose(work, common, c, r, rule, spans, records, lists, top, whole)) return;
     const Scale sc = scale_of(c, rule, logit_of(top));
     if (binned(rule, c.vocab)) {
       bin_chunk(lists, c, row, sc, 0);
-      choose_binned(work, common, c, r, rule, sc, lists);
+      choose_binned(work, common, c, r, rule, sc, lists, whole);
     } else {
-      general_row(work.general, common.sums, c, r, rule, sc);
+      general_row(work.general, common.sums, c, r, rule, sc, whole);
     }
     return;
   }
@@ -1228,7 +1290,14 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int 
     if (threadIdx.x == 0) answer(c, r, any ? (int)(0xffffffffu - (unsigned)top) : -1, any ? 1.0 : 0.0);
     return;
   }
-  general_row(work.general, common.sums, c, r, rule, scale_of(c, rule, logit_of(top_key)));
+  const Scale sc = scale_of(c, rule, logit_of(top_key));
+  const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
+  if (!count_cut && !weight_cut && sc.min_p == 0.0) {
+    draw_span<false>(common, c, r, rule, sc, spans, nullptr);
+    return;
+  }
+  const double whole = !count_cut && weight_cut ? row_weight<false>(common, c, row, rule, sc, spans, nullptr) : 0.0;
+  general_row(work.general, common.sums, c, r, rule, sc, whole);
 }
 
 }  // namespace
@@ -1241,7 +1310,7 @@ int sample_unit_log(int vocab) {
   return std::min(51, 62 - bits);
 }
 
-// Of a row: lists, records, a word for what is left, and bins; none where a workgroup holds them.
+// Of a row: lists, records, what is left of it, and bins; none where a workgroup holds them.
 struct RowBytes {
   size_t lists, records, bins, all;
 };
@@ -1249,7 +1318,7 @@ static RowBytes row_bytes(const SampleCall& c) {
   const size_t spans = (size_t)(c.vocab - 1) / kSpan + 1, chunks = (size_t)(c.vocab - 1) / kChunk + 1;
   if (spans <= kWaves) return {0, 0, 0, 0};
   RowBytes b{spans * kListMost * sizeof(u64), spans * sizeof(Record), chunks > kChunksMost ? 0 : chunks * kBins * sizeof(u64), 0};
-  b.all = b.lists + b.records + b.bins + 8;
+  b.all = b.lists + b.records + b.bins + sizeof(Left);
   return b;
 }
 constexpr size_t kMostBytes = (size_t)64 << 20;  // rows go through it in turn
@@ -1283,7 +1352,7 @@ hipError_t launch_sample(hipStream_t s, const SampleCall& call, int rows, void* 
       u64* lists = static_cast<u64*>(ws);
       u64* hists = lists + n * each.lists / sizeof(u64);
       Record* records = reinterpret_cast<Record*>(hists + n * each.bins / sizeof(u64));
-      unsigned* left = reinterpret_cast<unsigned*>(records + (size_t)n * spans);
+      Left* left = reinterpret_cast<Left*>(records + (size_t)n * spans);
       hipLaunchKernelGGL(sample_list_kernel, dim3((unsigned)(n * (long long)groups)), dim3(256), 0, s, c, spans, groups, records, lists);
       if ((e = hipGetLastError()) != hipSuccess) return e;
       hipLaunchKernelGGL(sample_choose_kernel, dim3(n), dim3(kThreads), 0, s, c, spans, records, lists, later, left);

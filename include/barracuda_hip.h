@@ -574,8 +574,9 @@ typedef struct bch_sampling {
  * the kernels run) each row has its own; there what is out of range is taken as the nearest that is in it, and
  * NaN as 0 for a temperature or min_p, as 1 for a top_p.  NaN logits count as -inf, which is never chosen;
  * a row of nothing else gives token -1, probability 0.  Tokens of +inf share all weight.  Weights are added up as whole numbers of 2^-U, U =
- * min(51, 62 - bits of vocab), to which they are rounded (44 for 131072 tokens): the same logits give the same
- * token whatever else is in the batch. */
+ * min(51, 62 - bits of vocab), to which they are rounded (44 for 131072 tokens); a row that only top_p cuts, or nothing,
+ * has its whole weight from 512 logits at a time, of 2^-51 of their largest.  The same logits, rule and number give the
+ * same token whatever else is in the batch and however much workspace there is. */
 bch_status bch_sample(bch_ctx *ctx, int rows, int vocab, const float *logits,
                       long long row_stride, const bch_sampling *rule,
                       const bch_sampling *row_rules, const float *u, int *tokens,
