@@ -852,7 +852,8 @@ __device__ bool list_draw(Lists& lists, Common& m, const SampleCall& c, long lon
   }
   return true;
 }
-// choose_few for up to kListedMost tokens, none below key `tau`.
+// choose_few for up to kListedMost tokens, none below key `tau`.  Their bins reach down to that, or of a row whose tokens are all listed,
+// where it is f32's lowest, to the least of them (else all would be in one bin); for weights to where they end.
 __device__ __forceinline__ bool choose_many(Lists& lists, Common& m, const SampleCall& c, long long r, const SampleRule& rule,
                                             const Scale& sc, int n, unsigned tau, double whole, bool complete) {
   const bool count_cut = by_count(rule, c.vocab), weight_cut = by_weight(rule);
@@ -860,11 +861,13 @@ __device__ __forceinline__ bool choose_many(Lists& lists, Common& m, const Sampl
   if (threadIdx.x == 0) m.least = 0xffffffffu;
   __syncthreads();
   u64 mine = 0, listed;
+  unsigned lowest = key_of(INFINITY);
 #pragma unroll 1
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const unsigned key = (unsigned)(lists.entry[i] >> 32);
     const double real = weight_of(sc, logit_of(key));
     mine += lists.weight[i] = units(sc, real);
+    lowest = min(lowest, key);
     if (sc.min_p > 0.0) {
       if (real >= sc.min_p)
         atomicMin(&m.least, key);
@@ -876,10 +879,18 @@ __device__ __forceinline__ bool choose_many(Lists& lists, Common& m, const Sampl
   const unsigned least = m.least;
   const bool short_of_min = sc.min_p > 0.0 && (complete || m.large > 0);
   if (!count_cut && !short_of_min && !(weight_cut && (complete || listed >= part_units(rule, whole)))) return false;
-  const Bins bins{sc.m, (float)kSlots / (sc.m - logit_of(tau)), 0.0f};
+  float end = logit_of(tau);
+  if (tau <= kNothing + 1) {
+    end = -bch::wave_allreduce(-logit_of(lowest), bch::OpMax());
+    if ((threadIdx.x & 63) == 0) m.sums[1][threadIdx.x >> 6] = key_of(end);
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) lowest = min(lowest, (unsigned)m.sums[1][w]);
+    end = logit_of(lowest);
+  }
+  const float end_weight = fmaxf(end, sc.m - 44.4f * rule.temperature);  // (2^-64 there)
   u64 last = 0, more = 0;
   if (count_cut && n > rule.top_k) {
-    if (!list_cut(lists, m, bins, n, 0, true, rule.top_k, last)) return false;
+    if (!list_cut(lists, m, Bins{sc.m, (float)kSlots / (sc.m - end), 0.0f}, n, 0, true, rule.top_k, last)) return false;
     if (weight_cut) {
       mine = 0;
       for (int i = threadIdx.x; i < n; i += kThreads) mine += lists.entry[i] >= last ? lists.weight[i] : 0;
@@ -887,7 +898,9 @@ __device__ __forceinline__ bool choose_many(Lists& lists, Common& m, const Sampl
     }
   }
   if (weight_cut) {
-    if (!list_cut(lists, m, bins, n, last, false, part_units(rule, count_cut ? (double)listed : whole), more)) return false;
+    if (!list_cut(lists, m, Bins{sc.m, (float)kSlots / (sc.m - end_weight), 0.0f}, n, last, false,
+                  part_units(rule, count_cut ? (double)listed : whole), more))
+      return false;
     last = max(last, more);
   }
   if (sc.min_p > 0.0) last = max(last, (u64)least << 32);
