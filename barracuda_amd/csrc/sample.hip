@@ -1125,7 +1125,7 @@ __device__ void choose_binned(Work& work, Common& m, const SampleCall& c, long l
         bool any = false;
 #pragma unroll
         for (int e = 0; e < 4; ++e) any |= x[f][e] >= low && x[f][e] <= high;
-        if (any) {
+        if (any && at + 4 * kThreads * f < c.vocab) {
           const int to = atomicAdd(&m.large, 1);
           if (to < kNearMost) near[to] = at + 4 * kThreads * f;
         }

@@ -8,6 +8,7 @@ import numpy as np
 import pytest
 
 from barracuda_amd import Sampling, Tensor
+from tests.sample_model import keep
 from tests.test_gpu_kv_cache import _p, _t
 from tests.test_gpu_sample import check
 
@@ -65,3 +66,19 @@ def test_an_outlier_does_not_spoil_the_bins_of_weights(dev, lowest):
     rng = np.random.default_rng(5)
     rule = Sampling(1.3, 0, 0.98)
     assert time_of(dev, left(rng, 16, 50021, 500, lowest), rule) <= 1.7 * time_of(dev, left(rng, 16, 50021, 100), rule)
+
+
+@pytest.mark.parametrize("vocab", [8195, 20001, 50021, 50257, 151936, 200000])
+@pytest.mark.parametrize("back", [1, 4])
+def test_a_row_whose_last_logits_lie_at_the_cut(dev, vocab, back):
+    """Thousands of tokens stay; one that lies where top_p cuts is among the row's last four, or none of those is near."""
+    rng = np.random.default_rng(vocab)
+    rule = Sampling(1.3, 0, 0.98)
+    x = 2 * rng.standard_normal((16, vocab), dtype=np.float32)
+    x[:, -4:] = 0.0
+    far = time_of(dev, x, rule)
+    for r in x:
+        ids, _, _ = keep(r, rule.temperature, rule.top_k, rule.top_p, rule.min_p)
+        r[-back] = r[ids].min()
+    # (a search of the row would add 60 us and more to 40 to 60)
+    assert time_of(dev, x, rule) <= 1.4 * far
