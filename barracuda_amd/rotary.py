@@ -31,6 +31,7 @@ from .tensor import HipDevice, Tensor, _Buffer, _check_i32, _dense, _numel, _sam
 
 __all__ = ["Rotary", "RotaryPositions", "rotary_freqs"]
 
+_FASTEST = 2.0**19  # radians a position: angles of 32-bit positions stay below 2^50, where 64 bits still tell their turns
 _SCALINGS = ("none", "linear", "base", "parts")
 
 
@@ -73,6 +74,8 @@ class Rotary:
             f = np.ascontiguousarray(freqs, dtype=np.float64).reshape(-1)
             if f.size != dim // 2:
                 raise ShapeMismatch([dim // 2], [f.size])
+        if not np.all(np.abs(f) <= _FASTEST):
+            raise InvalidInput(f"rotary: radians a position must be numbers of at most {_FASTEST:g}")
         self.head_dim, self.dim, self.interleaved, self.scale = int(head_dim), int(dim), bool(interleaved), float(scale)
         self.freqs = f
         self.device = device or get_device()

@@ -513,7 +513,8 @@ bch_status bch_kv_keep(bch_ctx *ctx, const bch_kv_pages *kv, int layers,
  * columns 2i and 2i + 1.  At position p a pair (a, b) becomes
  *   scale (a cos t - b sin t), scale (a sin t + b cos t),  t = p freq[i];
  * columns from dim on stay.  freq [dim/2], radians a position, is device
- * memory.  Angles are products in 64 bits. */
+ * memory.  Angles are products in 64 bits, for angles below 2^50 (positions of 32
+ * bits and freq of at most 2^19); what larger ones give is not defined. */
 typedef struct bch_rotary_plan {
   int dim;
   int interleaved;

@@ -99,3 +99,12 @@ def test_sinks_and_the_newest_keys(dev, h, hkv, d, page, rotary):
     m.cache.truncate(a, 3)
     m._only(a, range(3))
     m.step([(a, 2), (c, 1), (b, 1)])
+
+
+def test_the_fastest_pair_at_the_furthest_positions(dev):
+    """Angles of up to 2^50: cosines and sines are still those of the product in 64 bits."""
+    x = np.random.default_rng(1).standard_normal((1, 2, 64, 4), dtype=np.float32)
+    r = Rotary(4, freqs=[2.0**19, 523456.789], device=dev)
+    for first in (2**31 - 64, -(2**31) + 1, 12345678):
+        y, tol = turned(x, first + np.arange(64), r.freqs, 4, False, 1.0)
+        assert np.all(np.abs(_t(x, dev).rotary(r, first=first).to_numpy() - y) <= tol)

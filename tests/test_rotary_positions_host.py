@@ -7,7 +7,7 @@ import pytest
 
 from barracuda_amd import KvCache, Rotary, Tensor
 from barracuda_amd import _native as N
-from barracuda_amd.error import InvalidOperation, OutOfMemory
+from barracuda_amd.error import InvalidInput, InvalidOperation, OutOfMemory
 from tests.rotary_model import depths
 from tests.test_kv_cache_host import _HostDevice, _HostLib, _check_pages
 
@@ -216,3 +216,13 @@ def test_positions_beyond_32_bits_are_refused():
     with pytest.raises(InvalidOperation):
         cache.append_rotary(step, 0, r, x[0], x[1], x[1])
     cache.append(step, 0, x[1], x[1])
+
+
+def test_frequencies_beyond_what_angles_hold_are_refused():
+    dev = _device()
+    assert Rotary(4, freqs=[2.0**19, -(2.0**19)], device=dev).freqs[0] == 2.0**19
+    for bad in ([1.0, 2.0**19 + 1], [-1e6, 0.0], [np.inf, 1.0], [1.0, np.nan]):
+        with pytest.raises(InvalidInput):
+            Rotary(4, freqs=bad, device=dev)
+    with pytest.raises(InvalidInput):
+        Rotary(64, base=1e-9, device=dev)
