@@ -55,7 +55,7 @@ __device__ __forceinline__ int w4_group(const W4& w, int c) { return (int)(((uns
 // a bf16's.  The sign comes from where it was, and with it bit 12, where the shift leaves the sign: there it is 1 for those
 // exponents and 0 for 0, so the bf16 is (code - zero) * 2^-91 in every case.  17 operations take eight codes apart;
 // converting bytes to f32, subtracting and packing takes 23 (2048 rows of 4096 -> 11008: 479 and 494 us).
-// Codes as bf16 below its smallest normal number would take 11 (sign and magnitude are what a packed f16 addition of such numbers
+// Codes as bf16 below its smallest normal number would take 9 to 11 (sign and magnitude are what a packed f16 addition of such numbers
 // leaves), but the matrix cores add their products as if each magnitude began at bit 7: up to three bits of a small
 // code's are lost.
 constexpr int kW4Unit = 91;  // a sum of products with such weights is 2^-91 of what it stands for

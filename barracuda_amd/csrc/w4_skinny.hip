@@ -21,7 +21,7 @@ __device__ __forceinline__ f32x4_t mm16(u32x4 a, u32x4 b, f32x4_t c) {
 // ---- one or two rows: f32 multiplications ----
 // A workgroup has 16 outputs, its wavefronts every 16th or eighth block of inputs, two of them in flight each; x lies in LDS.  What
 // bounds it: the launch, the first trip to memory, the codes' stream.  One row, 4096 -> 11008 / 50000 and back, us: 16 wavefronts
-// 9.2 / 31 / 9.2, eight 8.9 / 26 / 10.9; two rows 11.2 / 36 / 10.9 and 12.1 / 38 / 12.  So eight where one row has more workgroups than two
+// 9.2 / 31 / 9.2, eight 8.9 / 25 to 26 / 10.9; two rows 11.2 / 36 / 10.9 and 12.1 / 38 / 12.  So eight where one row has more workgroups than two
 // a CU, else 16.  Four blocks in flight: eight wavefronts 9.8 / 33 / 10.4, 16 12.6 and 9.5.
 constexpr int kLineBlocks = 64;  // blocks of x in LDS at a time
 
