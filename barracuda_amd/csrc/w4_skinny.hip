@@ -164,14 +164,25 @@ __global__ __launch_bounds__(THREADS) void w4_line_kernel(W4 w, const float* __r
 #pragma unroll
     for (int v = 0; v < kOf; ++v) sum += part[v][kb][r];
   }
-  if (__any(!(fabsf(sum) < INFINITY))) {  // of a row of finite inputs: lost before the scale
-#pragma unroll
+  if (__any(!(fabsf(sum) < INFINITY))) {
+#pragma unroll 1
     for (int u = 0; u < MT; ++u) {
+      const bool lost = kb == u && !(fabsf(sum) < INFINITY);
+      if (!__any(lost)) continue;
+      // lost before the scale, if the row's inputs are finite (a row with one that is not: 11 us instead of 9, two 15 instead of 11)
+      const float* row = x + u * ldx;
       bool finite = true;
-      for (int i = lane; i < w.k; i += 64) finite = finite && fabsf(x[u * ldx + i]) < INFINITY;
+#pragma unroll 1
+      for (unsigned i = lane; i < (unsigned)w.k; i += 64 * 8) {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = row[min(i + 64 * e, (unsigned)w.k - 1)];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) finite &= fabsf(v[e]) < INFINITY;
+      }
       if (!__all(finite)) continue;
-      const float again = ldexpf(line_again(w, codes, scales, zeros, x + u * ldx, vec, 0, w.blocks, 1), kDown);
-      if (kb == u && !(fabsf(sum) < INFINITY)) sum = again;
+      const float again = ldexpf(line_again(w, codes, scales, zeros, row, vec, 0, w.blocks, 1), kDown);
+      if (lost) sum = again;
     }
   }
   if (on) {

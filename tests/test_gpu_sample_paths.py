@@ -115,3 +115,21 @@ def test_rules_with_and_without_a_workspace(dev, monkeypatch, vocab, kind):
     for i, r in enumerate(rules):
         token, _, near = choose(x[i], u[i], r.temperature, r.top_k, r.top_p, r.min_p)
         assert a[i] == token or near <= slack(x[i], r.temperature)
+
+
+@pytest.mark.parametrize("mask", [-1e9, -65504.0, np.finfo(np.float32).min])
+@pytest.mark.parametrize("vocab,n", [(600, 5), (9000, 40), (50021, 300), (50021, 5000)])
+def test_masks_of_finite_numbers(dev, monkeypatch, vocab, n, mask):
+    """A mask by a type's lowest number instead of -inf: masked tokens weigh nothing, but a top_k beyond the others takes them in."""
+    rng = np.random.default_rng(n)
+    rules = RULES + MANY
+    x = np.full((len(rules), vocab), mask, np.float32)
+    for r in x:
+        r[rng.permutation(vocab)[:n]] = 2 * rng.standard_normal(n, dtype=np.float32)
+    u = rng.random(len(rules), dtype=np.float32)
+    (a, pa), (b, pb) = both(dev, monkeypatch, x, u, rules)
+    assert np.array_equal(a, b) and np.array_equal(pa, pb)
+    for i, r in enumerate(rules):
+        token, p, near = choose(x[i], u[i], r.temperature, r.top_k, r.top_p, r.min_p)
+        if near > slack(x[i], r.temperature):
+            assert a[i] == token and abs(pa[i] - p) <= 2.0**-24 * p + 2 * slack(x[i], r.temperature), (i, r)

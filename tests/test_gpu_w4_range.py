@@ -71,3 +71,22 @@ def test_scales_of_any_magnitude(dev, m, k, group, x_log, scale_log):
     assert np.abs(want).max() < 2.0**127
     got = linear4(_t(x, dev), Weights4(c, s, k, group, z, dev)).to_numpy()
     assert np.all(np.abs(got - want) <= slack(x, w) + 2.0**-149 * (3 * k))
+
+
+@pytest.mark.parametrize("k", [96, 9000])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_two_rows_of_which_one_is_not_finite(dev, k, bad):
+    """What is lost before the scale is computed again in a row of finite inputs, whatever the other row holds."""
+    rng = np.random.default_rng(4)
+    n, group = 40, 32
+    c, s, z = weights(rng, n, k, group, True)
+    s *= np.float32(0.01)
+    w = wide(c, s, group, k, z)
+    for at in (0, 1):
+        x = rng.standard_normal((2, k), dtype=np.float32)
+        x[at, k // 2], x[1 - at, 5] = bad, 3e38
+        got = linear4(_t(x, dev), Weights4(c, s, k, group, z, dev)).to_numpy()
+        y = x[1 - at].astype(np.float64) @ w.T
+        assert np.all(np.abs(got[1 - at] - y) <= slack(x[1 - at:2 - at], w)[0])
+        with np.errstate(invalid="ignore"):
+            assert np.array_equal(got[at], (np.float32(bad) * w[:, k // 2]).astype(np.float32), equal_nan=True)
