@@ -419,7 +419,7 @@ __device__ __forceinline__ Record weigh_span(const SampleCall& c, const float* r
   for (int e = 0; e < 8; ++e) mine = max(mine, key_of(x[e]));
   Record q{};
   q.top = key_of(bch::wave_allreduce(logit_of(mine), bch::OpMax()));
-  if (q.top != kNothing) q.weight = weigh<false>(c, rule, x, q.top);
+  if (q.top != kNothing) q.weight = weigh<true>(c, rule, x, q.top);
   return q;
 }
 // A span's weight against the row's largest logit, in units of 2^-kSpanUnit.
@@ -1261,7 +1261,7 @@ __global__ __launch_bounds__(kThreads) void sample_binned_kernel(SampleCall c, i
                 left[r].whole);
 }
 
-// All of it for a row of up to kWaves spans, or, where there is no room for records, for a row of any length by general_row.
+// All of it for a row of up to kWaves spans.
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int spans) {
   __shared__ Work work;
   __shared__ Common common;
@@ -1271,22 +1271,29 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int 
   const long long r = blockIdx.x;
   const float* row = c.logits + r * c.stride;
   const SampleRule rule = c.rules ? c.rules[r] : c.rule;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  if (spans <= kWaves) {
-    if (wave < spans) list_span<false>(c, row, rule, spans, wave, &records[wave], &lists[wave * kListMost]);
-    __syncthreads();
-    unsigned top;
-    double whole;
-    if (choose(work, common, c, r, rule, spans, records, lists, top, whole)) return;
-    const Scale sc = scale_of(c, rule, logit_of(top));
-    if (binned(rule, c.vocab)) {
-      bin_chunk(lists, c, row, sc, 0);
-      choose_binned(work, common, c, r, rule, sc, lists, whole);
-    } else {
-      general_row(work.general, common.sums, c, r, rule, sc, whole);
-    }
-    return;
+  const int wave = threadIdx.x >> 6;
+  if (wave < spans) list_span<false>(c, row, rule, spans, wave, &records[wave], &lists[wave * kListMost]);
+  __syncthreads();
+  unsigned top;
+  double whole;
+  if (choose(work, common, c, r, rule, spans, records, lists, top, whole)) return;
+  const Scale sc = scale_of(c, rule, logit_of(top));
+  if (binned(rule, c.vocab)) {
+    bin_chunk(lists, c, row, sc, 0);
+    choose_binned(work, common, c, r, rule, sc, lists, whole);
+  } else {
+    general_row(work.general, common.sums, c, r, rule, sc, whole);
   }
+}
+
+// A row of any length where there is no room for records.
+__global__ __launch_bounds__(kThreads) void sample_whole_kernel(SampleCall c, int spans) {
+  __shared__ General general;
+  __shared__ Common common;
+  const long long r = blockIdx.x;
+  const float* row = c.logits + r * c.stride;
+  const SampleRule rule = c.rules ? c.rules[r] : c.rule;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // the largest logit, of equal ones the lowest index
   u64 top = 0;
   for (int i = threadIdx.x; i < c.vocab; i += kThreads)
@@ -1310,7 +1317,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleCall c, int 
     return;
   }
   const double whole = !count_cut && weight_cut ? row_weight<false>(common, c, row, rule, sc, spans, nullptr) : 0.0;
-  general_row(work.general, common.sums, c, r, rule, sc, whole);
+  general_row(general, common.sums, c, r, rule, sc, whole);
 }
 
 }  // namespace
@@ -1375,8 +1382,10 @@ hipError_t launch_sample(hipStream_t s, const SampleCall& call, int rows, void* 
         if ((e = hipGetLastError()) != hipSuccess) return e;
         hipLaunchKernelGGL(sample_binned_kernel, dim3(n), dim3(kThreads), 0, s, c, chunks, left, hists);
       }
-    } else {
+    } else if (spans <= kWaves) {
       hipLaunchKernelGGL(sample_row_kernel, dim3(n), dim3(kThreads), 0, s, c, spans);
+    } else {
+      hipLaunchKernelGGL(sample_whole_kernel, dim3(n), dim3(kThreads), 0, s, c, spans);
     }
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
